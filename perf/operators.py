@@ -112,7 +112,8 @@ def _codes(x):
     fine = torch.isfinite(xg).all(-1, keepdim=True)
     xc = xg.clamp(-LIM, LIM)
     lo, hi = xc.amin(-1, keepdim=True), xc.amax(-1, keepdim=True)
-    S = torch.maximum((hi - lo) * 16.0 / 15.0, lo.abs() / 128.0).half()
+    # a tensor divisor: torch multiplies by the reciprocal of a number
+    S = torch.maximum((hi - lo) * 16.0 / torch.full_like(lo, 15.0), lo.abs() / 128.0).half()
     Z = (lo - S.float()).half()
     t = torch.where(S > 0, (xc - Z.float()) / S.float() * 16.0, torch.full_like(xc, 16.0))
     c = (t.round() - 16.0).clamp(0.0, 15.0)
@@ -300,7 +301,7 @@ def _exact_group(x):
     f = x.float().reshape(x.shape[:-1] + (x.shape[-1] // 32, 32))
     f = torch.minimum(torch.maximum(f, f.new_tensor(-LIM)), f.new_tensor(LIM))
     lo = f.min(-1, keepdim=True).values
-    step16 = torch.maximum((f.max(-1, keepdim=True).values - lo) * 16 / 15, lo.abs() * 2.0 ** -7).to(torch.float16)
+    step16 = torch.maximum((f.max(-1, keepdim=True).values - lo) * 16 / torch.full_like(lo, 15), lo.abs() * 2.0 ** -7).to(torch.float16)
     zero = (lo - step16.float()).to(torch.float16)
     ratio = torch.nan_to_num((f - zero.float()) / step16.float(), nan=1.0, posinf=1.0, neginf=1.0)
     code = torch.clamp(torch.round(ratio * 16) - 16, 0, 15).double()
