@@ -187,7 +187,7 @@ def prepare(case, seed):
         k, v = _heads(g, NKV, HD, n), torch.randn((n, NKV, HD), device=DEV, generator=g)
         return {"case": c, "q": q.to(_dtype(c["x"])), "cache": _pack(k, v), "state": state}
     qkv = torch.cat([_heads(g, NH, HD, T), _heads(g, NKV, HD, T), torch.randn((T, NKV, HD), device=DEV, generator=g)], 1)
-    cos, sin = _tables(HD, n)
+    cos, sin = _tables(HD, n if c["cache"] == "f32" else (n + 31) // 32 * 32)  # a row per position of the cache
     st = {"case": c, "qkv": qkv.reshape(T, -1).to(_dtype(c["x"])), "state": state, "cos": cos, "sin": sin, "qn": None, "kn": None}
     if c["norm"]:
         st["qn"], st["kn"] = (1.0 + 0.2 * torch.randn(HD, device=DEV, generator=g) for _ in range(2))
