@@ -370,6 +370,73 @@ int miq_attention_decode(const float* qkv, const int32_t* state, const float* co
 int miq_attention(const float* q, const float* kcache, const float* vcache, const int32_t* state,
                   float* out, int T, int NH, int NKV, int HD, int LMAX, float scale, void* stream);
 
+/* QK-norm, RoPE and the cache write in one launch: miq_head_rmsnorm (a null weight leaves its part
+ * alone) followed by miq_rope_kv, bit for bit, with qkv left as it is. Rows lie ld >= (NH + 2 NKV) HD values
+ * apart. A position below 0 or from LMAX on writes nothing to the caches and zeros to its row of q_out.
+ * HD even, <= 256.
+ * Replaces: `self._rms(q, lay["qn"])`, `self._rms(k, lay["kn"])` and `_rope_np` of `CausalLM._qkv`
+ * with `kv_write` (webtorch/llm.py:1498-1519, 1259-1304; webtorch/_core.py:1504-1540). */
+int miq_qk_norm_rope_kv(const float* qkv, int64_t ld, const float* qn, const float* kn, float eps,
+                        const int32_t* state, const float* cos_tab, const float* sin_tab, float* q_out,
+                        float* kcache, float* vcache, int T, int NH, int NKV, int HD, int LMAX, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * The 4-bit key-value cache: miq_kv4_cache_bytes bytes per layer, 16-byte aligned, NKV x ceil(LMAX / 32)
+ * records of 40 HD bytes (5 bits a value), HD 64, 128, 192 or 256. A group of 32 consecutive dimensions
+ * of one position's key (or value) row has two fp16 numbers S and Z, and a code c in 0 .. 15 stands for
+ * fp16(S (1 + c / 16) + Z), rounded once:
+ *   x clamped to +-16384, lo and hi the group's least and largest value;
+ *   S = fp16(max((hi - lo) 16 / 15, |lo| / 128)), Z = fp16(lo - S);
+ *   c = rint((x - Z) / S 16) - 16 clamped to 0 .. 15 (0 where S = 0), each operation rounded to fp32.
+ * A group with a NaN or an infinity reads as NaN. A record holds 32 positions: the key codes (16 HD
+ * bytes), the value codes (16 HD), (S, Z) of the keys [position][group], and of the values [group][g]
+ * [S of 8 positions, Z of 8 positions]. A 32-bit word has 8 codes, number e at bits 4 (e / 2) + 16 (e % 2):
+ * dimensions 32 j + 8 g + e of the key of position 16 b + i, or dimension 16 t + i of the values of
+ * positions 16 (e / 4) + 4 g + e % 4; words lie as [n / 4][g][i][n % 4] with n = b HD / 32 + j for the
+ * keys, n = t for the values (i < 16, g < 4). The reference keeps its cache in fp32
+ * (`KVCache`, webtorch/_core.py:1543-1596).
+ * ------------------------------------------------------------------------------------- */
+int miq_kv4_cache_bytes(int NKV, int LMAX, int HD, size_t* bytes);
+
+/* miq_qk_norm_rope_kv into a 4-bit cache: qkv and q_out fp32 or fp16 (x_dtype); q and k are computed in
+ * fp64 and rounded once (to q_out's type; to fp32 for the cache), v enters as it is. A word's other
+ * positions keep their codes. */
+int miq_qk_norm_rope_kv4(const void* qkv, int x_dtype, int64_t ld, const float* qn, const float* kn, float eps,
+                         const int32_t* state, const float* cos_tab, const float* sin_tab, void* q_out, void* cache,
+                         int T, int NH, int NKV, int HD, int LMAX, void* stream);
+
+/* What positions start .. start + n - 1 of a 4-bit cache stand for: k_out and v_out fp32 [NKV][n][HD]
+ * (either may be null). */
+int miq_kv4_dequant_f32(const void* cache, float* k_out, float* v_out, int NKV, int LMAX, int HD, int start, int n,
+                        void* stream);
+
+/* miq_attention over a 4-bit cache: q and out [T][NH][HD] fp32 or fp16 (x_dtype); token t of head h
+ * attends to positions 0 .. min(state[0] + t, LMAX - 1) of kv head h / (NH / NKV); a token whose
+ * position is below 0 attends to nothing and gets zeros. fp32 q and the probabilities enter the fp16 matrix
+ * cores as two numbers each (22 bits); fp16 rows take one. A value that reads as NaN reaches
+ * exactly the tokens that attend to it, and what positions behind the last one hold does not matter.
+ * workspace: as miq_gptq_gemv's (counters zero before the first call and left zero; not shared by calls
+ * that run concurrently; null where miq_attention_kv4_workspace says 0). Results do not depend on the order of
+ * arrival. LMAX up to 2^30. */
+int miq_attention_kv4_workspace(int T, int NH, int NKV, int HD, int LMAX, size_t* bytes);
+int miq_attention_kv4(const void* q, int x_dtype, const void* cache, const int32_t* state, void* out, int T, int NH,
+                      int NKV, int HD, int LMAX, float scale, void* workspace, size_t ws_bytes, void* stream);
+
+/* Log probabilities of given tokens: for each of T rows of V logits (fp32 or fp16, ld >= V values apart)
+ *   logprobs[t] = x[ids[t]] - log sum exp x (0 for an id outside 0 .. V - 1, and rank -1),
+ *   entropy[t] = -sum p log p (nats), ranks[t] = the number of logits above x[ids[t]],
+ *   top_ids / top_logprobs [t][k]: the k largest logits, of equal ones the lower index first.
+ * Any output may be null. -inf logits are tokens of probability 0; a row of nothing else has log probabilities
+ * -inf and entropy 0; a row with NaN or +inf has NaN log probabilities and entropy (NaN counts as -inf in the
+ * order of alternatives). k <= 32. With a decode state (T = 1, after miq_argmax_advance) the results go
+ * to row state[1] - 1 of the outputs, the token just generated; rows from out_rows on are dropped. workspace as
+ * for miq_attention_kv4.
+ * Replaces: the host's reading of the logits after `_head_argmax` (webtorch/llm.py:1309-1336). */
+int miq_token_logprobs_workspace(int T, int V, int k, size_t* bytes);
+int miq_token_logprobs(const void* logits, int x_dtype, int64_t ld, const int32_t* ids, int T, int V, int k,
+                       float* logprobs, float* entropy, int32_t* ranks, int32_t* top_ids, float* top_logprobs,
+                       const int32_t* state, int out_rows, void* workspace, size_t ws_bytes, void* stream);
+
 /* out[t][i] = silu(gu[t][i]) * gu[t][I + i] for the fused gate|up rows.
  * Replaces: `silu(gate(x)) * up(x)` of `CausalLM._mlp` (webtorch/llm.py:1489-1496,
  * webtorch/_core.py:503-504). */

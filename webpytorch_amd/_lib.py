@@ -55,6 +55,14 @@ SIGNATURES = {
     "miq_rope_kv": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p],
     "miq_attention_decode": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _f, _p],
     "miq_attention": [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p],
+    "miq_qk_norm_rope_kv": [_p, _i64, _p, _p, _f] + [_p] * 6 + [_i] * 5 + [_p],
+    "miq_kv4_cache_bytes": [_i, _i, _i, _p],
+    "miq_qk_norm_rope_kv4": [_p, _i, _i64, _p, _p, _f] + [_p] * 5 + [_i] * 5 + [_p],
+    "miq_kv4_dequant_f32": [_p, _p, _p, _i, _i, _i, _i, _i, _p],
+    "miq_attention_kv4_workspace": [_i, _i, _i, _i, _i, _p],
+    "miq_attention_kv4": [_p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p, _sz, _p],
+    "miq_token_logprobs_workspace": [_i, _i, _i, _p],
+    "miq_token_logprobs": [_p, _i, _i64, _p, _i, _i, _i] + [_p] * 6 + [_i, _p, _sz, _p],
     "miq_silu_mul": [_p, _p, _i, _i, _p],
     "miq_add": [_p, _p, _i64, _p],
     "miq_argmax_advance": [_p, _i, _p, _p, _i, _p, _i, _p],

@@ -10,7 +10,9 @@ Tensors may be given as numpy arrays (uploaded once, at construction) or torch t
 weight layouts are the reference's: qweight int32 (K/per, N), qzeros int32 (K/gs, N/per),
 scales (K/gs, N), Q4_K rows of 144-byte super-blocks.
 """
+import collections
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -861,3 +863,198 @@ def moe_mlp(lm, lay, x):
             se = m["_shared"] = SharedExpert(m["shared"], m.get("shared_gate"))
         se.add_to(out, xt.reshape(T, -1))
     return out
+
+
+# ---- decoder operators: QK-norm + RoPE + cache write, the 4-bit cache, log probabilities ----
+KV4_BLOCK = 32       # positions of one record of a 4-bit cache
+KV4_HEADS = (64, 128, 192, 256)
+MAX_TOP_LOGPROBS = 32
+# a captured call's own workspace: counters this many bytes long are cleared (the library's split
+# attention uses fewer than 256 of 128 bytes, its split logits rows fewer than 1024)
+_CAPTURED_COUNTERS = 1 << 17
+
+
+def _gpu_tensor(name, t, dtypes, dim=None):
+    """Refuse what a kernel would read wrongly: no torch tensor of the current GPU, another dtype or rank."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError("%s must be a torch tensor on the GPU" % name)
+    if t.dtype not in dtypes:
+        raise TypeError("%s has dtype %s (%s)" % (name, t.dtype, " or ".join(str(d).replace("torch.", "") for d in dtypes)))
+    if dim is not None and t.dim() != dim:
+        raise ValueError("%s has shape %s: %d dimensions are expected" % (name, tuple(t.shape), dim))
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError("%s is on cuda:%d, the current device is cuda:%d" % (name, t.get_device(), torch.cuda.current_device()))
+
+
+def _call_workspace(nbytes):
+    """The workspace of one call: the stream's, or, under graph capture, one of the graph's own, so that two
+    graphs replayed at a time never share one."""
+    if nbytes == 0:
+        return None
+    if not torch.cuda.is_current_stream_capturing():
+        return workspace(nbytes)
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device())
+    t[:_CAPTURED_COUNTERS].zero_()
+    return t
+
+
+def _bytes(key, name, *args):
+    b = _WS_BYTES.get(key)
+    if b is None:
+        n = ctypes.c_size_t(0)
+        _lib.call(name, *args, ctypes.byref(n))
+        b = _WS_BYTES[key] = int(n.value)
+    return b
+
+
+def attention_kv4_workspace_bytes(T, NH, NKV, HD, LMAX):
+    """Bytes of workspace `miq_attention_kv4` needs (cached per shape)."""
+    return _bytes(("kv4", T, NH, NKV, HD, LMAX), "miq_attention_kv4_workspace", T, NH, NKV, HD, LMAX)
+
+
+def token_logprobs_workspace_bytes(T, V, k):
+    """Bytes of workspace `miq_token_logprobs` needs (cached per shape)."""
+    return _bytes(("logprobs", T, V, k), "miq_token_logprobs_workspace", T, V, k)
+
+
+def kv4_cache(nkv, lmax, hd):
+    """An empty 4-bit key-value cache of one layer: uint8 (nkv, ceil(lmax / 32), 40 hd), zeros. 5 bits a
+    value: groups of 32 dimensions share a scale and an offset (`include/miq.h` has the layout)."""
+    if hd not in KV4_HEADS:
+        raise NotImplementedError("a 4-bit cache holds heads of 64, 128, 192 or 256 dimensions, not %d" % hd)
+    if nkv < 1 or lmax < 1:
+        raise ValueError("kv4_cache: nkv=%d lmax=%d" % (nkv, lmax))
+    return torch.zeros((nkv, -(-lmax // KV4_BLOCK), 40 * hd), dtype=torch.uint8, device=device())
+
+
+def _kv4_shape(cache):
+    """(NKV, positions, HD) of a 4-bit cache tensor."""
+    _gpu_tensor("the 4-bit cache", cache, (torch.uint8,), 3)
+    nkv, nb, rec = cache.shape
+    if rec % 40 or rec // 40 not in KV4_HEADS or nb < 1 or nkv < 1 or not cache.is_contiguous():
+        raise ValueError("a 4-bit cache is a contiguous (NKV, blocks, 40 HD) tensor, HD 64, 128, 192 or 256: got %s"
+                         % (tuple(cache.shape),))
+    return nkv, nb * KV4_BLOCK, rec // 40
+
+
+def kv4_dequant(cache, start=0, n=None):
+    """The fp32 keys and values (NKV, n, HD) that positions start .. start + n - 1 of a 4-bit cache stand for."""
+    nkv, lmax, hd = _kv4_shape(cache)
+    n = lmax - start if n is None else n
+    if start < 0 or n < 0 or start + n > lmax:
+        raise ValueError("positions %d .. %d of a cache of %d" % (start, start + n - 1, lmax))
+    k, v = (torch.empty((nkv, n, hd), dtype=torch.float32, device=cache.device) for _ in range(2))
+    _lib.call("miq_kv4_dequant_f32", cache.data_ptr(), k.data_ptr(), v.data_ptr(), nkv, lmax, hd, start, n, stream_handle())
+    return k, v
+
+
+def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-6, out=None):
+    """One pass over the fused q|k|v rows `qkv` (T, (NH + 2 NKV) HD) of the tokens at positions state[0] ..:
+    RMSNorm of each query and key head by `qn` / `kn` (fp32 (HD,); None: no norm), rotate-half RoPE with
+    the fp32 tables `cos` / `sin` (positions, HD / 2), and k and v written into `cache`: a pair of fp32
+    caches (NKV, LMAX, HD), or a 4-bit cache (`kv4_cache`). Returns q (T, NH, HD) in qkv's dtype. With fp32
+    caches qkv is fp32, and the results are those of the library's separate norm and RoPE. Rows whose position
+    is outside the cache write nothing, and their q is zero. (`CausalLM._qkv`, `_rope_np`, `kv_write`:
+    `webtorch/llm.py:1498-1519, 1270-1304`, `webtorch/_core.py:1504-1540`.)"""
+    four = isinstance(cache, torch.Tensor)
+    f32 = (torch.float32,)
+    _gpu_tensor("qkv", qkv, (torch.float32, torch.float16) if four else f32, 2)
+    _gpu_tensor("state", state, (torch.int32,))
+    if four:
+        nkv, lmax, hd = _kv4_shape(cache)
+    else:
+        kc, vc = cache
+        for t in (kc, vc):
+            _gpu_tensor("the cache", t, f32, 3)
+        nkv, lmax, hd = kc.shape
+        if vc.shape != kc.shape or not kc.is_contiguous() or not vc.is_contiguous():
+            raise ValueError("the caches are two contiguous (NKV, LMAX, HD) tensors: got %s and %s" % (tuple(kc.shape), tuple(vc.shape)))
+    T, W = qkv.shape
+    if n_heads < 1 or n_heads % nkv or W != (n_heads + 2 * nkv) * hd:
+        raise ValueError("rows of %d values are not %d query, %d key and %d value heads of %d" % (W, n_heads, nkv, nkv, hd))
+    for name, t in (("cos", cos), ("sin", sin)):
+        _gpu_tensor(name, t, f32, 2)
+        if t.shape[1] * 2 != hd or t.shape[0] < lmax or not t.is_contiguous():
+            raise ValueError("%s is a contiguous (positions, %d) table of at least %d positions: got %s" % (name, hd // 2, lmax, tuple(t.shape)))
+    for name, t in (("qn", qn), ("kn", kn)):
+        if t is not None:
+            _gpu_tensor(name, t, f32, 1)
+            if t.shape[0] != hd or not t.is_contiguous():
+                raise ValueError("%s has shape %s: (%d,) is expected" % (name, tuple(t.shape), hd))
+    if state.numel() < 1:
+        raise ValueError("state is empty")
+    if qkv.stride(1) != 1 or (T > 1 and qkv.stride(0) < W):
+        qkv = qkv.contiguous()
+    if out is None:
+        out = torch.empty((T, n_heads, hd), dtype=qkv.dtype, device=qkv.device)
+    else:
+        _gpu_tensor("out", out, (qkv.dtype,))
+        if out.numel() != T * n_heads * hd or not out.is_contiguous():
+            raise ValueError("out is a contiguous tensor of %d values: got %s" % (T * n_heads * hd, tuple(out.shape)))
+    ld = qkv.stride(0) if T > 1 else W
+    qp, kp = (None if t is None else t.data_ptr() for t in (qn, kn))
+    if four:
+        _lib.call("miq_qk_norm_rope_kv4", qkv.data_ptr(), dtype_code(qkv), ld, qp, kp, float(eps), state.data_ptr(), cos.data_ptr(),
+                  sin.data_ptr(), out.data_ptr(), cache.data_ptr(), T, n_heads, nkv, hd, lmax, stream_handle())
+    else:
+        _lib.call("miq_qk_norm_rope_kv", qkv.data_ptr(), ld, qp, kp, float(eps), state.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                  out.data_ptr(), kc.data_ptr(), vc.data_ptr(), T, n_heads, nkv, hd, lmax, stream_handle())
+    return out
+
+
+def attention_kv4(q, cache, state, scale=None, out=None, ws=None):
+    """Causal grouped-query attention of q (T, NH, HD), fp32 or fp16, over a 4-bit cache: token t, at
+    position state[0] + t, attends to positions 0 .. state[0] + t; scale is 1 / sqrt(HD) unless given. A token
+    whose position is below 0 gets zeros. Returns (T, NH, HD) in q's dtype. (`KVCache.attn`, `gqa_attention`:
+    `webtorch/_core.py:1543-1596, 1319-1340`, which keep the cache in fp32.)"""
+    _gpu_tensor("q", q, (torch.float32, torch.float16), 3)
+    _gpu_tensor("state", state, (torch.int32,))
+    nkv, lmax, hd = _kv4_shape(cache)
+    T, nh, qd = q.shape
+    if qd != hd or nh < 1 or nh % nkv or state.numel() < 1:
+        raise ValueError("q %s does not go with a cache of %d heads of %d" % (tuple(q.shape), nkv, hd))
+    q = q.contiguous()
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _gpu_tensor("out", out, (q.dtype,))
+        if out.numel() != q.numel() or not out.is_contiguous():
+            raise ValueError("out is a contiguous tensor of %d values: got %s" % (q.numel(), tuple(out.shape)))
+    if ws is None:
+        ws = _call_workspace(attention_kv4_workspace_bytes(T, nh, nkv, hd, lmax))
+    _lib.call("miq_attention_kv4", q.data_ptr(), dtype_code(q), cache.data_ptr(), state.data_ptr(), out.data_ptr(), T, nh, nkv, hd, lmax,
+              1.0 / math.sqrt(hd) if scale is None else float(scale), None if ws is None else ws.data_ptr(),
+              0 if ws is None else ws.numel(), stream_handle())
+    return out
+
+
+TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs entropy ranks top_ids top_logprobs")
+
+
+def token_logprobs(logits, ids, top_k=0):
+    """Log probabilities of given tokens: `logits` (T, V) fp32 or fp16 (rows may lie further apart), `ids`
+    (T,) int32 or int64. Returns TokenLogprobs of logprobs, entropy (nats) and ranks (how many tokens are
+    likelier), each (T,), and the top_k <= 32 likeliest tokens, top_ids and top_logprobs (T, top_k), of
+    equal ones the lower id first. An id outside the vocabulary has log probability 0 and rank -1; logits of
+    -inf are tokens of probability 0."""
+    _gpu_tensor("logits", logits, (torch.float32, torch.float16), 2)
+    _gpu_tensor("ids", ids, (torch.int32, torch.int64), 1)
+    T, V = logits.shape
+    if ids.shape[0] != T:
+        raise ValueError("%d ids for %d rows of logits" % (ids.shape[0], T))
+    if not 0 <= top_k <= min(V, MAX_TOP_LOGPROBS):
+        raise ValueError("top_k=%d (0 .. %d)" % (top_k, min(V, MAX_TOP_LOGPROBS)))
+    if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    if ids.dtype != torch.int32:
+        ids = ids.clamp(-1, 0x7FFFFFFF).to(torch.int32)
+    ids = ids.contiguous()
+    r = TokenLogprobs(*(torch.empty(s, dtype=d, device=logits.device) for s, d in (
+        (T, torch.float32), (T, torch.float32), (T, torch.int32), ((T, top_k), torch.int32), ((T, top_k), torch.float32))))
+    for t0 in range(0, T, 65535):  # rows of one launch
+        n = min(T - t0, 65535)
+        ws = _call_workspace(token_logprobs_workspace_bytes(n, V, top_k))
+        _lib.call("miq_token_logprobs", logits[t0:].data_ptr(), dtype_code(logits), logits.stride(0) if T > 1 else V,
+                  ids[t0:].data_ptr(), n, V, top_k, *(x[t0:].data_ptr() for x in r), None, n,
+                  None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream_handle())
+    return r
