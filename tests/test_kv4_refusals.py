@@ -83,3 +83,9 @@ def test_tensors_off_the_gpu_are_refused():
         core.qk_norm_rope(z(1, 256), z(1, dtype=torch.int32), z(8, 32), z(8, 32), 2, (z(1, 8, 64), z(1, 8, 64)))
     with pytest.raises(NotImplementedError, match="not 80"):
         core.kv4_cache(1, 8, 80)
+
+
+def test_context_length_of_a_four_bit_cache():
+    from webpytorch_amd import checkpoint
+    assert checkpoint.auto_lmax(None, 10 ** 7, 24, 2, 64, 4) == (2 << 30) // (2 * 24 * 2 * 64 * 5 // 8)
+    assert checkpoint.auto_lmax(None, 4096, 24, 2, 64, 4) == 4096

@@ -137,12 +137,13 @@ def _text_config(cfg):
 KV_BUDGET = 2 << 30  # bytes of fp32 K and V cache the automatic context length may take
 
 
-def auto_lmax(requested, declared, L, NKV, HD):
+def auto_lmax(requested, declared, L, NKV, HD, kv_bits=None):
     """Context length to load with (`webtorch/llm.py:1381-1395`): an explicit request, else what
-    the model declares (2048 if nothing), capped by the KV-cache budget, at least 512."""
+    the model declares (2048 if nothing), capped by the KV-cache budget, at least 512. A 4-bit
+    cache takes 5 bits a value."""
     if requested:
         return int(requested)
-    per_tok = 2 * L * NKV * HD * 4
+    per_tok = 2 * L * NKV * HD * (5 if kv_bits == 4 else 32) // 8
     cap = max(512, KV_BUDGET // per_tok)
     want = int(declared) if declared else 2048
     return max(512, min(want, cap))

@@ -40,13 +40,15 @@ from .core import ptr, stream_handle
 
 
 class GenResult:
-    """Result of `generate` (`webtorch/llm.py:273-279`)."""
+    """Result of `generate` (`webtorch/llm.py:273-279`); `logprobs` is a `core.TokenLogprobs` of the
+    generated tokens where they were asked for, else None."""
 
-    def __init__(self, text, tokens, ttft_s, decode_tok_s):
+    def __init__(self, text, tokens, ttft_s, decode_tok_s, logprobs=None):
         self.text = text
         self.tokens = tokens
         self.ttft_s = ttft_s
         self.decode_tok_s = decode_tok_s
+        self.logprobs = logprobs
 
     def __repr__(self):
         return "GenResult(ttft=%.4fs, %.1f tok/s, %d tokens)" % (self.ttft_s, self.decode_tok_s, len(self.tokens))
@@ -175,10 +177,20 @@ class CausalLM:
     "in_ln", "post_ln"), the fp16 "embed" table, optionally an fp16 "head" (V, H) for an untied
     model (else the head is tied to the embedding), "final_norm" and "cfg"
     (L, H, NH, NKV, HD, I, V, gs, bits[, eps, theta]); or with `CausalLM.from_gptq(path)` from an
-    AutoGPTQ safetensors directory."""
+    AutoGPTQ safetensors directory.
 
-    def __init__(self, weights, lmax=256, fused=True, persistent=None):
+    `kv_bits=4` keeps keys and values in the 4-bit cache (`core.kv4_cache`: 5 bits a value instead of 32, and
+    contexts past the fp32 attention's 16384 positions); the steps are then launch sequences."""
+
+    SCORE_ROWS = 256  # rows of logits that `score` holds at a time
+
+    def __init__(self, weights, lmax=256, fused=True, persistent=None, kv_bits=None):
         c = weights["cfg"]
+        if kv_bits not in (None, 4, 32):
+            raise ValueError("kv_bits must be 4 or 32 (fp32), got %r" % (kv_bits,))
+        self.kv_bits = 4 if kv_bits == 4 else 32
+        if self.kv_bits == 4 and c["HD"] not in core.KV4_HEADS:
+            raise NotImplementedError("a 4-bit cache holds heads of %s dimensions, not %d" % (core.KV4_HEADS, c["HD"]))
         # decode tokens per captured graph: a replay costs ~5 us more than a plain launch of the
         # same kernel, so one graph holds several one-token steps (348.5 against 351.7 us per token
         # for the persistent step of the Qwen2-0.5B shape, eager launches 346.7 us)
@@ -240,25 +252,28 @@ class CausalLM:
         if self.native_gguf or self.padded:
             self.fused = False
         self._alloc()
-        self._graphs = {}  # decode tokens -> captured graph of them
+        self._graphs = {}  # decode tokens (with log probabilities: and alternatives) -> captured graph of them
+        self._lp_rows = {}  # alternatives -> buffers of log probabilities
+        self._lp = None    # the ones that the steps write, or None
         self.fallback_steps = 0  # tokens of the last generate() that a timed-out persistent step left
 
     @classmethod
-    def from_weights(cls, weights, lmax=256, fused=True, persistent=None):
-        return cls(weights, lmax, fused, persistent)
+    def from_weights(cls, weights, lmax=256, fused=True, persistent=None, kv_bits=None):
+        return cls(weights, lmax, fused, persistent, kv_bits)
 
     @classmethod
-    def from_gptq(cls, path, lmax=None, fused=True, persistent=None):
+    def from_gptq(cls, path, lmax=None, fused=True, persistent=None, kv_bits=None):
         """Load an AutoGPTQ safetensors directory (config.json + model.safetensors or an index
         and shards), as the reference's `from_gptq` does (`webtorch/llm.py:614-647`). `lmax=None`
         takes the model's declared context, capped by a 2 GiB KV-cache budget."""
         from . import checkpoint
         w, declared = checkpoint.gptq_weights(path)
         c = w["cfg"]
-        return cls(w, checkpoint.auto_lmax(lmax, declared, c["L"], c["NKV"], c["HD"]), fused, persistent)
+        return cls(w, checkpoint.auto_lmax(lmax, declared, c["L"], c["NKV"], c["HD"], kv_bits), fused, persistent,
+                   kv_bits)
 
     @classmethod
-    def from_fp16(cls, path, lmax=None, quantize=None, fused=True, persistent=None):
+    def from_fp16(cls, path, lmax=None, quantize=None, fused=True, persistent=None, kv_bits=None):
         """Load a plain fp16/bf16 HuggingFace safetensors directory, quantizing every linear to
         int`quantize` (4 or 8) on the device as it loads (`webtorch/llm.py:1221-1257`: group
         size 128, zero offset 0, fp32 scales; the tied head as `_quantize_head`). Unquantized
@@ -269,10 +284,11 @@ class CausalLM:
         from . import checkpoint
         w, declared = checkpoint.fp16_weights(path, int(quantize))
         c = w["cfg"]
-        return cls(w, checkpoint.auto_lmax(lmax, declared, c["L"], c["NKV"], c["HD"]), fused, persistent)
+        return cls(w, checkpoint.auto_lmax(lmax, declared, c["L"], c["NKV"], c["HD"], kv_bits), fused, persistent,
+                   kv_bits)
 
     @classmethod
-    def from_gguf(cls, path, lmax=None, bits=None, weights="native", persistent=None):
+    def from_gguf(cls, path, lmax=None, bits=None, weights="native", persistent=None, kv_bits=None):
         """Load a llama.cpp GGUF decoder (`CausalLM.from_gguf`, `webtorch/llm.py:856-1129`).
         `weights="native"` (the default) keeps every weight whose block type has a kernel here
         in the file's own encoding and runs the unfused launch sequence; "requant" decodes each
@@ -282,7 +298,7 @@ class CausalLM:
         from . import checkpoint
         w, declared = checkpoint.gguf_weights(path, bits, weights)
         c = w["cfg"]
-        return cls(w, checkpoint.auto_lmax(lmax, declared, c["L"], c["NKV"], c["HD"]), True, persistent)
+        return cls(w, checkpoint.auto_lmax(lmax, declared, c["L"], c["NKV"], c["HD"], kv_bits), True, persistent, kv_bits)
 
     # ---- load-time ----
     def _quantize_head(self, head=None):
@@ -304,8 +320,11 @@ class CausalLM:
         if self.has_moe:
             E = max(_lin_n(lay["moe"]["router"]) for lay in self.layers if "moe" in lay)
             self.buf["rlog"] = z(T, E)
-        self.kc = torch.zeros((self.L, self.NKV, self.lmax, self.HD), dtype=f32, device=dev)
-        self.vc = torch.zeros_like(self.kc)
+        if self.kv_bits == 4:
+            self.kv4 = [core.kv4_cache(self.NKV, self.lmax, self.HD) for _ in range(self.L)]
+        else:
+            self.kc = torch.zeros((self.L, self.NKV, self.lmax, self.HD), dtype=f32, device=dev)
+            self.vc = torch.zeros_like(self.kc)
         # RoPE tables exactly as `_rope_np` builds them (float64 angles, rounded once to fp32)
         inv = 1.0 / (self.theta ** (np.arange(0, self.HD, 2, dtype=np.float64) / self.HD))
         ang = np.arange(0, T, dtype=np.float64)[:, None] * inv[None, :]
@@ -333,6 +352,9 @@ class CausalLM:
                 need = max(need, core.gemv_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits, _lib.MIQ_F32))
                 if M > core.GEMV_MAX_M:  # prefill rows on the matrix cores
                     need = max(need, core.gemm_f32x_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits))
+            if self.kv_bits == 4:
+                need = max(need, core.attention_kv4_workspace_bytes(M, self.NH, self.NKV, self.HD, self.lmax))
+        need = max(need, core.token_logprobs_workspace_bytes(1, self.V, min(self.V, core.MAX_TOP_LOGPROBS)))
         self.ws = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=dev)
         self._alloc_persistent()
 
@@ -342,9 +364,9 @@ class CausalLM:
         self.pws = None
         if self.persistent is False or not self.fused:
             return
-        if self.has_moe or self.has_qk_norm:
+        if self.has_moe or self.has_qk_norm or self.kv_bits == 4:
             if self.persistent:
-                raise ValueError("the persistent decode step covers dense layers without QK-norm")
+                raise ValueError("the persistent decode step covers dense layers without QK-norm, with fp32 caches")
             return
         lays = self.layers
         lins = [lay[k] for lay in lays for k in ("qkv", "o", "gate_up", "down")]
@@ -452,9 +474,13 @@ class CausalLM:
         scale = 1.0 / math.sqrt(self.HD)
         for i, lay in enumerate(self.layers):
             self._fused(lay["qkv"], h, _lib.MIQ_X_RMSNORM, lay["in_ln"], b["qkv"])
-            self._qk_norm(lay, 1)
-            _lib.call("miq_attention_decode", ptr(b["qkv"]), ptr(self.state), ptr(self.cos_t), ptr(self.sin_t),
-                      ptr(self.kc[i]), ptr(self.vc[i]), ptr(b["att"]), self.NH, self.NKV, self.HD, self.lmax, scale, st)
+            if self.kv_bits == 4:
+                self._attention(lay, i, 1, scale)
+            else:
+                self._qk_norm(lay, 1)
+                _lib.call("miq_attention_decode", ptr(b["qkv"]), ptr(self.state), ptr(self.cos_t), ptr(self.sin_t),
+                          ptr(self.kc[i]), ptr(self.vc[i]), ptr(b["att"]), self.NH, self.NKV, self.HD, self.lmax, scale,
+                          st)
             self._linear(lay["o"], b["att"][:1], h, bias=h)
             if "moe" in lay:
                 self._moe(lay, h, 1)
@@ -467,22 +493,32 @@ class CausalLM:
 
     def _step(self, T):
         """T tokens (ids[:T]) at positions state[0].. -> next token on the device
-        (`_kv_forward`, `webtorch/llm.py:1619-1636`)."""
+        (`_kv_forward`, `webtorch/llm.py:1619-1636`), and its log probabilities where they are asked for."""
         if T == 1 and self.fused:
-            return self._decode_step()
+            self._decode_step()
+        else:
+            self._layers(T)
+            b, st = self.buf, stream_handle()
+            _lib.call("miq_rmsnorm", ptr(b["h"][T - 1:T]), ptr(self.final_norm), ptr(b["hl"]), 1, self.H, self.eps, st)
+            self._linear(self.head, b["hl"], b["logits"])
+            _lib.call("miq_argmax_advance", ptr(b["logits"]), self.V, ptr(self.ids), ptr(self.history), self.lmax,
+                      ptr(self.state), T, st)
+        if self._lp is not None:
+            _lib.call("miq_token_logprobs", ptr(self.buf["logits"]), _lib.MIQ_F32, self.V, ptr(self.ids), 1, self.V,
+                      int(self._lp.top_ids.shape[1]), *(ptr(t) for t in self._lp), ptr(self.state), self.lmax,
+                      ptr(self.ws), self.ws.numel(), stream_handle())
+
+    def _layers(self, T):
+        """The decoder layers over T tokens (ids[:T]) at positions state[0]..: their rows of buf["h"]."""
         b, st = self.buf, stream_handle()
-        H, NH, NKV, HD, I = self.H, self.NH, self.NKV, self.HD, self.I
+        H, I = self.H, self.I
         h, xn = b["h"][:T], b["xn"][:T]
         self._embed(T)
-        scale = 1.0 / math.sqrt(HD)
+        scale = 1.0 / math.sqrt(self.HD)
         for i, lay in enumerate(self.layers):
             _lib.call("miq_rmsnorm", ptr(h), ptr(lay["in_ln"]), ptr(xn), T, H, self.eps, st)
             self._linear(lay["qkv"], xn, b["qkv"][:T])
-            self._qk_norm(lay, T)
-            _lib.call("miq_rope_kv", ptr(b["qkv"]), ptr(self.state), ptr(self.cos_t), ptr(self.sin_t), ptr(b["q"]),
-                      ptr(self.kc[i]), ptr(self.vc[i]), T, NH, NKV, HD, self.lmax, st)
-            _lib.call("miq_attention", ptr(b["q"]), ptr(self.kc[i]), ptr(self.vc[i]), ptr(self.state), ptr(b["att"]), T,
-                      NH, NKV, HD, self.lmax, scale, st)
+            self._attention(lay, i, T, scale)
             self._residual(lay["o"], b["att"][:T], h, T)
             if "moe" in lay:
                 self._moe(lay, h, T)
@@ -491,14 +527,28 @@ class CausalLM:
             self._linear(lay["gate_up"], xn, b["gu"][:T])
             _lib.call("miq_silu_mul", ptr(b["gu"]), ptr(b["act"]), T, I, st)
             self._residual(lay["down"], b["act"][:T], h, T)
-        _lib.call("miq_rmsnorm", ptr(h[T - 1:T]), ptr(self.final_norm), ptr(b["hl"]), 1, H, self.eps, st)
-        self._linear(self.head, b["hl"], b["logits"])
-        _lib.call("miq_argmax_advance", ptr(b["logits"]), self.V, ptr(self.ids), ptr(self.history), self.lmax,
-                  ptr(self.state), T, st)
+
+    def _attention(self, lay, i, T, scale):
+        """QK-norm, RoPE and the cache write of layer i's T fused q|k|v rows in one launch
+        (`CausalLM._qkv`, `webtorch/llm.py:1498-1519`), then the attention: buf["att"]."""
+        b, st = self.buf, stream_handle()
+        NH, NKV, HD, W = self.NH, self.NKV, self.HD, (self.NH + 2 * self.NKV) * self.HD
+        if self.kv_bits == 4:
+            _lib.call("miq_qk_norm_rope_kv4", ptr(b["qkv"]), _lib.MIQ_F32, W, ptr(lay["qn"]), ptr(lay["kn"]), self.eps,
+                      ptr(self.state), ptr(self.cos_t), ptr(self.sin_t), ptr(b["q"]), ptr(self.kv4[i]), T, NH, NKV, HD,
+                      self.lmax, st)
+            _lib.call("miq_attention_kv4", ptr(b["q"]), _lib.MIQ_F32, ptr(self.kv4[i]), ptr(self.state), ptr(b["att"]), T,
+                      NH, NKV, HD, self.lmax, scale, ptr(self.ws), self.ws.numel(), st)
+            return
+        _lib.call("miq_qk_norm_rope_kv", ptr(b["qkv"]), W, ptr(lay["qn"]), ptr(lay["kn"]), self.eps, ptr(self.state),
+                  ptr(self.cos_t), ptr(self.sin_t), ptr(b["q"]), ptr(self.kc[i]), ptr(self.vc[i]), T, NH, NKV, HD, self.lmax,
+                  st)
+        _lib.call("miq_attention", ptr(b["q"]), ptr(self.kc[i]), ptr(self.vc[i]), ptr(self.state), ptr(b["att"]), T,
+                  NH, NKV, HD, self.lmax, scale, st)
 
     def _qk_norm(self, lay, T):
-        """Per-head RMSNorm of q and k in the fused q|k|v rows, before RoPE (Qwen3's QK-norm,
-        `CausalLM._qkv`, `webtorch/llm.py:1498-1519`); nothing for layers without it."""
+        """Per-head RMSNorm of q and k in the fused q|k|v rows, ahead of the one-token attention, which rotates
+        (Qwen3's QK-norm, `CausalLM._qkv`, `webtorch/llm.py:1498-1519`); nothing for layers without it."""
         if lay["qn"] is None and lay["kn"] is None:
             return
         _lib.call("miq_head_rmsnorm", ptr(self.buf["qkv"]), ptr(lay["qn"]), ptr(lay["kn"]), T, self.NH, self.NKV,
@@ -548,12 +598,15 @@ class CausalLM:
         with torch.cuda.graph(g):
             for _ in range(tokens):
                 self._step(1)
-        self._graphs[tokens] = g
+        self._graphs[self._graph_key(tokens)] = g
         return g
+
+    def _graph_key(self, tokens):
+        return tokens if self._lp is None else (tokens, int(self._lp.top_ids.shape[1]))
 
     def graph(self, tokens):
         """The captured graph of `tokens` decode tokens, recorded on first use."""
-        g = self._graphs.get(tokens)
+        g = self._graphs.get(self._graph_key(tokens))
         return g if g is not None else self.capture(tokens)
 
     def _chunks(self, n):
@@ -592,9 +645,11 @@ class CausalLM:
             return 0
         if err & 2:
             raise _lib.MiqError("persistent decode step failed (error bits %d): position past the KV cache" % err)
+        if self._lp is not None:  # the steps after the one that timed out wrote over its predecessor's row
+            return None
         left = max_new - int(self.state[1].item())
         warnings.warn("persistent decode step timed out waiting (another kernel on the GPU?); the remaining %d "
-                      "token(s) run as the launch sequence" % left, RuntimeWarning, stacklevel=3)
+                      "token(s) run as the launch sequence" % left, RuntimeWarning, stacklevel=4)
         pws, self.pws = self.pws, None
         try:
             pws.zero_()
@@ -605,12 +660,53 @@ class CausalLM:
             self.pws = pws
         return left
 
-    def generate(self, ids, max_new, use_graph=True):
+    def _logprob_rows(self, k):
+        """The buffers that steps with k alternatives write, a row per generated token: kept for the captured
+        graphs that hold their addresses."""
+        if not 0 <= k <= min(self.V, core.MAX_TOP_LOGPROBS):
+            raise ValueError("logprobs=%d (0 .. %d alternatives)" % (k, min(self.V, core.MAX_TOP_LOGPROBS)))
+        if k not in self._lp_rows:
+            n, dev = self.lmax, core.device()
+            self._lp_rows[k] = core.TokenLogprobs(*(torch.zeros(s, dtype=d, device=dev) for s, d in (
+                (n, torch.float32), (n, torch.float32), (n, torch.int32), ((n, k), torch.int32), ((n, k), torch.float32))))
+        return self._lp_rows[k]
+
+    def score(self, ids, top_k=0):
+        """Log probabilities of a given text: a `core.TokenLogprobs` with a row per token of ids[1:], each given
+        the tokens before it (with entropy, rank and top_k alternatives). The sequence state is left reset."""
+        ids = [int(i) for i in ids]
+        n = len(ids) - 1
+        if n < 1 or len(ids) > self.lmax:
+            raise ValueError("score takes 2 .. lmax (%d) tokens, got %d" % (self.lmax, len(ids)))
+        self._logprob_rows(top_k)
+        self.reset()
+        self.ids[:n + 1].copy_(torch.tensor(ids, dtype=torch.int32))
+        given = self.ids[1:n + 1].clone()
+        self._layers(n)
+        parts, rows = [], self.SCORE_ROWS
+        logits = torch.empty((min(n, rows), self.V), dtype=torch.float32, device=core.device())
+        for t0 in range(0, n, rows):
+            m = min(rows, n - t0)
+            h = self.buf["h"][t0:t0 + m]
+            _lib.call("miq_rmsnorm", ptr(h), ptr(self.final_norm), ptr(self.buf["xn"]), m, self.H, self.eps, stream_handle())
+            self._linear(self.head, self.buf["xn"][:m], logits[:m])
+            parts.append(core.token_logprobs(logits[:m], given[t0:t0 + m], top_k))
+        return parts[0] if len(parts) == 1 else core.TokenLogprobs(*(torch.cat(p) for p in zip(*parts)))
+
+    def generate(self, ids, max_new, use_graph=True, logprobs=None):
         """Greedy decode with no end token (`webtorch/llm.py:1716-1817` with do_sample off):
         prefill the prompt, then max_new - 1 decode steps. Returns a GenResult whose `tokens`
-        are the max_new generated ids."""
+        are the max_new generated ids. With `logprobs` (0 .. 32 alternatives) its `logprobs` are those of the
+        generated tokens, computed on the device in the same steps."""
         ids = [int(i) for i in ids]
         self._plan_length(len(ids), max_new)
+        self._lp = None if logprobs is None else self._logprob_rows(int(logprobs))
+        try:
+            return self._generate(ids, max_new, use_graph)
+        finally:
+            self._lp = None
+
+    def _generate(self, ids, max_new, use_graph):
         self.reset()
         self.ids[:len(ids)].copy_(torch.tensor(ids, dtype=torch.int32))
         torch.cuda.synchronize()
@@ -626,23 +722,36 @@ class CausalLM:
         if use_graph:
             for t, r in chunks:
                 for _ in range(r):
-                    self._graphs[t].replay()
+                    self._graphs[self._graph_key(t)].replay()
         else:
             for _ in range(max_new - 1):
                 self._step(1)
         torch.cuda.synchronize()
-        self.fallback_steps = self._finish_after_timeout(max_new)
+        left = self._finish_after_timeout(max_new)
+        if left is None:  # the whole sequence again, as the launch sequence
+            warnings.warn("persistent decode step timed out waiting (another kernel on the GPU?); the sequence runs "
+                          "again as the launch sequence", RuntimeWarning, stacklevel=3)
+            pws, self.pws = self.pws, None
+            try:
+                pws.zero_()
+                again = self._generate(ids, max_new, False)
+            finally:
+                self.pws = pws
+            self.fallback_steps = max_new
+            return again
+        self.fallback_steps = left
         dt = time.perf_counter() - t1
         toks = [int(t) for t in self.history[:max_new].cpu().numpy()]
         rate = (max_new - 1) / dt if max_new > 1 and dt > 0 else 0.0
-        return GenResult("", toks, ttft, rate)
+        lp = None if self._lp is None else core.TokenLogprobs(*(t[:max_new].clone() for t in self._lp))
+        return GenResult("", toks, ttft, rate, lp)
 
 
 class AutoModelForCausalLM:
     """Entry point with the reference SDK's signature (`webtorch/_sdk.py:72-115`)."""
 
     @staticmethod
-    def from_pretrained(path, dtype="auto", bits=None, lmax=None, weights="native"):
+    def from_pretrained(path, dtype="auto", bits=None, lmax=None, weights="native", kv_bits=None):
         """Load a decoder for the quantized engine, dispatching on `dtype` as the reference does
         (`AutoModelForCausalLM._load_raw`, `webtorch/_sdk.py:98-115`):
 
@@ -653,7 +762,7 @@ class AutoModelForCausalLM:
         * a `.gguf` file loads through `from_gguf` ("auto" keeps the width the file stores,
           "int4" / "int8" requantize, `bits` overrides, `weights` as in the reference).
 
-        Unquantized execution ("fp16", or "auto" on a plain fp16 directory) is not part of this
+        `kv_bits=4` keeps the KV cache in 4 bits (`CausalLM`). Unquantized execution ("fp16", or "auto" on a plain fp16 directory) is not part of this
         library and raises NotImplementedError. Unlike the reference this call is synchronous
         and does not cache loaded models."""
         p = str(path).rstrip("/")
@@ -663,9 +772,9 @@ class AutoModelForCausalLM:
             if dtype == "fp16":
                 raise NotImplementedError("unquantized fp16 execution is not part of this library")
             gb = 8 if dtype == "int8" else (4 if dtype == "int4" else bits)
-            return CausalLM.from_gguf(p, lmax=lmax, bits=gb, weights=weights)
+            return CausalLM.from_gguf(p, lmax=lmax, bits=gb, weights=weights, kv_bits=kv_bits)
         from . import checkpoint
         if checkpoint.is_quantized_dir(p):
-            return CausalLM.from_gptq(p, lmax=lmax)
+            return CausalLM.from_gptq(p, lmax=lmax, kv_bits=kv_bits)
         q = {"int4": 4, "int8": 8}.get(dtype)
-        return CausalLM.from_fp16(p, lmax=lmax, quantize=q)
+        return CausalLM.from_fp16(p, lmax=lmax, quantize=q, kv_bits=kv_bits)
