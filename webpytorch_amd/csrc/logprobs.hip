@@ -5,13 +5,17 @@
 // The greedy loop of the reference reads the row back to the host and picks there (`_head_argmax`,
 // `_pick`: webtorch/llm.py:1309-1336).
 //
-// A workgroup takes a segment of a row in chunks that stay in registers, and every thread keeps a running
-// maximum m with s0 = sum exp(x - m) and s1 = sum exp(x - m) (x - m) (fp32; the threads' sums meet in fp64):
-// entropy = log s0 - s1 / s0. Alternatives go by 64-bit keys (the value in an order of integers, then the
-// inverted index), all different, so that a result does not depend on the order of arrival: a chunk's
-// keys above the segment's k-th best so far are collected in LDS, and a key's place is the number of keys
-// above it. The first chunk has no k-th best yet: of 32 groups of threads the least of their largest keys bounds
-// it from below. Segments of one row meet in the workspace, at the last to arrive.
+// A workgroup takes a segment of a row, each of its waves every fourth chunk of 1024 values, which stay in
+// registers while the next chunk's loads are in flight; the waves meet once, at the end, so that none waits for
+// another in the loop. With the running maximum m and y = (x - m) log2 e, s0 = sum 2^y and s1 = sum 2^y y (fp32)
+// give lse = m + ln 2 log2 s0 and entropy = ln 2 (log2 s0 - s1 / s0), in fp64.
+//
+// Alternatives go by 64-bit keys (the value in an order of integers, then the inverted index), all
+// different, so that a result does not depend on any order of arrival. A wave keeps up to 128 keys in LDS; a
+// chunk whose maximum is below the wave's k-th best is done with one ballot, otherwise the lanes' values
+// above it are appended, and past 64 keys the wave keeps the best k: a key's place is the number of keys above
+// it. The first chunk's bound: of 2^n >= k groups of lanes, the least of their maxima.
+// Segments of one row meet in the workspace, at the last to arrive.
 #include <math.h>
 
 #include "miq_common.h"
@@ -19,12 +23,12 @@
 namespace miq {
 
 constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
-constexpr int kLpPer = 16;                        // values of a thread and chunk
-constexpr int kLpChunk = kLpThreads * kLpPer;
+constexpr int kLpPer = 16;             // values of a lane and chunk
+constexpr int kLpChunk = 64 * kLpPer;  // of a wave
 constexpr int kLpMaxTop = 32;
-constexpr int kLpGroups = 32;                     // >= kLpMaxTop groups of 8 threads
-constexpr int kLpCand = kLpChunk + 2 * kLpMaxTop; // a chunk's keys, its row's unaligned ends, and those kept
-constexpr int kLpCtrStride = 32;                  // ints between arrival counters: a 128-byte line each
+constexpr int kLpList = 128;           // keys of a wave: at most 64, and 64 appended at a time
+constexpr int kLpJoin = 1024;          // keys of all segments of a row
+constexpr int kLpCtrStride = 32;       // ints between arrival counters: a 128-byte line each
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ uint64_t lp_key(float v, uint32_t idx) {
@@ -38,7 +42,6 @@ __device__ __forceinline__ float lp_value(uint64_t key) {
 }
 __device__ __forceinline__ int lp_index(uint64_t key) { return (int)(0xFFFFFFFFu - (uint32_t)key); }
 
-// running maximum and sums
 struct LpSum {
   float m, s0, s1;
 };
@@ -48,11 +51,14 @@ __device__ __forceinline__ void lp_merge(LpSum& a, float m, float s0, float s1) 
     a.s0 += s0;
     return;
   }
-  const float da = fmaxf(a.m - mn, -1e4f), db = fmaxf(m - mn, -1e4f);
-  const float fa = __builtin_amdgcn_exp2f(da * kLog2e), fb = __builtin_amdgcn_exp2f(db * kLog2e);
+  const float da = fmaxf((a.m - mn) * kLog2e, -1e4f), db = fmaxf((m - mn) * kLog2e, -1e4f);
+  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
   a.s1 = fa * fmaf(a.s0, da, a.s1) + fb * fmaf(s0, db, s1);
   a.s0 = fa * a.s0 + fb * s0;
   a.m = mn;
+}
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int s) {
+  return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), s) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, s);
 }
 
 template <typename T> struct LpLoad;
@@ -68,14 +74,29 @@ template <> struct LpLoad<__half> {
   static __device__ __forceinline__ void get(const __half* p, float* v) { load8(p, v); }
 };
 
-// The k largest of the n keys in cand, sorted, to best (k <= n): a key's place is the number above it.
-__device__ __forceinline__ void lp_select(const uint64_t* cand, int n, int k, uint64_t* best) {
-  for (int i = threadIdx.x; i < n; i += kLpThreads) {
-    const uint64_t key = cand[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += cand[j] > key;
-    if (above < k) best[above] = key;
+// One wave: the k largest of the n <= 128 keys of list, sorted, at its start (zeros where n < k).
+__device__ __forceinline__ void lp_keep(uint64_t* list, int n, int k) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t a = lane < n ? list[lane] : 0, b = lane + 64 < n ? list[lane + 64] : 0;
+  if (lane >= n) list[lane] = 0;
+  if (lane + 64 >= n) list[lane + 64] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  int ra = 0, rb = 0;
+  for (int j = 0; j < n; j += 8) {
+    uint64_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = list[j + i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ra += c[i] > a;
+      rb += c[i] > b;
+    }
   }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (a && ra < k) list[ra] = a;
+  if (b && rb < k) list[rb] = b;
+  if (lane >= n && lane < k) list[lane] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 template <typename T>
@@ -84,48 +105,52 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
     float* __restrict__ ent_out, int32_t* __restrict__ rank_out, int32_t* __restrict__ top_ids, float* __restrict__ top_lp,
     const int32_t* __restrict__ state, int out_rows, int* __restrict__ counters, uint64_t* __restrict__ parts) {
   constexpr int VEC = LpLoad<T>::VEC, U = kLpPer / VEC;
-  __shared__ uint64_t cand[kLpCand], best[kLpMaxTop], gbest[kLpGroups];
+  __shared__ __align__(16) uint64_t lists[kLpWaves][kLpList], join[kLpJoin];
   __shared__ LpSum sums[kLpWaves];
-  __shared__ int cnts[kLpWaves], ncand, last;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ uint64_t bounds[kLpWaves];
+  __shared__ int cnts[kLpWaves], njoin, last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int t = blockIdx.y, seg = blockIdx.x, segs = gridDim.x;
   const T* x = logits + (size_t)t * ld;
   const int id = ids[t];
   const bool given = id >= 0 && id < V;
   const float xt = given ? to_f32<T>(x[id]) : INFINITY;
+  uint64_t* list = lists[wave];
+  if (tid == 0) njoin = 0;
 
-  // vectors of 16 bytes from the first aligned value on, the same number for each segment (the last may
-  // have fewer); the values before and after them are one more value of segment 0's first threads
+  // vectors of 16 bytes from the first aligned value on, whole workgroup chunks for each segment (the last
+  // may have fewer); the values before and after them are one more value of segment 0's first lanes
   const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int head = min(V, mis ? VEC - mis : 0), nvec = (V - head) / VEC, ends = V - nvec * VEC;
+  constexpr int step = 64 * U;  // vectors of a wave's chunk
   const int per = (nvec + segs - 1) / segs, v0 = min(nvec, seg * per), v1 = min(nvec, v0 + per);
   const T* xv = x + head;
 
   LpSum a = {-INFINITY, 0.f, 0.f};
-  int above = 0, kept = 0;
-  uint64_t bound = 0;  // keys below it are not among the best k
-  if (tid == 0) ncand = 0;
+  int above = 0, n = 0;
+  uint64_t kth = 0;       // keys that are not above it are not among the best k
+  float bv = -INFINITY;   // nor values below it
   float nxt[kLpPer];
   auto load = [&](int vb) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int vi = vb + u * kLpThreads + tid;
+      const int vi = vb + u * 64 + lane;
       if (vi < v1) LpLoad<T>::get(xv + (size_t)vi * VEC, &nxt[u * VEC]);
       else
 #pragma unroll
         for (int e = 0; e < VEC; ++e) nxt[u * VEC + e] = -INFINITY;
     }
   };
-  load(v0);
+  load(v0 + wave * step);
   bool first = true;
-  for (int vb = v0; vb < v1 || first; vb += U * kLpThreads) {
+  for (int vb = v0 + wave * step; vb < v1 || first; vb += kLpWaves * step) {
     float v[kLpPer];
 #pragma unroll
     for (int e = 0; e < kLpPer; ++e) v[e] = nxt[e];
     const bool ext = first && seg == 0 && tid < ends;
-    const int xi = tid < head ? tid : head + nvec * VEC + (tid - head);
+    const int xi = tid < head ? tid : nvec * VEC + tid;
     const float xe = ext ? to_f32<T>(x[xi]) : -INFINITY;
-    if (vb + U * kLpThreads < v1) load(vb + U * kLpThreads);
+    if (vb + kLpWaves * step < v1) load(vb + kLpWaves * step);
 
     // ---- sums ----
     float cm = xe;  // the chunk's maximum
@@ -133,23 +158,22 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
     for (int e = 0; e < kLpPer; ++e) cm = fmaxf(cm, v[e]);
     const float mx = fmaxf(a.m, cm);
     if (mx > a.m) {
-      const float d = fmaxf(a.m - mx, -1e4f), f = __builtin_amdgcn_exp2f(d * kLog2e);
+      const float d = fmaxf((a.m - mx) * kLog2e, -1e4f), f = __builtin_amdgcn_exp2f(d);
       a.s1 = f * fmaf(a.s0, d, a.s1);
       a.s0 = f * a.s0;
       a.m = mx;
     }
     auto add = [&](float y) __attribute__((always_inline)) {
-      float d = y - a.m;
-      d = d < -1e4f ? -1e4f : d;  // exp is 0 there; a NaN stays
-      const float e = __builtin_amdgcn_exp2f(d * kLog2e);
-      a.s0 += e;
-      a.s1 = fmaf(e, d, a.s1);
+      const float d = (y - a.m) * kLog2e;
+      const float e = __builtin_amdgcn_exp2f(d);
+      a.s0 += e;  // NaN comes in here
+      a.s1 = fmaf(e, fmaxf(d, -1e4f), a.s1);
       above += y > xt;
     };
     if (mx > -INFINITY) {
 #pragma unroll
       for (int e = 0; e < kLpPer; ++e) add(v[e]);
-      add(xe);
+      if (ext) add(xe);
     } else {  // nothing but -inf and NaN so far
 #pragma unroll
       for (int e = 0; e < kLpPer; ++e) a.s0 += v[e] != v[e] ? v[e] : 0.f;
@@ -158,69 +182,60 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
 
     // ---- alternatives ----
     if (k) {
-      auto index = [&](int e) __attribute__((always_inline)) {
-        return (uint32_t)(head + (vb + (e / VEC) * kLpThreads + tid) * VEC + e % VEC);
-      };
-      auto valid = [&](int e) __attribute__((always_inline)) { return vb + (e / VEC) * kLpThreads + tid < v1; };
       if (first) {
-        uint64_t top = ext ? lp_key(xe, xi) : 0;
-#pragma unroll
-        for (int e = 0; e < kLpPer; ++e)
-          if (valid(e)) {
-            const uint64_t key = lp_key(v[e], index(e));
-            top = key > top ? key : top;
-          }
-#pragma unroll
-        for (int s = 1; s < 8; s <<= 1) {
-          const uint64_t o = ((uint64_t)(uint32_t)__shfl_xor((int)(top >> 32), s) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)top, s);
-          top = o > top ? o : top;
-        }
-        if ((tid & 7) == 0) gbest[tid >> 3] = top;
-        __syncthreads();
-        bound = gbest[0];
-        for (int i = 1; i < kLpGroups; ++i) bound = gbest[i] < bound ? gbest[i] : bound;
+        float g = cm;
+        for (int s = 1; s * k <= 32; s <<= 1) g = fmaxf(g, __shfl_xor(g, s));  // groups of the largest 2^n <= 64 / k lanes
+        bv = -wave_max(-g);
       }
-      const float bv = bound ? lp_value(bound) : -INFINITY;
-      const bool any = !bound || !(cm < bv);
-      if (__syncthreads_or(any)) {
-        if (any) {
-          auto push = [&](float y, uint32_t i) __attribute__((always_inline)) {
-            const uint64_t key = lp_key(y, i);
-            if (key >= bound) cand[atomicAdd(&ncand, 1)] = key;
-          };
-          if (ext) push(xe, xi);
+      if (__ballot(cm >= bv)) {
+        auto push = [&](float y, uint32_t i, bool valid) __attribute__((always_inline)) {
+          const uint64_t key = lp_key(y, i);
+          const uint64_t mask = __ballot(valid && !(y < bv) && key > kth);
+          if (!mask) return;
+          if ((mask >> lane) & 1) list[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
+          n += __popcll(mask);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          if (n > kLpList - 64) {
+            lp_keep(list, n, k);
+            n = k;
+            kth = list[k - 1];
+            bv = lp_value(kth);
+          }
+        };
+        if (first && seg == 0 && wave == 0) push(xe, xi, ext);
 #pragma unroll
-          for (int e = 0; e < kLpPer; ++e)
-            if (valid(e)) push(v[e], index(e));
-        }
-        __syncthreads();
-        const int n = ncand;
-        if (n > kept) {  // keys came: the best k of them and of those kept
-          const int nk = min(n, k);
-          lp_select(cand, n, nk, best);
-          __syncthreads();
-          if (tid < nk) cand[tid] = best[tid];
-          if (tid == 0) ncand = nk;
-          kept = nk;
-          bound = nk == k ? best[k - 1] + 1 : bound;
-          __syncthreads();
+        for (int e = 0; e < kLpPer; ++e) {
+          const int vi = vb + (e / VEC) * 64 + lane;
+          push(v[e], (uint32_t)(head + vi * VEC + e % VEC), vi < v1);
         }
       }
     }
     first = false;
   }
 
-  // ---- the threads' sums ----
+  // ---- the lanes' and the waves' parts ----
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) {
     lp_merge(a, __shfl_xor(a.m, s), __shfl_xor(a.s0, s), __shfl_xor(a.s1, s));
     above += __shfl_xor(above, s);
   }
+  if (k) lp_keep(list, n, k);
   if (lane == 0) {
     sums[wave] = a;
     cnts[wave] = above;
   }
   __syncthreads();
+  if (wave == 0 && k) {  // 4 k <= 128 keys
+    uint64_t key[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (lane + 64 * i < kLpWaves * k) key[i] = lists[(lane + 64 * i) / k][(lane + 64 * i) % k];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < 2; ++i) list[lane + 64 * i] = key[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    lp_keep(list, kLpWaves * k, k);
+  }
   a = sums[0];
   above = cnts[0];
   for (int w = 1; w < kLpWaves; ++w) {
@@ -229,78 +244,88 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
   }
 
   if (segs > 1) {
-    // a segment's part: (m, s0), (s1, above), keys kept, keys
-    const size_t step = 3 + (size_t)k;
-    uint64_t* part = parts + ((size_t)t * segs + seg) * step;
+    // a segment's part: (m, s0), (s1, above), keys
+    const size_t words = 2 + (size_t)k;
+    uint64_t* part = parts + ((size_t)t * segs + seg) * words;
     auto put = [](uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     auto get = [](const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-    if (tid == 0) {
-      put(part, (uint64_t)__float_as_uint(a.m) | ((uint64_t)__float_as_uint(a.s0) << 32));
-      put(part + 1, (uint64_t)__float_as_uint(a.s1) | ((uint64_t)(uint32_t)above << 32));
-      put(part + 2, (uint64_t)kept);
-    }
-    if (tid < kept) put(part + 3 + tid, cand[tid]);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (tid == 0) {
-      int* ctr = counters + (size_t)t * kLpCtrStride;
-      last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == segs - 1;
-      if (last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // re-armed
-      ncand = 0;
+    if (wave == 0) {  // it alone has the keys, and counts itself in
+      if (lane == 0) {
+        put(part, (uint64_t)__float_as_uint(a.m) | ((uint64_t)__float_as_uint(a.s0) << 32));
+        put(part + 1, (uint64_t)__float_as_uint(a.s1) | ((uint64_t)(uint32_t)above << 32));
+      }
+      if (lane < k) put(part + 2 + lane, list[lane]);
+      __builtin_amdgcn_s_waitcnt(0);
+      if (lane == 0) {
+        int* ctr = counters + (size_t)t * kLpCtrStride;
+        last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == segs - 1;
+        if (last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // re-armed
+      }
     }
     __syncthreads();
     if (!last) return;
-    const uint64_t* p0 = parts + (size_t)t * segs * step;
+    const uint64_t* p0 = parts + (size_t)t * segs * words;
+    // every load at once: the sums and the k-th key of segment tid, and a share of all keys
+    constexpr int KU = kLpJoin / kLpThreads;
+    uint64_t w0 = 0, w1 = 0, lb = 0, key[KU];
+    const bool mine = tid < segs;
+    if (mine) {
+      const uint64_t* p = p0 + (size_t)tid * words;
+      w0 = get(p);
+      w1 = get(p + 1);
+      if (k) lb = get(p + 1 + k);
+    }
+#pragma unroll
+    for (int i = 0; i < KU; ++i) {
+      const int q = tid + i * kLpThreads;
+      key[i] = 0;
+      if (q < segs * k) key[i] = get(p0 + (size_t)(q / k) * words + 2 + q % k);
+    }
     a = {-INFINITY, 0.f, 0.f};
     above = 0;
-    // the best of the segments' k-th keys: no key below it is among the row's best k
-    uint64_t lb = 0;
-    for (int s = tid; s < segs; s += kLpThreads) {
-      const uint64_t* p = p0 + (size_t)s * step;
-      const uint64_t w0 = get(p), w1 = get(p + 1);
-      lp_merge(a, __uint_as_float((uint32_t)w0), __uint_as_float((uint32_t)(w0 >> 32)), __uint_as_float((uint32_t)w1));
-      above += (int)(w1 >> 32);
-      if (k && (int)get(p + 2) == k) {
-        const uint64_t key = get(p + 3 + k - 1);
-        lb = key > lb ? key : lb;
-      }
+    if (mine) {
+      a = {__uint_as_float((uint32_t)w0), __uint_as_float((uint32_t)(w0 >> 32)), __uint_as_float((uint32_t)w1)};
+      above = (int)(w1 >> 32);
     }
+    // no key below the best of the segments' k-th keys is among the row's best k
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
       lp_merge(a, __shfl_xor(a.m, s), __shfl_xor(a.s0, s), __shfl_xor(a.s1, s));
       above += __shfl_xor(above, s);
-      const uint64_t o = ((uint64_t)(uint32_t)__shfl_xor((int)(lb >> 32), s) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)lb, s);
+      const uint64_t o = shfl_xor64(lb, s);
       lb = o > lb ? o : lb;
     }
+    __syncthreads();  // sums and cnts are read above
     if (lane == 0) {
       sums[wave] = a;
       cnts[wave] = above;
-      gbest[wave] = lb;
+      bounds[wave] = lb;
     }
     __syncthreads();
     a = sums[0];
     above = cnts[0];
-    lb = gbest[0];
+    lb = bounds[0];
     for (int w = 1; w < kLpWaves; ++w) {
       lp_merge(a, sums[w].m, sums[w].s0, sums[w].s1);
       above += cnts[w];
-      lb = gbest[w] > lb ? gbest[w] : lb;
+      lb = bounds[w] > lb ? bounds[w] : lb;
     }
-    for (int i = tid; i < segs * k; i += kLpThreads) {
-      const int s = i / k, j = i % k;
-      const uint64_t* p = p0 + (size_t)s * step;
-      if (j >= (int)get(p + 2)) continue;
-      const uint64_t key = get(p + 3 + j);
-      if (key >= lb) cand[atomicAdd(&ncand, 1)] = key;
-    }
-    __syncthreads();
     if (k) {
-      lp_select(cand, ncand, k, best);
+#pragma unroll
+      for (int i = 0; i < KU; ++i)
+        if (key[i] && key[i] >= lb) join[atomicAdd(&njoin, 1)] = key[i];
       __syncthreads();
-      if (tid < k) cand[tid] = best[tid];
-      __syncthreads();
+      const int nj = njoin;
+      for (int i = tid; i < nj; i += kLpThreads) {
+        const uint64_t me = join[i];
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < nj; ++j) place += join[j] > me;
+        if (place < k) lists[0][place] = me;
+      }
     }
   }
+  __syncthreads();
 
   // ---- the row's results ----
   int row = t;
@@ -310,35 +335,38 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
   }
   if (row >= out_rows) return;
   const bool none = a.m == -INFINITY && a.s0 == 0.f;  // every value -inf
-  const double lz = log((double)a.s0);                // lse = m + lz
-  auto logp = [&](float y) { return none || y == -INFINITY ? (a.s0 != a.s0 ? NAN : -INFINITY) : (float)(((double)y - (double)a.m) - lz); };
+  constexpr double kLn2 = 0.69314718055994530942;
+  const double lz = log2((double)a.s0) * kLn2;  // lse = m + lz
+  auto logp = [&](float y) {
+    return none || y == -INFINITY ? (a.s0 != a.s0 ? NAN : -INFINITY) : (float)(((double)y - (double)a.m) - lz);
+  };
   if (tid == 0) {
     if (lp_out) lp_out[row] = given ? logp(xt) : 0.f;
-    if (ent_out) ent_out[row] = none ? 0.f : (float)(lz - (double)a.s1 / (double)a.s0);
+    if (ent_out) ent_out[row] = none ? 0.f : (float)(lz - (double)a.s1 / (double)a.s0 * kLn2);
     if (rank_out) rank_out[row] = given ? above : -1;
   }
   if (tid < k) {
-    if (top_ids) top_ids[(size_t)row * k + tid] = lp_index(cand[tid]);
+    const int i = lp_index(lists[0][tid]);
+    if (top_ids) top_ids[(size_t)row * k + tid] = i;
     if (top_lp) {
-      const int i = lp_index(cand[tid]);
       top_lp[(size_t)row * k + tid] = logp(to_f32<T>(x[i]));
     }
   }
 }
 
-// Segments of a row: as many as give every CU four workgroups, of at least a chunk each, their keys within
-// the buffer that the last one collects them in.
+// Segments of a row: as many as give every CU four workgroups, of at least a chunk a wave each, their keys
+// within the buffer of the last one, and a thread of it for each.
 static int lp_segments(int T, int V, int k) {
-  const int most = (V + kLpChunk - 1) / kLpChunk;
+  const int most = (V + kLpWaves * kLpChunk - 1) / (kLpWaves * kLpChunk);
   int s = T >= 4 * kCUs ? 1 : (4 * kCUs + T - 1) / T;
   if (s > most) s = most;
-  const int cap = kLpCand / (k > 0 ? k : 1);
-  if (s > cap) s = cap;
+  if (s > kLpThreads) s = kLpThreads;
+  if (k && s > kLpJoin / k) s = kLpJoin / k;
   return s < 1 ? 1 : s;
 }
 static size_t lp_part_bytes(int T, int V, int k) {
   const int s = lp_segments(T, V, k);
-  return s > 1 ? (size_t)T * s * (3 + k) * 8 : 0;
+  return s > 1 ? (size_t)T * s * (2 + k) * 8 : 0;
 }
 
 }  // namespace miq
