@@ -114,7 +114,6 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
   const T* x = logits + (size_t)t * ld;
   const int id = ids[t];
   const bool given = id >= 0 && id < V;
-  const float xt = given ? to_f32<T>(x[id]) : INFINITY;
   uint64_t* list = lists[wave];
   if (tid == 0) njoin = 0;
 
@@ -142,6 +141,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
     }
   };
   load(v0 + wave * step);
+  const float xt = given ? to_f32<T>(x[id]) : INFINITY;  // behind the chunk's loads
   bool first = true;
   for (int vb = v0 + wave * step; vb < v1 || first; vb += kLpWaves * step) {
     float v[kLpPer];
@@ -346,19 +346,17 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
     if (rank_out) rank_out[row] = given ? above : -1;
   }
   if (tid < k) {
-    const int i = lp_index(lists[0][tid]);
-    if (top_ids) top_ids[(size_t)row * k + tid] = i;
-    if (top_lp) {
-      top_lp[(size_t)row * k + tid] = logp(to_f32<T>(x[i]));
-    }
+    const uint64_t key = lists[0][tid];
+    if (top_ids) top_ids[(size_t)row * k + tid] = lp_index(key);
+    if (top_lp) top_lp[(size_t)row * k + tid] = logp(lp_value(key));
   }
 }
 
-// Segments of a row: as many as give every CU four workgroups, of at least a chunk a wave each, their keys
+// Segments of a row: as many as give every CU two workgroups, of at least a chunk a wave each, their keys
 // within the buffer of the last one, and a thread of it for each.
 static int lp_segments(int T, int V, int k) {
   const int most = (V + kLpWaves * kLpChunk - 1) / (kLpWaves * kLpChunk);
-  int s = T >= 4 * kCUs ? 1 : (4 * kCUs + T - 1) / T;
+  int s = T >= 2 * kCUs ? 1 : (2 * kCUs + T - 1) / T;
   if (s > most) s = most;
   if (s > kLpThreads) s = kLpThreads;
   if (k && s > kLpJoin / k) s = kLpJoin / k;
