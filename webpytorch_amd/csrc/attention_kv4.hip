@@ -20,21 +20,15 @@ constexpr int kA4Rows = 16;
 constexpr float kA4Unit = 16384.f;  // a probability of 1
 constexpr int kA4CtrStride = 32;    // ints between arrival counters: a 128-byte line each
 constexpr int kA4MaxSlices = 64;
+constexpr int kA4MinSteps = 8;      // key steps of a slice of many rows, at least
 
-// the maximum (the sum) over the four lanes c, c + 16, c + 32, c + 48
+// the maximum over the four lanes c, c + 16, c + 32, c + 48
 __device__ __forceinline__ float rows_max(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float rows_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // 2^n of a row: q 2^n has its largest magnitude in [2^13, 2^14); 1 for zero and non-finite rows
 __device__ __forceinline__ int row_shift(float mx) {
   const int e = (int)((__float_as_uint(mx) >> 23) & 255);
@@ -52,6 +46,133 @@ __device__ __forceinline__ half8v unpack_value(uint32_t w, const uint32_t* S, co
   return cat4(fma2(kv4_pair<0>(w), as_h2(S[0]), as_h2(Z[0])), fma2(kv4_pair<1>(w), as_h2(S[1]), as_h2(Z[1])),
               fma2(kv4_pair<2>(w), as_h2(S[2]), as_h2(Z[2])), fma2(kv4_pair<3>(w), as_h2(S[3]), as_h2(Z[3])));
 }
+
+// q of this lane (8 dimensions of every 32) as matrix-core operands: hi, and for fp32 rows lo, of q 2^n with the
+// row's largest magnitude in [2^13, 2^14); `back` takes a product to units of log 2 and is positive (the sign
+// of the scale goes into q; a scale of 0 makes q 0).
+template <int HD, typename XT>
+__device__ __forceinline__ void load_q(const XT* qr, float scale, half8v (&qh)[sizeof(XT) == 4 ? 2 : 1][HD / 32], float& back) {
+  constexpr int P = sizeof(XT) == 4 ? 2 : 1, NJ = HD / 32;
+  float v[NJ][8], mx = 0.f;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[j][e] = to_f32<XT>(qr[32 * j + e]);
+      mx = fmaxf(mx, fabsf(v[j][e]));
+    }
+  const float sign = scale < 0.f ? -1.f : scale == 0.f ? 0.f : 1.f;
+  const int n = P == 2 ? row_shift(rows_max(mx)) : 0;
+  back = scale == 0.f ? 1.f : fmaxf(ldexpf(fabsf(scale) * 1.44269504088896340736f, -n), 0x1p-126f);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = sign * (P == 2 ? ldexpf(v[j][e], n) : v[j][e]);
+      const _Float16 hi = (_Float16)x;
+      qh[0][j][e] = hi;
+      if constexpr (P == 2) qh[1][j][e] = (_Float16)(x - (float)hi);
+    }
+}
+
+// Parts of slices pass through the device-scope coherence point: stores and loads past the XCD's own L2.
+__device__ __forceinline__ void put2(float* p, float a, float b) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t get2(const float* p) {
+  return __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Whether this workgroup is the last of the `slices` that stored their parts (the counter is left zero).
+__device__ __forceinline__ bool last_slice(int* ctr, int slices, int* last) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    *last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == slices - 1;
+    if (*last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *last;
+}
+// out rows r0 .. r0 + nr - 1 from the slices' parts ([row][HD + 4]: the output, the maximum and the sum), in
+// slice order
+template <int HD, typename XT, int THREADS>
+__device__ __forceinline__ void join_slices(const float* p0, size_t step, int slices, XT* out, int r0, int nr, int rep, int kv, int NH) {
+  for (int x = threadIdx.x; x < nr * (HD / 2); x += THREADS) {
+    const int row = x / (HD / 2), d = 2 * (x % (HD / 2));
+    const float* pr = p0 + (size_t)row * (HD + 4);
+    float mx = -INFINITY, sum = 0.f, a[2] = {0.f, 0.f};
+    constexpr int U = 8;
+    for (int k0 = 0; k0 < slices; k0 += U) {
+      uint64_t st[U], v[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const float* ps = pr + (size_t)min(k0 + i, slices - 1) * step;
+        st[i] = get2(ps + HD);
+        v[i] = get2(ps + d);
+      }
+      float mn = mx;
+#pragma unroll
+      for (int i = 0; i < U; ++i) mn = fmaxf(mn, __uint_as_float((uint32_t)st[i]));
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float al = __builtin_amdgcn_exp2f(mx - ref);
+      sum *= al;
+      a[0] *= al;
+      a[1] *= al;
+      mx = mn;
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (k0 + i < slices) {
+          const float f = __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)st[i]) - ref);
+          sum = fmaf(f, __uint_as_float((uint32_t)(st[i] >> 32)), sum);
+          a[0] = fmaf(f, __uint_as_float((uint32_t)v[i]), a[0]);
+          a[1] = fmaf(f, __uint_as_float((uint32_t)(v[i] >> 32)), a[1]);
+        }
+    }
+    const int rr = r0 + row;
+    XT* orow = out + ((size_t)(rr / rep) * NH + kv * rep + rr % rep) * HD + d;
+    orow[0] = from_f32<XT>(sum == 0.f ? 0.f : a[0] / sum);
+    orow[1] = from_f32<XT>(sum == 0.f ? 0.f : a[1] / sum);
+  }
+}
+
+// 8 probabilities as matrix-core operands: rounded towards zero to fp16, and for fp32 rows what that leaves
+// (the sum of probabilities is taken of the operands, by the matrix cores, so that a rounding to one side
+// cancels in the quotient).
+template <int P> __device__ __forceinline__ void split_p(const float* p, half8v* ph) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const half2v hi = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(p[2 * x], p[2 * x + 1]));
+    ph[0][2 * x] = hi.x;
+    ph[0][2 * x + 1] = hi.y;
+    if constexpr (P == 2) {
+      const half2v lo = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, -1.f, p[2 * x]), fmaf((float)hi.y, -1.f, p[2 * x + 1])));
+      ph[1][2 * x] = lo.x;
+      ph[1][2 * x + 1] = lo.y;
+    }
+  }
+}
+__device__ __forceinline__ half8v ones() { return (half8v){1, 1, 1, 1, 1, 1, 1, 1}; }
+
+// Groups with a NaN or an infinity (S negative) among a lane's 8 keys: their S and Z are cleared; the
+// return value has a bit for each such key of the block (all lanes together).
+__device__ __forceinline__ uint32_t clear_bad(uint32_t* S, uint32_t* Z) {
+  uint32_t hit = 0;
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const uint32_t lo = (S[p] >> 15) & 1, hi = S[p] >> 31, keep = (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+    hit |= (lo | hi << 1) << kv4_key(g, 2 * p);
+    S[p] &= keep;
+    Z[p] &= keep;
+  }
+  hit |= (uint32_t)__shfl_xor((int)hit, 16);
+  return hit | (uint32_t)__shfl_xor((int)hit, 32);
+}
+// bits of the keys k0 .. k0 + 31 that a row attends to, its last key being lim
+__device__ __forceinline__ uint32_t attends(int k0, int lim) { return lim < k0 ? 0u : lim - k0 >= 31 ? 0xFFFFFFFFu : (2u << (lim - k0)) - 1u; }
+// the halves of a pair of keys k, k + 1 below end
+__device__ __forceinline__ uint32_t keep_pair(int k, int end) { return (k < end ? 0xFFFFu : 0u) | (k + 1 < end ? 0xFFFF0000u : 0u); }
 
 // Rows that fit a few tiles: the waves of a workgroup share a tile's 16 rows and split its keys, and so do
 // the slices (blockIdx.x) of one tile and kv head. A slice's result (maximum, sum, output) goes to the
@@ -71,33 +192,9 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
   const int t = r / rep, h = kv * rep + r % rep;
   const uint8_t* C = cache + (size_t)kv * kv4_blocks(LMAX) * kv4_record(HD);
 
-  // ---- q as matrix-core operands ----
   half8v qh[P][NJ];
-  float back = scale * 1.44269504088896340736f;  // scores in units of log 2
-  {
-    const XT* qr = q + ((size_t)t * NH + h) * HD + 8 * g;
-    float v[NJ][8];
-    float mx = 0.f;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[j][e] = to_f32<XT>(qr[32 * j + e]);
-        mx = fmaxf(mx, fabsf(v[j][e]));
-      }
-    }
-    const int n = P == 2 ? row_shift(rows_max(mx)) : 0;
-    back = ldexpf(back, -n);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = P == 2 ? ldexpf(v[j][e], n) : v[j][e];
-        const _Float16 hi = (_Float16)x;
-        qh[0][j][e] = hi;
-        if constexpr (P == 2) qh[1][j][e] = (_Float16)(x - (float)hi);
-      }
-  }
+  float back;
+  load_q<HD, XT>(q + ((size_t)t * NH + h) * HD + 8 * g, scale, qh, back);
 
   const int64_t pos0 = state[0];
   const int lim = (int)(pos0 + t < LMAX ? pos0 + t : LMAX - 1);  // this row's last key
@@ -112,7 +209,8 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
   const int b1 = min(nblk, (slice + 1) * per);
 
   float4v o[NT];
-  float m = -INFINITY, l = 0.f;
+  float4v l = (float4v){0.f, 0.f, 0.f, 0.f};  // the sum of probabilities, in every row of the product
+  float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NT; ++i) o[i] = (float4v){0.f, 0.f, 0.f, 0.f};
   for (int blk = slice * per + wave; blk < b1; blk += NW) {
@@ -164,16 +262,13 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
     const float alpha = __builtin_amdgcn_exp2f(m - ref);
     m = mn;
     half8v ph[P];
-    float ps = 0.f;
+    float p8[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float p = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - ref) * kA4Unit;
-      ps += p;
-      const _Float16 hi = (_Float16)p;
-      ph[0][e] = hi;
-      if constexpr (P == 2) ph[1][e] = (_Float16)(p - (float)hi);
-    }
-    l = l * alpha + ps;
+    for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - ref) * kA4Unit;
+    split_p<P>(p8, ph);
+    l *= alpha;
+#pragma unroll
+    for (int p = P - 1; p >= 0; --p) l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones(), ph[p], l, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i] *= alpha;
 
@@ -183,8 +278,7 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
     if (masked) {
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        const int k = blk * kKv4Block + kv4_key(g, 2 * p);
-        const uint32_t keep = (k < S ? 0xFFFFu : 0u) | (k + 1 < S ? 0xFFFF0000u : 0u);
+        const uint32_t keep = keep_pair(blk * kKv4Block + kv4_key(g, 2 * p), S);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           vm[j][p] &= keep;
@@ -198,51 +292,32 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
 #pragma unroll
       for (int p = 0; p < 4; ++p) odd |= vm[j][p];
     const bool bad = __ballot((odd & 0x80008000u) != 0) != 0ull;
-    uint32_t hit[NJ];  // keys e of this lane whose group j is bad
-    if (bad) {
+    uint32_t hit[NJ] = {};  // keys whose group j is bad
+    if (bad)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        hit[j] = 0;
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const uint32_t w = vm[j][p];
-          const uint32_t keep = ((w >> 15) & 1 ? 0u : 0xFFFFu) | (w >> 31 ? 0u : 0xFFFF0000u);
-          hit[j] |= (((w >> 15) & 1) | ((w >> 31) << 1)) << (2 * p);
-          vm[j][p] &= keep;
-          vm[j][4 + p] &= keep;
-        }
-      }
-    }
+      for (int j = 0; j < NJ; ++j) hit[j] = clear_bad(&vm[j][0], &vm[j][4]);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const half8v v = unpack_value(vw[i], &vm[i >> 1][0], &vm[i >> 1][4]);
 #pragma unroll
       for (int p = P - 1; p >= 0; --p) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[p], o[i], 0, 0, 0);
     }
-    if (bad) {
+    if (bad)
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
-        for (int gg = 0; gg < 4; ++gg) {
-          const uint32_t hs = (uint32_t)__builtin_amdgcn_readlane((int)hit[j], 16 * gg);
-          bool nan = false;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) nan |= ((hs >> e) & 1) && blk * kKv4Block + kv4_key(gg, e) <= lim;
-          if (nan) {
-            o[2 * j] += NAN;
-            o[2 * j + 1] += NAN;
-          }
+        if (hit[j] & attends(blk * kKv4Block, lim)) {
+          o[2 * j] += NAN;
+          o[2 * j + 1] += NAN;
         }
-    }
   }
 
   // ---- the waves' parts, rescaled to their common maximum ----
   const int nw = max(1, min(NW, b1 - slice * per));  // waves that had keys (wave 0 always takes part)
   const int nr = min(QR, R - r0);
   if (wave < nw) {
-    l = rows_sum(l);
     if (g == 0) {
       ms[wave][c] = m;
-      ls[wave][c] = l;
+      ls[wave][c] = l[0];
     }
     if (c < nr)
 #pragma unroll
@@ -266,15 +341,9 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
       for (int e = 0; e < 4; ++e) a[e] = fmaf(f, v[e], a[e]);
     }
     if (slices > 1) {
-      uint64_t* o8 = reinterpret_cast<uint64_t*>(part + row * (HD + 4) + d);
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        __hip_atomic_store(o8 + e, (uint64_t)__float_as_uint(a[2 * e]) | ((uint64_t)__float_as_uint(a[2 * e + 1]) << 32),
-                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (d == 0)
-        __hip_atomic_store(reinterpret_cast<uint64_t*>(part + row * (HD + 4) + HD),
-                           (uint64_t)__float_as_uint(mx) | ((uint64_t)__float_as_uint(sum) << 32), __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
+      put2(part + row * (HD + 4) + d, a[0], a[1]);
+      put2(part + row * (HD + 4) + d + 2, a[2], a[3]);
+      if (d == 0) put2(part + row * (HD + 4) + HD, mx, sum);
       continue;
     }
     const int rr = r0 + row;
@@ -284,74 +353,298 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
   }
   if (slices == 1) return;
 
-  // ---- the slices' parts, by the last to arrive ----
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int* ctr = counters + (kv * gridDim.y + tile) * kA4CtrStride;
-    last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == slices - 1;
-    if (last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // re-armed
-  }
-  __syncthreads();
-  if (!last) return;
-  const float* p0 = parts + (size_t)(kv * gridDim.y + tile) * gridDim.x * QR * (HD + 4);
-  const size_t step = (size_t)QR * (HD + 4);
-  for (int x = threadIdx.x; x < nr * (HD / 2); x += 64 * NW) {
-    const int row = x / (HD / 2), d = 2 * (x % (HD / 2));
-    const float* pr = p0 + row * (HD + 4);
-    float mx = -INFINITY, sum = 0.f, a[2] = {0.f, 0.f};
-    constexpr int U = 8;
-    for (int k0 = 0; k0 < slices; k0 += U) {
-      uint64_t st[U], v[U];
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const float* ps = pr + (size_t)min(k0 + i, slices - 1) * step;
-        st[i] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(ps + HD), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        v[i] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(ps + d), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      float mn = mx;
-#pragma unroll
-      for (int i = 0; i < U; ++i) mn = fmaxf(mn, __uint_as_float((uint32_t)st[i]));
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      const float al = __builtin_amdgcn_exp2f(mx - ref);
-      sum *= al;
-      a[0] *= al;
-      a[1] *= al;
-      mx = mn;
-#pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (k0 + i < slices) {
-          const float f = __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)st[i]) - ref);
-          sum = fmaf(f, __uint_as_float((uint32_t)(st[i] >> 32)), sum);
-          a[0] = fmaf(f, __uint_as_float((uint32_t)v[i]), a[0]);
-          a[1] = fmaf(f, __uint_as_float((uint32_t)(v[i] >> 32)), a[1]);
-        }
-    }
-    const int rr = r0 + row;
-    XT* orow = out + ((size_t)(rr / rep) * NH + kv * rep + rr % rep) * HD + d;
-    orow[0] = from_f32<XT>(sum == 0.f ? 0.f : a[0] / sum);
-    orow[1] = from_f32<XT>(sum == 0.f ? 0.f : a[1] / sum);
-  }
+  if (!last_slice(counters + (kv * gridDim.y + tile) * kA4CtrStride, slices, &last)) return;
+  join_slices<HD, XT, 64 * NW>(parts + (size_t)(kv * gridDim.y + tile) * gridDim.x * QR * (HD + 4), (size_t)QR * (HD + 4), slices,
+                               out, r0, nr, rep, kv, NH);
 }
 
-// Slices of each tile's keys: as many as give every CU a workgroup, of at least a block a wave of a full cache.
+// Many rows: a workgroup takes 4 x 16 QT of them, every wave its own, and all their keys (or a slice of
+// them), 32 at a time (64 for HD 64). The waves unpack the records' words together, once for all rows, into
+// operands in LDS, in operand order: each write and read is 16 consecutive bytes a lane. Two buffers, one
+// barrier a step: while a step's products run, the next step's words, loaded a step before that, are unpacked.
+// The reference of the exponentials is raised only when a score passes it by more than 2^8 (p then stays
+// below 2^15), so that the output is seldom rescaled.
+constexpr int kA4TileWaves = 4;
+constexpr float kA4TileUnitLog2 = 7.f;  // a probability of 1 is 2^7 at the reference
+constexpr float kA4Slack = 8.f;
+__host__ __device__ constexpr int kv4_step_blocks(int HD) { return HD == 64 ? 2 : 1; }
+__host__ __device__ constexpr int kv4_tile_qt(int HD) { return HD <= 128 ? 2 : 1; }
+__host__ __device__ constexpr int kv4_tile_rows(int HD) { return kA4TileWaves * 16 * kv4_tile_qt(HD); }
+
+template <int HD, typename XT>
+__global__ __launch_bounds__(64 * kA4TileWaves, 2) void attention_kv4_tiles_kernel(
+    const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ state, XT* __restrict__ out,
+    int T, int NH, int NKV, int LMAX, float scale, int* __restrict__ counters, float* __restrict__ parts) {
+  constexpr int P = sizeof(XT) == 4 ? 2 : 1, NJ = HD / 32, NT = HD / 16, QT = kv4_tile_qt(HD), NBK = kv4_step_blocks(HD);
+  constexpr int RW = 16 * QT, QR = kv4_tile_rows(HD);
+  constexpr int HALF = NBK * NT / 4, GROUPS = 2 * HALF, GPW = (GROUPS + kA4TileWaves - 1) / kA4TileWaves;
+  extern __shared__ __align__(16) half8v ops[];  // [2][K, V][NBK NT][64]
+  __shared__ uint32_t flags[2][kA4TileWaves], hits[2][NBK][NJ];
+  __shared__ int last;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int kv = blockIdx.x, tile = (int)gridDim.y - 1 - (int)blockIdx.y, slice = blockIdx.z, rep = NH / NKV;  // long tiles first
+  const int R = T * rep, r0 = tile * QR, rw = r0 + wave * RW;
+  const uint8_t* C = cache + (size_t)kv * kv4_blocks(LMAX) * kv4_record(HD);
+
+  const int64_t pos0 = state[0];
+  const auto last_key = [&](int r) { return (int)min(pos0 + r / rep, (int64_t)LMAX - 1); };  // below 0: none
+  const int S = max(0, last_key(min(r0 + QR, R) - 1) + 1);  // keys that any row attends to
+  const int steps = (S + kKv4Block * NBK - 1) / (kKv4Block * NBK);
+  const int per = max(kA4MinSteps, (steps + (int)gridDim.z - 1) / (int)gridDim.z);
+  const int slices = max(1, (steps + per - 1) / per);
+  if (slice >= slices) return;
+  const int s0 = slice * per, s1 = min(steps, s0 + per);
+  const int nblk = (S + kKv4Block - 1) / kKv4Block;
+
+  // ---- words of a step on their way: group x of 64 x 16 bytes, K groups first ----
+  uint4 rw4[GPW], rm[GPW][4];
+  auto fetch = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < GPW; ++x) {
+      const int gi = wave + x * kA4TileWaves;
+      if (GROUPS % kA4TileWaves && gi >= GROUPS) break;
+      const int gg = gi % HALF, u = gg % (NT / 4);
+      const uint8_t* rec = C + (size_t)min(step * NBK + gg / (NT / 4), nblk - 1) * kv4_record(HD);
+      if (gi < HALF) {
+        rw4[x] = *reinterpret_cast<const uint4*>(rec + (u * 64 + lane) * 16);
+        if constexpr (NJ % 4 == 0) {
+          rm[x][0] = *reinterpret_cast<const uint4*>(rec + kv4_kmeta(HD) + ((16 * (4 * u / NJ) + c) * NJ + 4 * u % NJ) * 4);
+        } else {
+          uint2 m[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int n = 4 * u + 2 * i;
+            m[i] = *reinterpret_cast<const uint2*>(rec + kv4_kmeta(HD) + ((16 * (n / NJ) + c) * NJ + n % NJ) * 4);
+          }
+          rm[x][0] = make_uint4(m[0].x, m[0].y, m[1].x, m[1].y);
+        }
+      } else {
+        rw4[x] = *reinterpret_cast<const uint4*>(rec + kv4_vcodes(HD) + (u * 64 + lane) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          rm[x][i] = *reinterpret_cast<const uint4*>(rec + kv4_vmeta(HD) + ((2 * u + (i >> 1)) * 4 + g) * 32 + 16 * (i & 1));
+      }
+    }
+  };
+  auto stage = [&](int step, int buf) __attribute__((always_inline)) {
+    uint32_t odd = 0;
+#pragma unroll
+    for (int x = 0; x < GPW; ++x) {
+      const int gi = wave + x * kA4TileWaves;
+      if (GROUPS % kA4TileWaves && gi >= GROUPS) break;
+      const int gg = gi % HALF, u = gg % (NT / 4), bo = gg / (NT / 4);
+      half8v* dst = ops + ((size_t)(buf * 2 + (gi >= HALF)) * NBK * NT + bo * NT + 4 * u) * 64 + lane;
+      const uint32_t* w = &rw4[x].x;
+      if (gi < HALF) {
+        const uint32_t* m = &rm[x][0].x;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) dst[n * 64] = unpack_key(w[n], m[n]);
+      } else {
+        const int k0 = (step * NBK + bo) * kKv4Block;
+        if (k0 + kKv4Block > S) {  // keys behind the last one hold anything
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const uint32_t keep = keep_pair(k0 + kv4_key(g, 2 * p), S);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) (&rm[x][i].x)[p] &= keep;
+          }
+        }
+        // groups with a NaN or an infinity (S negative) are cleared, and noted for the rows
+        uint32_t neg = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) neg |= (&rm[x][i].x)[p];
+        if (__ballot((neg & 0x80008000u) != 0)) {
+          odd = 1;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t hit = clear_bad(&rm[x][2 * i].x, &rm[x][2 * i + 1].x);
+            if (lane == 0) hits[buf][bo][2 * u + i] = hit;
+          }
+        } else if (lane < 2) {
+          hits[buf][bo][2 * u + lane] = 0;
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) dst[n * 64] = unpack_value(w[n], &rm[x][2 * (n >> 1)].x, &rm[x][2 * (n >> 1) + 1].x);
+      }
+    }
+    if (lane == 0) flags[buf][wave] = odd;
+  };
+  if (s0 < s1) fetch(s0);
+
+  // ---- q as matrix-core operands; scores in units of log 2, their factor positive ----
+  half8v qh[QT][P][NJ];
+  float back[QT];
+  int lim[QT];
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    const int r = min(rw + 16 * i + c, R - 1);
+    lim[i] = last_key(r);
+    load_q<HD, XT>(q + ((size_t)(r / rep) * NH + kv * rep + r % rep) * HD + 8 * g, scale, qh[i], back[i]);
+  }
+  const int first = last_key(min(rw, R - 1)), wlast = last_key(min(rw + RW, R) - 1);
+
+  float4v o[QT][NT];
+  float4v l[QT];  // the sum of probabilities, in every row of the product
+  float m[QT];
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    m[i] = -INFINITY;
+    l[i] = (float4v){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[i][n] = (float4v){0.f, 0.f, 0.f, 0.f};
+  }
+  if (s0 < s1) stage(s0, 0);
+  if (s0 + 1 < s1) fetch(s0 + 1);
+  __syncthreads();
+  for (int step = s0; step < s1; ++step) {
+    const int buf = (step - s0) & 1;
+    const half8v* kf = ops + (size_t)buf * 2 * NBK * NT * 64 + lane;
+    const half8v* vf = kf + (size_t)NBK * NT * 64;
+    const bool live = rw < R && step * NBK * kKv4Block <= wlast;  // wave-uniform
+    float4v s[QT][2 * NBK];
+    if (live) {
+#pragma unroll
+      for (int b = 0; b < 2 * NBK; ++b) {
+#pragma unroll
+        for (int i = 0; i < QT; ++i) s[i][b] = (float4v){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const half8v k = kf[(b * NJ + j) * 64];
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+            for (int i = 0; i < QT; ++i) s[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[i][p][j], s[i][b], 0, 0, 0);
+        }
+      }
+    }
+    if (step + 1 < s1) {
+      stage(step + 1, buf ^ 1);
+      if (step + 2 < s1) fetch(step + 2);
+    }
+    if (live) {
+      half8v ph[QT][NBK][P];
+      const int k0 = step * NBK * kKv4Block;
+      const bool masked = k0 + NBK * kKv4Block - 1 > first;  // wave-uniform
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
+        if (masked) {
+#pragma unroll
+          for (int b = 0; b < 2 * NBK; ++b)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (k0 + 16 * b + 4 * g + x > lim[i]) s[i][b][x] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2 * NBK; ++b)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mx = fmaxf(mx, s[i][b][x]);
+        mx = rows_max(mx) * back[i];
+        if (__ballot(mx > m[i] + kA4Slack)) {  // m = -inf: always
+          const float mn = fmaxf(m[i], mx);
+          const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i] - mn);
+          m[i] = mn;
+          l[i] *= alpha;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) o[i][n] *= alpha;
+        }
+        const float ref = (m[i] == -INFINITY ? 0.f : m[i]) - kA4TileUnitLog2;  // no key yet: every probability is 0
+#pragma unroll
+        for (int b = 0; b < NBK; ++b) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[i][2 * b + (e >> 2)][e & 3], back[i], -ref));
+          split_p<P>(p, ph[i][b]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < NBK; ++b)
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+          for (int i = 0; i < QT; ++i) l[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones(), ph[i][b][p], l[i], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int b = 0; b < NBK; ++b) {
+          const half8v v = vf[(b * NT + n) * 64];
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+            for (int i = 0; i < QT; ++i) o[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[i][b][p], o[i][n], 0, 0, 0);
+        }
+      if (uniform((int)(flags[buf][0] | flags[buf][1] | flags[buf][2] | flags[buf][3]))) {
+#pragma unroll
+        for (int b = 0; b < NBK; ++b)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < QT; ++i)
+              if (hits[buf][b][j] & attends(k0 + kKv4Block * b, lim[i])) {
+                o[i][2 * j] += NAN;
+                o[i][2 * j + 1] += NAN;
+              }
+      }
+    }
+    __syncthreads();
+  }
+
+  // ---- out, or the slice's part ----
+  float* part = slices > 1 ? parts + ((size_t)(kv * gridDim.y + tile) * gridDim.z + slice) * QR * (HD + 4) : nullptr;
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    const float sum = l[i][0];
+    const int r = rw + 16 * i + c;
+    if (r >= R) continue;
+    if (slices > 1) {
+      float* pr = part + (size_t)(r - r0) * (HD + 4);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2)
+          put2(pr + 16 * n + 4 * g + e, o[i][n][e], o[i][n][e + 1]);
+      if (g == 0) put2(pr + HD, m[i], sum);
+      continue;
+    }
+    XT* orow = out + ((size_t)(r / rep) * NH + kv * rep + r % rep) * HD + 4 * g;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) orow[16 * n + e] = from_f32<XT>(sum == 0.f ? 0.f : o[i][n][e] / sum);  // a row without keys: zeros
+  }
+  if (slices == 1) return;
+  if (!last_slice(counters + (kv * gridDim.y + tile) * kA4CtrStride, slices, &last)) return;
+  join_slices<HD, XT, 64 * kA4TileWaves>(parts + (size_t)(kv * gridDim.y + tile) * gridDim.z * QR * (HD + 4), (size_t)QR * (HD + 4),
+                                         slices, out, r0, min(QR, R - r0), rep, kv, NH);
+}
+
+// Up to kA4FewRows rows of a kv head go by the rows kernel, more by the tiles kernel. Each tile's keys are
+// split into as many slices as give every CU a workgroup, of at least a block a wave (8 steps) of a full cache.
+constexpr int kA4FewRows = 48;
 struct Kv4Plan {
-  int tiles, slices;
+  int tiles, slices, rows;  // rows of a tile
+  bool few;
 };
-static Kv4Plan kv4_plan(int T, int NH, int NKV, int LMAX) {
+static Kv4Plan kv4_plan(int T, int NH, int NKV, int HD, int LMAX) {
   Kv4Plan p;
-  p.tiles = (int)(((int64_t)T * (NH / NKV) + kA4Rows - 1) / kA4Rows);
+  const int64_t R = (int64_t)T * (NH / NKV);
+  p.few = R <= kA4FewRows;
+  p.rows = p.few ? kA4Rows : kv4_tile_rows(HD);
+  p.tiles = (int)((R + p.rows - 1) / p.rows);
   const int64_t wgs = (int64_t)p.tiles * NKV;
-  const int most = (kv4_blocks(LMAX) + kA4Waves - 1) / kA4Waves;
+  const int steps = p.few ? kv4_blocks(LMAX) : (kv4_blocks(LMAX) + kv4_step_blocks(HD) - 1) / kv4_step_blocks(HD);
+  const int least = p.few ? kA4Waves : kA4MinSteps;
   int64_t s = wgs >= kCUs ? 1 : kCUs / wgs;
-  if (s > most) s = most;
+  if (s > (steps + least - 1) / least) s = (steps + least - 1) / least;
   if (s > kA4MaxSlices) s = kA4MaxSlices;
   p.slices = (int)s;
   return p;
 }
 
 static size_t kv4_part_bytes(const Kv4Plan& p, int NKV, int HD) {
-  return p.slices > 1 ? (size_t)p.slices * p.tiles * NKV * kA4Rows * (HD + 4) * 4 : 0;
+  return p.slices > 1 ? (size_t)p.slices * p.tiles * NKV * p.rows * (HD + 4) * 4 : 0;
 }
 
 }  // namespace miq
@@ -362,7 +655,7 @@ static int check_attention_kv4(const char* what, int T, int NH, int NKV, int HD,
   MIQ_REQUIRE(T >= 0 && NH > 0 && NKV > 0 && NH % NKV == 0 && NH <= (1 << 16) && NKV <= 65535 && HD > 0 && LMAX > 0 && LMAX <= (1 << 30),
               MIQ_ERR_INVALID, "%s: T=%d NH=%d NKV=%d HD=%d LMAX=%d", what, T, NH, NKV, HD, LMAX);
   MIQ_REQUIRE(kv4_head(HD), MIQ_ERR_UNSUPPORTED, "%s: HD=%d (64, 128, 192 or 256)", what, HD);
-  MIQ_REQUIRE((int64_t)T * (NH / NKV) <= (int64_t)65535 * kA4Rows, MIQ_ERR_UNSUPPORTED, "%s: T=%d rows of %d heads a kv head are past the grid",
+  MIQ_REQUIRE((int64_t)T * (NH / NKV) <= (int64_t)65535 * kv4_tile_rows(HD), MIQ_ERR_UNSUPPORTED, "%s: T=%d rows of %d heads a kv head are past the grid",
               what, T, NH / NKV);
   return MIQ_OK;
 }
@@ -372,7 +665,7 @@ extern "C" int miq_attention_kv4_workspace(int T, int NH, int NKV, int HD, int L
   if (int rc = check_attention_kv4("attention_kv4_workspace", T, NH, NKV, HD, LMAX)) return rc;
   *bytes = 0;
   if (T == 0) return MIQ_OK;
-  const size_t part = kv4_part_bytes(kv4_plan(T, NH, NKV, LMAX), NKV, HD);
+  const size_t part = kv4_part_bytes(kv4_plan(T, NH, NKV, HD, LMAX), NKV, HD);
   *bytes = part ? kCounterBytes + part : 0;
   return MIQ_OK;
 }
@@ -385,20 +678,25 @@ extern "C" int miq_attention_kv4(const void* q, int x_dtype, const void* cache, 
   if (T == 0) return MIQ_OK;
   MIQ_REQUIRE(q && cache && state && out, MIQ_ERR_INVALID, "attention_kv4: null pointer");
   MIQ_REQUIRE(aligned(cache, 16), MIQ_ERR_ALIGN, "attention_kv4: the cache must be 16-byte aligned");
-  const Kv4Plan p = kv4_plan(T, NH, NKV, LMAX);
+  const Kv4Plan p = kv4_plan(T, NH, NKV, HD, LMAX);
   const size_t part = kv4_part_bytes(p, NKV, HD);
   MIQ_REQUIRE(!part || (workspace && ws_bytes >= kCounterBytes + part), MIQ_ERR_INVALID,
               "attention_kv4: workspace of %zu bytes, %zu needed", workspace ? ws_bytes : (size_t)0, kCounterBytes + part);
   MIQ_REQUIRE(!part || aligned(workspace, 256), MIQ_ERR_ALIGN, "attention_kv4: the workspace must be 256-byte aligned");
   int* counters = static_cast<int*>(workspace);
   float* parts = part ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes) : nullptr;
-  const size_t lds = (size_t)kA4Waves * kA4Rows * (HD + 4) * 4;
+  const size_t lds = p.few ? (size_t)kA4Waves * kA4Rows * (HD + 4) * 4
+                           : (size_t)4 * kv4_step_blocks(HD) * (HD / 16) * 64 * sizeof(half8v);
   if (int rc = require_lds("attention_kv4", lds + 2048)) return rc;
-  const dim3 grid((unsigned)p.slices, (unsigned)p.tiles, (unsigned)NKV), block(64 * kA4Waves);
+  const dim3 grid = p.few ? dim3((unsigned)p.slices, (unsigned)p.tiles, (unsigned)NKV) : dim3((unsigned)NKV, (unsigned)p.tiles, (unsigned)p.slices);
   const hipStream_t st = static_cast<hipStream_t>(stream);
 #define MIQ_A4(HDV, XT)                                                                                              \
-  hipLaunchKernelGGL((attention_kv4_rows_kernel<HDV, XT>), grid, block, lds, st, static_cast<const XT*>(q),          \
-                     static_cast<const uint8_t*>(cache), state, static_cast<XT*>(out), T, NH, NKV, LMAX, scale, counters, parts)
+  if (p.few)                                                                                                         \
+    hipLaunchKernelGGL((attention_kv4_rows_kernel<HDV, XT>), grid, dim3(64 * kA4Waves), lds, st, static_cast<const XT*>(q), \
+                       static_cast<const uint8_t*>(cache), state, static_cast<XT*>(out), T, NH, NKV, LMAX, scale, counters, parts); \
+  else                                                                                                               \
+    hipLaunchKernelGGL((attention_kv4_tiles_kernel<HDV, XT>), grid, dim3(64 * kA4TileWaves), lds, st, static_cast<const XT*>(q), \
+                       static_cast<const uint8_t*>(cache), state, static_cast<XT*>(out), T, NH, NKV, LMAX, scale, counters, parts)
 #define MIQ_A4_HD(XT)                 \
   switch (HD) {                       \
     case 64: MIQ_A4(64, XT); break;   \
