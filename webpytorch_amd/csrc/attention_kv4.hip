@@ -377,8 +377,9 @@ __global__ __launch_bounds__(64 * kA4TileWaves, 2) void attention_kv4_tiles_kern
     int T, int NH, int NKV, int LMAX, float scale, int* __restrict__ counters, float* __restrict__ parts) {
   constexpr int P = sizeof(XT) == 4 ? 2 : 1, NJ = HD / 32, NT = HD / 16, QT = kv4_tile_qt(HD), NBK = kv4_step_blocks(HD);
   constexpr int RW = 16 * QT, QR = kv4_tile_rows(HD);
-  constexpr int HALF = NBK * NT / 4, GROUPS = 2 * HALF, GPW = (GROUPS + kA4TileWaves - 1) / kA4TileWaves;
-  extern __shared__ __align__(16) half8v ops[];  // [2][K, V][NBK NT][64]
+  constexpr int WPW = NBK * NT / kA4TileWaves;      // words of K, and of V, that a lane unpacks per step
+  constexpr int NM = WPW % 2 ? WPW : WPW / 2;       // sets of S and Z of those of V (two adjacent tiles share one)
+  extern __shared__ __align__(16) half8v ops[];  // [2 of K, 2 of V][NBK NT][64]
   __shared__ uint32_t flags[2][kA4TileWaves], hits[2][NBK][NJ];
   __shared__ int last;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
@@ -396,82 +397,75 @@ __global__ __launch_bounds__(64 * kA4TileWaves, 2) void attention_kv4_tiles_kern
   const int s0 = slice * per, s1 = min(steps, s0 + per);
   const int nblk = (S + kKv4Block - 1) / kKv4Block;
 
-  // ---- words of a step on their way: group x of 64 x 16 bytes, K groups first ----
-  uint4 rw4[GPW], rm[GPW][4];
-  auto fetch = [&](int step) __attribute__((always_inline)) {
+  // ---- words on their way: numbers n0 .. of a step's K and V words ----
+  const int n0 = wave * WPW % NT, bo = wave * WPW / NT;
+  uint32_t kw[WPW], km[WPW], vw[WPW], vm[NM][8];
+  auto words = [&](const uint8_t* part, uint32_t* w) __attribute__((always_inline)) {
+    const uint8_t* at = part + kv4_word(n0, g, c);
+    if constexpr (WPW == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(at);
+    else if constexpr (WPW == 4) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(at);
+    else
 #pragma unroll
-    for (int x = 0; x < GPW; ++x) {
-      const int gi = wave + x * kA4TileWaves;
-      if (GROUPS % kA4TileWaves && gi >= GROUPS) break;
-      const int gg = gi % HALF, u = gg % (NT / 4);
-      const uint8_t* rec = C + (size_t)min(step * NBK + gg / (NT / 4), nblk - 1) * kv4_record(HD);
-      if (gi < HALF) {
-        rw4[x] = *reinterpret_cast<const uint4*>(rec + (u * 64 + lane) * 16);
-        if constexpr (NJ % 4 == 0) {
-          rm[x][0] = *reinterpret_cast<const uint4*>(rec + kv4_kmeta(HD) + ((16 * (4 * u / NJ) + c) * NJ + 4 * u % NJ) * 4);
-        } else {
-          uint2 m[2];
+      for (int x = 0; x < WPW; ++x) w[x] = *reinterpret_cast<const uint32_t*>(part + kv4_word(n0 + x, g, c));
+  };
+  auto fetch_k = [&](int step) __attribute__((always_inline)) {
+    const uint8_t* rec = C + (size_t)min(step * NBK + bo, nblk - 1) * kv4_record(HD);
+    words(rec, kw);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int n = 4 * u + 2 * i;
-            m[i] = *reinterpret_cast<const uint2*>(rec + kv4_kmeta(HD) + ((16 * (n / NJ) + c) * NJ + n % NJ) * 4);
-          }
-          rm[x][0] = make_uint4(m[0].x, m[0].y, m[1].x, m[1].y);
+    for (int x = 0; x < WPW; ++x)
+      km[x] = *reinterpret_cast<const uint32_t*>(rec + kv4_kmeta(HD) + ((16 * ((n0 + x) / NJ) + c) * NJ + (n0 + x) % NJ) * 4);
+  };
+  auto fetch_v = [&](int step) __attribute__((always_inline)) {
+    const uint8_t* rec = C + (size_t)min(step * NBK + bo, nblk - 1) * kv4_record(HD);
+    words(rec + kv4_vcodes(HD), vw);
+#pragma unroll
+    for (int x = 0; x < NM; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        *reinterpret_cast<uint4*>(&vm[x][4 * y]) =
+            *reinterpret_cast<const uint4*>(rec + kv4_vmeta(HD) + (((n0 + x * (WPW / NM)) / 2 * 4 + g) * 2 + y) * 16);
+  };
+  // S and Z of step's values made fit: keys behind the last one hold anything and are cleared; so are groups
+  // with a NaN or an infinity, which are noted for the rows
+  auto check_v = [&](int step) __attribute__((always_inline)) {
+    const int k0 = (step * NBK + bo) * kKv4Block;
+    if (k0 + kKv4Block > S) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const uint32_t keep = keep_pair(k0 + kv4_key(g, 2 * p), S);
+#pragma unroll
+        for (int x = 0; x < NM; ++x) {
+          vm[x][p] &= keep;
+          vm[x][4 + p] &= keep;
         }
-      } else {
-        rw4[x] = *reinterpret_cast<const uint4*>(rec + kv4_vcodes(HD) + (u * 64 + lane) * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          rm[x][i] = *reinterpret_cast<const uint4*>(rec + kv4_vmeta(HD) + ((2 * u + (i >> 1)) * 4 + g) * 32 + 16 * (i & 1));
       }
     }
-  };
-  auto stage = [&](int step, int buf) __attribute__((always_inline)) {
-    uint32_t odd = 0;
+    uint32_t neg = 0;
 #pragma unroll
-    for (int x = 0; x < GPW; ++x) {
-      const int gi = wave + x * kA4TileWaves;
-      if (GROUPS % kA4TileWaves && gi >= GROUPS) break;
-      const int gg = gi % HALF, u = gg % (NT / 4), bo = gg / (NT / 4);
-      half8v* dst = ops + ((size_t)(buf * 2 + (gi >= HALF)) * NBK * NT + bo * NT + 4 * u) * 64 + lane;
-      const uint32_t* w = &rw4[x].x;
-      if (gi < HALF) {
-        const uint32_t* m = &rm[x][0].x;
+    for (int x = 0; x < NM; ++x)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) dst[n * 64] = unpack_key(w[n], m[n]);
-      } else {
-        const int k0 = (step * NBK + bo) * kKv4Block;
-        if (k0 + kKv4Block > S) {  // keys behind the last one hold anything
+      for (int p = 0; p < 4; ++p) neg |= vm[x][p];
+    const bool bad = __ballot((neg & 0x80008000u) != 0) != 0ull;
+    uint32_t hit[NM] = {};
+    if (bad)
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            const uint32_t keep = keep_pair(k0 + kv4_key(g, 2 * p), S);
+      for (int x = 0; x < NM; ++x) hit[x] = clear_bad(&vm[x][0], &vm[x][4]);
+    if (lane == 0) {
+      flags[step & 1][wave] = bad;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) (&rm[x][i].x)[p] &= keep;
-          }
-        }
-        // groups with a NaN or an infinity (S negative) are cleared, and noted for the rows
-        uint32_t neg = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i += 2)
-#pragma unroll
-          for (int p = 0; p < 4; ++p) neg |= (&rm[x][i].x)[p];
-        if (__ballot((neg & 0x80008000u) != 0)) {
-          odd = 1;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t hit = clear_bad(&rm[x][2 * i].x, &rm[x][2 * i + 1].x);
-            if (lane == 0) hits[buf][bo][2 * u + i] = hit;
-          }
-        } else if (lane < 2) {
-          hits[buf][bo][2 * u + lane] = 0;
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) dst[n * 64] = unpack_value(w[n], &rm[x][2 * (n >> 1)].x, &rm[x][2 * (n >> 1) + 1].x);
-      }
+      for (int x = 0; x < NM; ++x) hits[step & 1][bo][(n0 + x * (WPW / NM)) / 2] = hit[x];
     }
-    if (lane == 0) flags[buf][wave] = odd;
   };
-  if (s0 < s1) fetch(s0);
+  auto stage_k = [&](int step) __attribute__((always_inline)) {
+    half8v* dst = ops + ((size_t)(step & 1) * NBK * NT + wave * WPW) * 64 + lane;
+#pragma unroll
+    for (int x = 0; x < WPW; ++x) dst[x * 64] = unpack_key(kw[x], km[x]);
+  };
+  auto stage_v = [&](int step) __attribute__((always_inline)) {
+    half8v* dst = ops + ((size_t)(2 + (step & 1)) * NBK * NT + wave * WPW) * 64 + lane;
+#pragma unroll
+    for (int x = 0; x < WPW; ++x) dst[x * 64] = unpack_value(vw[x], &vm[x * NM / WPW][0], &vm[x * NM / WPW][4]);
+  };
 
   // ---- q as matrix-core operands; scores in units of log 2, their factor positive ----
   half8v qh[QT][P][NJ];
@@ -483,111 +477,138 @@ __global__ __launch_bounds__(64 * kA4TileWaves, 2) void attention_kv4_tiles_kern
     lim[i] = last_key(r);
     load_q<HD, XT>(q + ((size_t)(r / rep) * NH + kv * rep + r % rep) * HD + 8 * g, scale, qh[i], back[i]);
   }
-  const int first = last_key(min(rw, R - 1)), wlast = last_key(min(rw + RW, R) - 1);
+  const int first = last_key(min(rw, R - 1));
 
-  float4v o[QT][NT];
+  float4v o[QT][NT], s[QT][2 * NBK];
   float4v l[QT];  // the sum of probabilities, in every row of the product
-  float m[QT];
+  float m[QT], neg[QT];  // the reference, and what is added to a score for the exponent
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     m[i] = -INFINITY;
+    neg[i] = kA4TileUnitLog2;
     l[i] = (float4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[i][n] = (float4v){0.f, 0.f, 0.f, 0.f};
   }
-  if (s0 < s1) stage(s0, 0);
-  if (s0 + 1 < s1) fetch(s0 + 1);
-  __syncthreads();
-  for (int step = s0; step < s1; ++step) {
-    const int buf = (step - s0) & 1;
-    const half8v* kf = ops + (size_t)buf * 2 * NBK * NT * 64 + lane;
-    const half8v* vf = kf + (size_t)NBK * NT * 64;
-    const bool live = rw < R && step * NBK * kKv4Block <= wlast;  // wave-uniform
-    float4v s[QT][2 * NBK];
-    if (live) {
+  auto scores = [&](int step) __attribute__((always_inline)) {
+    const half8v* kf = ops + (size_t)(step & 1) * NBK * NT * 64 + lane;
 #pragma unroll
-      for (int b = 0; b < 2 * NBK; ++b) {
+    for (int b = 0; b < 2 * NBK; ++b) {
 #pragma unroll
-        for (int i = 0; i < QT; ++i) s[i][b] = (float4v){0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < QT; ++i) s[i][b] = (float4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const half8v k = kf[(b * NJ + j) * 64];
-#pragma unroll
-          for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-            for (int i = 0; i < QT; ++i) s[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[i][p][j], s[i][b], 0, 0, 0);
-        }
-      }
-    }
-    if (step + 1 < s1) {
-      stage(step + 1, buf ^ 1);
-      if (step + 2 < s1) fetch(step + 2);
-    }
-    if (live) {
-      half8v ph[QT][NBK][P];
-      const int k0 = step * NBK * kKv4Block;
-      const bool masked = k0 + NBK * kKv4Block - 1 > first;  // wave-uniform
-#pragma unroll
-      for (int i = 0; i < QT; ++i) {
-        if (masked) {
-#pragma unroll
-          for (int b = 0; b < 2 * NBK; ++b)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (k0 + 16 * b + 4 * g + x > lim[i]) s[i][b][x] = -INFINITY;
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < 2 * NBK; ++b)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) mx = fmaxf(mx, s[i][b][x]);
-        mx = rows_max(mx) * back[i];
-        if (__ballot(mx > m[i] + kA4Slack)) {  // m = -inf: always
-          const float mn = fmaxf(m[i], mx);
-          const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i] - mn);
-          m[i] = mn;
-          l[i] *= alpha;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) o[i][n] *= alpha;
-        }
-        const float ref = (m[i] == -INFINITY ? 0.f : m[i]) - kA4TileUnitLog2;  // no key yet: every probability is 0
-#pragma unroll
-        for (int b = 0; b < NBK; ++b) {
-          float p[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[i][2 * b + (e >> 2)][e & 3], back[i], -ref));
-          split_p<P>(p, ph[i][b]);
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < NBK; ++b)
+      for (int j = 0; j < NJ; ++j) {
+        const half8v k = kf[(b * NJ + j) * 64];
 #pragma unroll
         for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-          for (int i = 0; i < QT; ++i) l[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones(), ph[i][b][p], l[i], 0, 0, 0);
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int b = 0; b < NBK; ++b) {
-          const half8v v = vf[(b * NT + n) * 64];
-#pragma unroll
-          for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-            for (int i = 0; i < QT; ++i) o[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[i][b][p], o[i][n], 0, 0, 0);
-        }
-      if (uniform((int)(flags[buf][0] | flags[buf][1] | flags[buf][2] | flags[buf][3]))) {
-#pragma unroll
-        for (int b = 0; b < NBK; ++b)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int i = 0; i < QT; ++i)
-              if (hits[buf][b][j] & attends(k0 + kKv4Block * b, lim[i])) {
-                o[i][2 * j] += NAN;
-                o[i][2 * j + 1] += NAN;
-              }
+          for (int i = 0; i < QT; ++i) s[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[i][p][j], s[i][b], 0, 0, 0);
       }
     }
+  };
+  // masks the scores of `step` and raises the references they need
+  auto refer = [&](int step) __attribute__((always_inline)) {
+    const int k0 = step * NBK * kKv4Block;
+    if (k0 + NBK * kKv4Block - 1 > first) {  // wave-uniform
+#pragma unroll
+      for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int b = 0; b < 2 * NBK; ++b)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (k0 + 16 * b + 4 * g + x > lim[i]) s[i][b][x] = -INFINITY;
+    }
+    float mx[QT];
+    bool raise = false;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      mx[i] = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2 * NBK; ++b)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) mx[i] = fmaxf(mx[i], s[i][b][x]);
+      mx[i] = rows_max(mx[i]) * back[i];
+      raise |= mx[i] > m[i] + kA4Slack;  // m = -inf: any score
+    }
+    if (__ballot(raise)) {
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
+        const float mn = fmaxf(m[i], mx[i]);
+        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i] - mn);
+        m[i] = mn;
+        neg[i] = kA4TileUnitLog2 - (mn == -INFINITY ? 0.f : mn);  // no key yet: every probability is 0
+        l[i] *= alpha;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[i][n] *= alpha;
+      }
+    }
+  };
+
+  // K runs a step ahead of V: in step t the waves multiply K(t + 1) and V(t), unpack K(t + 2) and V(t + 1), and
+  // load the words after those. Words past the slice are loaded (from the last record) and not used.
+  if (s0 < s1) {
+    fetch_k(s0);
+    fetch_v(s0);
+    stage_k(s0);
+    fetch_k(s0 + 1);
+    check_v(s0);
+    stage_v(s0);
+    fetch_v(s0 + 1);
+    __syncthreads();
+    scores(s0);
+    stage_k(s0 + 1);
+    fetch_k(s0 + 2);
+    refer(s0);
+    __syncthreads();
+  }
+  for (int step = s0; step < s1; ++step) {
+    check_v(step + 1);
+    const half8v* vf = ops + (size_t)(2 + (step & 1)) * NBK * NT * 64 + lane;
+    half8v ph[QT][NBK][P];
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+      for (int b = 0; b < NBK; ++b) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[i][2 * b + (e >> 2)][e & 3], back[i], neg[i]));
+        split_p<P>(p, ph[i][b]);
+      }
+    scores(step + 1);
+    stage_k(step + 2);
+    stage_v(step + 1);
+    fetch_k(step + 3);
+    fetch_v(step + 2);
+#pragma unroll
+    for (int b = 0; b < NBK; ++b)
+#pragma unroll
+      for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < QT; ++i) l[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones(), ph[i][b][p], l[i], 0, 0, 0);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int b = 0; b < NBK; ++b) {
+        const half8v v = vf[(b * NT + n) * 64];
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+          for (int i = 0; i < QT; ++i) o[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[i][b][p], o[i][n], 0, 0, 0);
+      }
+    const int fb = step & 1;
+    if (uniform((int)(flags[fb][0] | flags[fb][1] | flags[fb][2] | flags[fb][3]))) {
+#pragma unroll
+      for (int b = 0; b < NBK; ++b)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < QT; ++i)
+            if (hits[fb][b][j] & attends((step * NBK + b) * kKv4Block, lim[i])) {
+              o[i][2 * j] += NAN;
+              o[i][2 * j + 1] += NAN;
+            }
+    }
+    if (step + 1 < s1) refer(step + 1);
     __syncthreads();
   }
 
