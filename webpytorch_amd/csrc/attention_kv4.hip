@@ -367,21 +367,29 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
 constexpr int kA4TileWaves = 4;
 constexpr float kA4TileUnitLog2 = 7.f;  // a probability of 1 is 2^7 at the reference
 constexpr float kA4Slack = 8.f;
-__host__ __device__ constexpr int kv4_step_blocks(int HD) { return HD == 64 ? 2 : 1; }
-__host__ __device__ constexpr int kv4_tile_qt(int HD) { return HD <= 128 ? 2 : 1; }
-__host__ __device__ constexpr int kv4_tile_rows(int HD) { return kA4TileWaves * 16 * kv4_tile_qt(HD); }
+// blocks of a step and 16-row tiles of a wave: what the registers hold (fp32 rows take twice the operands)
+__host__ __device__ constexpr int kv4_step_blocks(int HD, bool f32) { return HD == 64 ? 2 : HD == 128 && !f32 ? 2 : 1; }
+__host__ __device__ constexpr int kv4_tile_qt(int HD, bool f32) { return HD <= 128 && !f32 ? 2 : 1; }
+__host__ __device__ constexpr int kv4_tile_rows(int HD, bool f32) { return kA4TileWaves * 16 * kv4_tile_qt(HD, f32); }
+
+// Slices of `steps` key steps, of `per` steps each
+__device__ __forceinline__ int tile_slices(int steps, int most, int& per) {
+  per = max(kA4MinSteps, (steps + most - 1) / most);
+  return max(1, (steps + per - 1) / per);
+}
+// float4s of a slice's part: per 16 rows the lanes' outputs [HD / 16][64] and (maximum, sum) of its rows
+__host__ __device__ constexpr int kv4_part_unit(int HD) { return HD * 4 + 8; }
 
 template <int HD, typename XT>
-__global__ __launch_bounds__(64 * kA4TileWaves, 2) void attention_kv4_tiles_kernel(
+__global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3 : 2) void attention_kv4_tiles_kernel(
     const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ state, XT* __restrict__ out,
-    int T, int NH, int NKV, int LMAX, float scale, int* __restrict__ counters, float* __restrict__ parts) {
-  constexpr int P = sizeof(XT) == 4 ? 2 : 1, NJ = HD / 32, NT = HD / 16, QT = kv4_tile_qt(HD), NBK = kv4_step_blocks(HD);
-  constexpr int RW = 16 * QT, QR = kv4_tile_rows(HD);
+    int T, int NH, int NKV, int LMAX, float scale, float4v* __restrict__ parts) {
+  constexpr int P = sizeof(XT) == 4 ? 2 : 1, NJ = HD / 32, NT = HD / 16, QT = kv4_tile_qt(HD, P == 2), NBK = kv4_step_blocks(HD, P == 2);
+  constexpr int RW = 16 * QT, QR = kv4_tile_rows(HD, P == 2);
   constexpr int WPW = NBK * NT / kA4TileWaves;      // words of K, and of V, that a lane unpacks per step
   constexpr int NM = WPW % 2 ? WPW : WPW / 2;       // sets of S and Z of those of V (two adjacent tiles share one)
   extern __shared__ __align__(16) half8v ops[];  // [2 of K, 2 of V][NBK NT][64]
   __shared__ uint32_t flags[2][kA4TileWaves], hits[2][NBK][NJ];
-  __shared__ int last;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int kv = blockIdx.x, tile = (int)gridDim.y - 1 - (int)blockIdx.y, slice = blockIdx.z, rep = NH / NKV;  // long tiles first
   const int R = T * rep, r0 = tile * QR, rw = r0 + wave * RW;
@@ -391,8 +399,8 @@ __global__ __launch_bounds__(64 * kA4TileWaves, 2) void attention_kv4_tiles_kern
   const auto last_key = [&](int r) { return (int)min(pos0 + r / rep, (int64_t)LMAX - 1); };  // below 0: none
   const int S = max(0, last_key(min(r0 + QR, R) - 1) + 1);  // keys that any row attends to
   const int steps = (S + kKv4Block * NBK - 1) / (kKv4Block * NBK);
-  const int per = max(kA4MinSteps, (steps + (int)gridDim.z - 1) / (int)gridDim.z);
-  const int slices = max(1, (steps + per - 1) / per);
+  int per;
+  const int slices = tile_slices(steps, gridDim.z, per);
   if (slice >= slices) return;
   const int s0 = slice * per, s1 = min(steps, s0 + per);
   const int nblk = (S + kKv4Block - 1) / kKv4Block;
@@ -613,51 +621,101 @@ __global__ __launch_bounds__(64 * kA4TileWaves, 2) void attention_kv4_tiles_kern
   }
 
   // ---- out, or the slice's part ----
-  float* part = slices > 1 ? parts + ((size_t)(kv * gridDim.y + tile) * gridDim.z + slice) * QR * (HD + 4) : nullptr;
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const float sum = l[i][0];
     const int r = rw + 16 * i + c;
-    if (r >= R) continue;
     if (slices > 1) {
-      float* pr = part + (size_t)(r - r0) * (HD + 4);
+      float4v* part = parts + (((size_t)(kv * gridDim.y + tile) * (QR / 16) + wave * QT + i) * gridDim.z + slice) * kv4_part_unit(HD);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2)
-          put2(pr + 16 * n + 4 * g + e, o[i][n][e], o[i][n][e + 1]);
-      if (g == 0) put2(pr + HD, m[i], sum);
+      for (int n = 0; n < NT; ++n) part[n * 64 + lane] = o[i][n];
+      if (g == 0) reinterpret_cast<float2*>(part + NT * 64)[c] = make_float2(m[i], sum);
       continue;
     }
+    if (r >= R) continue;
     XT* orow = out + ((size_t)(r / rep) * NH + kv * rep + r % rep) * HD + 4 * g;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) orow[16 * n + e] = from_f32<XT>(sum == 0.f ? 0.f : o[i][n][e] / sum);  // a row without keys: zeros
   }
-  if (slices == 1) return;
-  if (!last_slice(counters + (kv * gridDim.y + tile) * kA4CtrStride, slices, &last)) return;
-  join_slices<HD, XT, 64 * kA4TileWaves>(parts + (size_t)(kv * gridDim.y + tile) * gridDim.z * QR * (HD + 4), (size_t)QR * (HD + 4),
-                                         slices, out, r0, min(QR, R - r0), rep, kv, NH);
+}
+
+// The parts of a tile's slices, added in slice order: a workgroup takes 16 rows, its waves a quarter of the
+// dimensions each. (In a launch of its own: one workgroup's last arrival would read all of a tile's parts alone.)
+template <int HD, typename XT>
+__global__ __launch_bounds__(256) void attention_kv4_join_kernel(const int32_t* __restrict__ state, const float4v* __restrict__ parts,
+                                                                 XT* __restrict__ out, int T, int NH, int NKV, int LMAX, int most) {
+  constexpr int NT = HD / 16, NW = NT / 4, QR = kv4_tile_rows(HD, sizeof(XT) == 4), STEP = kKv4Block * kv4_step_blocks(HD, sizeof(XT) == 4);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int kv = blockIdx.y, unit = blockIdx.x, tile = unit / (QR / 16), rep = NH / NKV, R = T * rep, r = unit * 16 + c;
+  const int64_t pos0 = state[0];
+  const int S = max(0, (int)min(pos0 + (min((tile + 1) * QR, R) - 1) / rep, (int64_t)LMAX - 1) + 1);
+  int per;
+  const int slices = tile_slices((S + STEP - 1) / STEP, most, per);
+  if (slices == 1 || unit * 16 >= R) return;
+  const float4v* part = parts + ((size_t)kv * gridDim.x + unit) * most * kv4_part_unit(HD);
+  float mx = -INFINITY, sum = 0.f;
+  float4v a[NW];
+#pragma unroll
+  for (int n = 0; n < NW; ++n) a[n] = (float4v){0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 4;
+  for (int k0 = 0; k0 < slices; k0 += U) {
+    float2 st[U];
+    float4v v[U][NW];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const float4v* pk = part + (size_t)min(k0 + i, slices - 1) * kv4_part_unit(HD);
+      st[i] = reinterpret_cast<const float2*>(pk + NT * 64)[c];
+#pragma unroll
+      for (int n = 0; n < NW; ++n) v[i][n] = pk[(wave * NW + n) * 64 + lane];
+    }
+    float mn = mx;
+#pragma unroll
+    for (int i = 0; i < U; ++i) mn = fmaxf(mn, st[i].x);
+    const float ref = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(mx - ref);
+    mx = mn;
+    sum *= al;
+#pragma unroll
+    for (int n = 0; n < NW; ++n) a[n] *= al;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (k0 + i < slices) {
+        const float f = __builtin_amdgcn_exp2f(st[i].x - ref);
+        sum = fmaf(f, st[i].y, sum);
+#pragma unroll
+        for (int n = 0; n < NW; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[n][e] = fmaf(f, v[i][n][e], a[n][e]);
+      }
+  }
+  if (r >= R) return;
+  XT* orow = out + ((size_t)(r / rep) * NH + kv * rep + r % rep) * HD + 4 * g;
+#pragma unroll
+  for (int n = 0; n < NW; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) orow[16 * (wave * NW + n) + e] = from_f32<XT>(sum == 0.f ? 0.f : a[n][e] / sum);
 }
 
 // Up to kA4FewRows rows of a kv head go by the rows kernel, more by the tiles kernel. Each tile's keys are
-// split into as many slices as give every CU a workgroup, of at least a block a wave (8 steps) of a full cache.
+// split into as many slices as give every CU a workgroup (two of the tiles kernel's), of at least a block a
+// wave (8 steps) of a full cache.
 constexpr int kA4FewRows = 48;
 struct Kv4Plan {
   int tiles, slices, rows;  // rows of a tile
   bool few;
 };
-static Kv4Plan kv4_plan(int T, int NH, int NKV, int HD, int LMAX) {
+static Kv4Plan kv4_plan(int T, int NH, int NKV, int HD, int LMAX, bool f32) {
   Kv4Plan p;
   const int64_t R = (int64_t)T * (NH / NKV);
   p.few = R <= kA4FewRows;
-  p.rows = p.few ? kA4Rows : kv4_tile_rows(HD);
+  p.rows = p.few ? kA4Rows : kv4_tile_rows(HD, f32);
   p.tiles = (int)((R + p.rows - 1) / p.rows);
   const int64_t wgs = (int64_t)p.tiles * NKV;
-  const int steps = p.few ? kv4_blocks(LMAX) : (kv4_blocks(LMAX) + kv4_step_blocks(HD) - 1) / kv4_step_blocks(HD);
+  const int steps = p.few ? kv4_blocks(LMAX) : (kv4_blocks(LMAX) + kv4_step_blocks(HD, f32) - 1) / kv4_step_blocks(HD, f32);
   const int least = p.few ? kA4Waves : kA4MinSteps;
-  int64_t s = wgs >= kCUs ? 1 : kCUs / wgs;
+  const int want = p.few ? kCUs : 2 * kCUs;
+  int64_t s = wgs >= want ? 1 : want / wgs;
   if (s > (steps + least - 1) / least) s = (steps + least - 1) / least;
   if (s > kA4MaxSlices) s = kA4MaxSlices;
   p.slices = (int)s;
@@ -665,7 +723,8 @@ static Kv4Plan kv4_plan(int T, int NH, int NKV, int HD, int LMAX) {
 }
 
 static size_t kv4_part_bytes(const Kv4Plan& p, int NKV, int HD) {
-  return p.slices > 1 ? (size_t)p.slices * p.tiles * NKV * p.rows * (HD + 4) * 4 : 0;
+  if (p.slices == 1) return 0;
+  return (size_t)p.slices * p.tiles * NKV * (p.few ? (size_t)p.rows * (HD + 4) * 4 : (size_t)p.rows / 16 * kv4_part_unit(HD) * 16);
 }
 
 }  // namespace miq
@@ -676,7 +735,7 @@ static int check_attention_kv4(const char* what, int T, int NH, int NKV, int HD,
   MIQ_REQUIRE(T >= 0 && NH > 0 && NKV > 0 && NH % NKV == 0 && NH <= (1 << 16) && NKV <= 65535 && HD > 0 && LMAX > 0 && LMAX <= (1 << 30),
               MIQ_ERR_INVALID, "%s: T=%d NH=%d NKV=%d HD=%d LMAX=%d", what, T, NH, NKV, HD, LMAX);
   MIQ_REQUIRE(kv4_head(HD), MIQ_ERR_UNSUPPORTED, "%s: HD=%d (64, 128, 192 or 256)", what, HD);
-  MIQ_REQUIRE((int64_t)T * (NH / NKV) <= (int64_t)65535 * kv4_tile_rows(HD), MIQ_ERR_UNSUPPORTED, "%s: T=%d rows of %d heads a kv head are past the grid",
+  MIQ_REQUIRE((int64_t)T * (NH / NKV) <= (int64_t)65535 * 16 * kA4TileWaves, MIQ_ERR_UNSUPPORTED, "%s: T=%d rows of %d heads a kv head are past the grid",
               what, T, NH / NKV);
   return MIQ_OK;
 }
@@ -686,8 +745,9 @@ extern "C" int miq_attention_kv4_workspace(int T, int NH, int NKV, int HD, int L
   if (int rc = check_attention_kv4("attention_kv4_workspace", T, NH, NKV, HD, LMAX)) return rc;
   *bytes = 0;
   if (T == 0) return MIQ_OK;
-  const size_t part = kv4_part_bytes(kv4_plan(T, NH, NKV, HD, LMAX), NKV, HD);
-  *bytes = part ? kCounterBytes + part : 0;
+  const size_t a = kv4_part_bytes(kv4_plan(T, NH, NKV, HD, LMAX, true), NKV, HD);
+  const size_t b = kv4_part_bytes(kv4_plan(T, NH, NKV, HD, LMAX, false), NKV, HD);
+  *bytes = a || b ? kCounterBytes + (a > b ? a : b) : 0;  // of either type of rows
   return MIQ_OK;
 }
 
@@ -699,7 +759,8 @@ extern "C" int miq_attention_kv4(const void* q, int x_dtype, const void* cache, 
   if (T == 0) return MIQ_OK;
   MIQ_REQUIRE(q && cache && state && out, MIQ_ERR_INVALID, "attention_kv4: null pointer");
   MIQ_REQUIRE(aligned(cache, 16), MIQ_ERR_ALIGN, "attention_kv4: the cache must be 16-byte aligned");
-  const Kv4Plan p = kv4_plan(T, NH, NKV, HD, LMAX);
+  const bool f32 = x_dtype == MIQ_F32;
+  const Kv4Plan p = kv4_plan(T, NH, NKV, HD, LMAX, f32);
   const size_t part = kv4_part_bytes(p, NKV, HD);
   MIQ_REQUIRE(!part || (workspace && ws_bytes >= kCounterBytes + part), MIQ_ERR_INVALID,
               "attention_kv4: workspace of %zu bytes, %zu needed", workspace ? ws_bytes : (size_t)0, kCounterBytes + part);
@@ -707,17 +768,25 @@ extern "C" int miq_attention_kv4(const void* q, int x_dtype, const void* cache, 
   int* counters = static_cast<int*>(workspace);
   float* parts = part ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes) : nullptr;
   const size_t lds = p.few ? (size_t)kA4Waves * kA4Rows * (HD + 4) * 4
-                           : (size_t)4 * kv4_step_blocks(HD) * (HD / 16) * 64 * sizeof(half8v);
+                           : (size_t)4 * kv4_step_blocks(HD, f32) * (HD / 16) * 64 * sizeof(half8v);
   if (int rc = require_lds("attention_kv4", lds + 2048)) return rc;
   const dim3 grid = p.few ? dim3((unsigned)p.slices, (unsigned)p.tiles, (unsigned)NKV) : dim3((unsigned)NKV, (unsigned)p.tiles, (unsigned)p.slices);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  // the join reads what the tiles kernel left in the workspace: another thread's call on the stream waits
+  std::unique_lock<std::mutex> lock(stream_lock(st), std::defer_lock);
+  if (!p.few && part) lock.lock();
 #define MIQ_A4(HDV, XT)                                                                                              \
-  if (p.few)                                                                                                         \
+  if (p.few) {                                                                                                       \
     hipLaunchKernelGGL((attention_kv4_rows_kernel<HDV, XT>), grid, dim3(64 * kA4Waves), lds, st, static_cast<const XT*>(q), \
                        static_cast<const uint8_t*>(cache), state, static_cast<XT*>(out), T, NH, NKV, LMAX, scale, counters, parts); \
-  else                                                                                                               \
+  } else {                                                                                                           \
     hipLaunchKernelGGL((attention_kv4_tiles_kernel<HDV, XT>), grid, dim3(64 * kA4TileWaves), lds, st, static_cast<const XT*>(q), \
-                       static_cast<const uint8_t*>(cache), state, static_cast<XT*>(out), T, NH, NKV, LMAX, scale, counters, parts)
+                       static_cast<const uint8_t*>(cache), state, static_cast<XT*>(out), T, NH, NKV, LMAX, scale,    \
+                       reinterpret_cast<float4v*>(parts));                                                           \
+    if (part)                                                                                                        \
+      hipLaunchKernelGGL((attention_kv4_join_kernel<HDV, XT>), dim3((unsigned)(p.tiles * (p.rows / 16)), (unsigned)NKV), dim3(256), 0, st, \
+                         state, reinterpret_cast<const float4v*>(parts), static_cast<XT*>(out), T, NH, NKV, LMAX, p.slices); \
+  }
 #define MIQ_A4_HD(XT)                 \
   switch (HD) {                       \
     case 64: MIQ_A4(64, XT); break;   \
