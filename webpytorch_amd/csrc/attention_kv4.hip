@@ -102,7 +102,7 @@ __device__ __forceinline__ void join_slices(const float* p0, size_t step, int sl
     const int row = x / (HD / 2), d = 2 * (x % (HD / 2));
     const float* pr = p0 + (size_t)row * (HD + 4);
     float mx = -INFINITY, sum = 0.f, a[2] = {0.f, 0.f};
-    constexpr int U = 8;
+    constexpr int U = 16;
     for (int k0 = 0; k0 < slices; k0 += U) {
       uint64_t st[U], v[U];
 #pragma unroll
@@ -192,48 +192,58 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
   const int t = r / rep, h = kv * rep + r % rep;
   const uint8_t* C = cache + (size_t)kv * kv4_blocks(LMAX) * kv4_record(HD);
 
-  half8v qh[P][NJ];
-  float back;
-  load_q<HD, XT>(q + ((size_t)t * NH + h) * HD + 8 * g, scale, qh, back);
-
   const int64_t pos0 = state[0];
   const int lim = (int)(pos0 + t < LMAX ? pos0 + t : LMAX - 1);  // this row's last key
   const int tl = (min(r0 + QR, R) - 1) / rep, tf = r0 / rep;
   const int S = (int)max((int64_t)0, min(pos0 + tl, (int64_t)LMAX - 1) + 1);  // keys that any row attends to
   const int first = (int)min(pos0 + tf, (int64_t)LMAX - 1);                   // the smallest last key
   const int nblk = (S + kKv4Block - 1) / kKv4Block;
-  // blocks of a slice: at least one a wave
-  const int per = max(NW, (nblk + (int)gridDim.x - 1) / (int)gridDim.x);
+  // blocks of a slice: joining costs 3 us or more, so that up to 3 blocks a wave are one slice (700 positions of 2
+  // heads of 64: 8.6 -> 7.5 us), and from 512 blocks on a slice has two a wave (16000 positions: 14.7 -> 12.5 us)
+  const int per = nblk <= 3 * NW ? 3 * NW : max(nblk >= 512 ? 2 * NW : NW, (nblk + (int)gridDim.x - 1) / (int)gridDim.x);
   const int slices = max(1, (nblk + per - 1) / per);
   if (slice >= slices) return;
-  const int b1 = min(nblk, (slice + 1) * per);
+  const int b0 = slice * per, b1 = min(nblk, b0 + per);
+
+  // ---- a block's words: the next one's are loaded while one is multiplied, where the registers hold both ----
+  constexpr int NR = HD <= 128 ? 2 : 1;
+  struct Raw {
+    uint32_t kw[NT], vw[NT], km[2][NJ], vm[NJ][8];
+  } raw[NR];
+  auto load = [&](Raw& x, int blk) __attribute__((always_inline)) {
+    const uint8_t* rec = C + (size_t)blk * kv4_record(HD);
+#pragma unroll
+    for (int u = 0; u < NT / 4; ++u) *reinterpret_cast<uint4*>(&x.kw[4 * u]) = *reinterpret_cast<const uint4*>(rec + (u * 64 + lane) * 16);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < NJ; j += 2)
+        *reinterpret_cast<uint2*>(&x.km[b][j]) = *reinterpret_cast<const uint2*>(rec + kv4_kmeta(HD) + ((16 * b + c) * NJ + j) * 4);
+#pragma unroll
+    for (int u = 0; u < NT / 4; ++u)
+      *reinterpret_cast<uint4*>(&x.vw[4 * u]) = *reinterpret_cast<const uint4*>(rec + kv4_vcodes(HD) + (u * 64 + lane) * 16);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        *reinterpret_cast<uint4*>(&x.vm[j][4 * u]) = *reinterpret_cast<const uint4*>(rec + kv4_vmeta(HD) + (j * 4 + g) * 32 + 16 * u);
+  };
+  const bool work = b0 + wave < b1;  // wave-uniform
+  if (work) load(raw[0], b0 + wave);
+  half8v qh[P][NJ];
+  float back;
+  load_q<HD, XT>(q + ((size_t)t * NH + h) * HD + 8 * g, scale, qh, back);
 
   float4v o[NT];
   float4v l = (float4v){0.f, 0.f, 0.f, 0.f};  // the sum of probabilities, in every row of the product
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NT; ++i) o[i] = (float4v){0.f, 0.f, 0.f, 0.f};
-  for (int blk = slice * per + wave; blk < b1; blk += NW) {
-    const uint8_t* rec = C + (size_t)blk * kv4_record(HD);
-    uint32_t kw[NT], vw[NT], km[2][NJ], vm[NJ][8];
-#pragma unroll
-    for (int u = 0; u < NT / 4; ++u) {
-      *reinterpret_cast<uint4*>(&kw[4 * u]) = *reinterpret_cast<const uint4*>(rec + (u * 64 + lane) * 16);
-      *reinterpret_cast<uint4*>(&vw[4 * u]) = *reinterpret_cast<const uint4*>(rec + kv4_vcodes(HD) + (u * 64 + lane) * 16);
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int j = 0; j < NJ; j += 2)
-        *reinterpret_cast<uint2*>(&km[b][j]) =
-            *reinterpret_cast<const uint2*>(rec + kv4_kmeta(HD) + ((16 * b + c) * NJ + j) * 4);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        *reinterpret_cast<uint4*>(&vm[j][4 * u]) =
-            *reinterpret_cast<const uint4*>(rec + kv4_vmeta(HD) + (j * 4 + g) * 32 + 16 * u);
-
+  auto multiply = [&](Raw& w, int blk) __attribute__((always_inline)) {
+    auto& kw = w.kw;
+    auto& vw = w.vw;
+    auto& km = w.km;
+    auto& vm = w.vm;
     // ---- scores ----
     float4v s[2];
 #pragma unroll
@@ -309,10 +319,27 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
           o[2 * j] += NAN;
           o[2 * j + 1] += NAN;
         }
+  };
+  if (work) {
+    if constexpr (NR == 2) {
+      for (int blk = b0 + wave;; blk += 2 * NW) {
+        load(raw[1], min(blk + NW, b1 - 1));
+        multiply(raw[0], blk);
+        if (blk + NW >= b1) break;
+        load(raw[0], min(blk + 2 * NW, b1 - 1));
+        multiply(raw[1], blk + NW);
+        if (blk + 2 * NW >= b1) break;
+      }
+    } else {
+      for (int blk = b0 + wave; blk < b1; blk += NW) {
+        if (blk != b0 + wave) load(raw[0], blk);
+        multiply(raw[0], blk);
+      }
+    }
   }
 
   // ---- the waves' parts, rescaled to their common maximum ----
-  const int nw = max(1, min(NW, b1 - slice * per));  // waves that had keys (wave 0 always takes part)
+  const int nw = max(1, min(NW, b1 - b0));  // waves that had keys (wave 0 always takes part)
   const int nr = min(QR, R - r0);
   if (wave < nw) {
     if (g == 0) {
@@ -697,10 +724,14 @@ __global__ __launch_bounds__(256) void attention_kv4_join_kernel(const int32_t* 
     for (int e = 0; e < 4; ++e) orow[16 * (wave * NW + n) + e] = from_f32<XT>(sum == 0.f ? 0.f : a[n][e] / sum);
 }
 
-// Up to kA4FewRows rows of a kv head go by the rows kernel, more by the tiles kernel. Each tile's keys are
+// Up to kA4FewRows rows of a kv head go by the rows kernel, and up to kA4SomeRows where the cache is short: it unpacks
+// a block for 16 rows where the tiles kernel does for 64 or 128, but starts sooner and needs no second launch
+// (32 / 8 heads of 128, us, rows / tiles kernel: 64 rows, 8000 positions 21 / 29, 60000 70 / 70; 256 rows,
+// 0 positions 5.5 / 9.9, 1000 16 / 20, 8000 44 / 42, 60000 230 / 168). The position is the device's, so the rule goes by LMAX. Each tile's keys are
 // split into as many slices as give every CU a workgroup (two of the tiles kernel's), of at least a block a
 // wave (8 steps) of a full cache.
-constexpr int kA4FewRows = 48;
+constexpr int kA4FewRows = 64, kA4SomeRows = 512;
+constexpr int64_t kA4SomeKeys = 1 << 21;  // rows times positions
 struct Kv4Plan {
   int tiles, slices, rows;  // rows of a tile
   bool few;
@@ -708,7 +739,7 @@ struct Kv4Plan {
 static Kv4Plan kv4_plan(int T, int NH, int NKV, int HD, int LMAX, bool f32) {
   Kv4Plan p;
   const int64_t R = (int64_t)T * (NH / NKV);
-  p.few = R <= kA4FewRows;
+  p.few = R <= kA4FewRows || (R <= kA4SomeRows && R * LMAX <= kA4SomeKeys);
   p.rows = p.few ? kA4Rows : kv4_tile_rows(HD, f32);
   p.tiles = (int)((R + p.rows - 1) / p.rows);
   const int64_t wgs = (int64_t)p.tiles * NKV;
