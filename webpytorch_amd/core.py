@@ -874,28 +874,45 @@ MAX_TOP_LOGPROBS = 32
 _CAPTURED_COUNTERS = 1 << 17
 
 
-def _gpu_tensor(name, t, dtypes, dim=None):
-    """Refuse what a kernel would read wrongly: no torch tensor of the current GPU, another dtype or rank."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+def _gpu_of(name, t):
+    """The device index of a torch tensor, which has to be the current GPU's."""
+    d = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if d < 0:
         raise ValueError("%s must be a torch tensor on the GPU" % name)
+    if d != torch.cuda.current_device():
+        raise ValueError("%s is on cuda:%d, the current device is cuda:%d" % (name, d, torch.cuda.current_device()))
+    return d
+
+
+def _check_tensor(name, t, dtypes, dim, dev):
+    """Refuse what a kernel would read wrongly: no tensor on GPU `dev`, another dtype or rank (dim None: any)."""
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and (dim is None or t.dim() == dim) and t.get_device() == dev:
+        return
+    if _gpu_of(name, t) != dev:
+        raise ValueError("%s is on another GPU than the other tensors" % name)
     if t.dtype not in dtypes:
         raise TypeError("%s has dtype %s (%s)" % (name, t.dtype, " or ".join(str(d).replace("torch.", "") for d in dtypes)))
-    if dim is not None and t.dim() != dim:
-        raise ValueError("%s has shape %s: %d dimensions are expected" % (name, tuple(t.shape), dim))
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError("%s is on cuda:%d, the current device is cuda:%d" % (name, t.get_device(), torch.cuda.current_device()))
+    raise ValueError("%s has shape %s: %d dimensions are expected" % (name, tuple(t.shape), dim))
 
 
-def _call_workspace(nbytes):
-    """The workspace of one call: the stream's, or, under graph capture, one of the graph's own, so that two
-    graphs replayed at a time never share one."""
+def _raw_stream(dev):
+    """The current stream's handle, without the Stream object around it (0.1 instead of 2.8 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _call_workspace(nbytes, dev):
+    """(address, bytes) of the workspace of one call: the stream's, or, under graph capture, one of the graph's
+    own, so that two graphs replayed at a time never share one. The third item keeps it alive."""
     if nbytes == 0:
-        return None
-    if not torch.cuda.is_current_stream_capturing():
-        return workspace(nbytes)
-    t = torch.empty(nbytes, dtype=torch.uint8, device=device())
-    t[:_CAPTURED_COUNTERS].zero_()
-    return t
+        return None, 0, None
+    if torch.cuda.is_current_stream_capturing():
+        t = torch.empty(nbytes, dtype=torch.uint8, device=device())
+        t[:_CAPTURED_COUNTERS].zero_()
+    else:
+        t = _WORKSPACE.get((dev, _raw_stream(dev)))
+        if t is None or t.numel() < nbytes:
+            t = workspace(nbytes)
+    return t.data_ptr(), t.numel(), t
 
 
 def _bytes(key, name, *args):
@@ -927,9 +944,9 @@ def kv4_cache(nkv, lmax, hd):
     return torch.zeros((nkv, -(-lmax // KV4_BLOCK), 40 * hd), dtype=torch.uint8, device=device())
 
 
-def _kv4_shape(cache):
+def _kv4_shape(cache, dev):
     """(NKV, positions, HD) of a 4-bit cache tensor."""
-    _gpu_tensor("the 4-bit cache", cache, (torch.uint8,), 3)
+    _check_tensor("the 4-bit cache", cache, (torch.uint8,), 3, dev)
     nkv, nb, rec = cache.shape
     if rec % 40 or rec // 40 not in KV4_HEADS or nb < 1 or nkv < 1 or not cache.is_contiguous():
         raise ValueError("a 4-bit cache is a contiguous (NKV, blocks, 40 HD) tensor, HD 64, 128, 192 or 256: got %s"
@@ -939,12 +956,14 @@ def _kv4_shape(cache):
 
 def kv4_dequant(cache, start=0, n=None):
     """The fp32 keys and values (NKV, n, HD) that positions start .. start + n - 1 of a 4-bit cache stand for."""
-    nkv, lmax, hd = _kv4_shape(cache)
+    dev = _gpu_of("the 4-bit cache", cache)
+    nkv, lmax, hd = _kv4_shape(cache, dev)
     n = lmax - start if n is None else n
     if start < 0 or n < 0 or start + n > lmax:
         raise ValueError("positions %d .. %d of a cache of %d" % (start, start + n - 1, lmax))
-    k, v = (torch.empty((nkv, n, hd), dtype=torch.float32, device=cache.device) for _ in range(2))
-    _lib.call("miq_kv4_dequant_f32", cache.data_ptr(), k.data_ptr(), v.data_ptr(), nkv, lmax, hd, start, n, stream_handle())
+    k = torch.empty((nkv, n, hd), dtype=torch.float32, device=cache.device)
+    v = torch.empty_like(k)
+    _lib.call("miq_kv4_dequant_f32", cache.data_ptr(), k.data_ptr(), v.data_ptr(), nkv, lmax, hd, start, n, _raw_stream(dev))
     return k, v
 
 
@@ -958,14 +977,15 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
     `webtorch/llm.py:1498-1519, 1270-1304`, `webtorch/_core.py:1504-1540`.)"""
     four = isinstance(cache, torch.Tensor)
     f32 = (torch.float32,)
-    _gpu_tensor("qkv", qkv, (torch.float32, torch.float16) if four else f32, 2)
-    _gpu_tensor("state", state, (torch.int32,))
+    dev = _gpu_of("qkv", qkv)
+    _check_tensor("qkv", qkv, (torch.float32, torch.float16) if four else f32, 2, dev)
+    _check_tensor("state", state, (torch.int32,), None, dev)
     if four:
-        nkv, lmax, hd = _kv4_shape(cache)
+        nkv, lmax, hd = _kv4_shape(cache, dev)
     else:
         kc, vc = cache
         for t in (kc, vc):
-            _gpu_tensor("the cache", t, f32, 3)
+            _check_tensor("the cache", t, f32, 3, dev)
         nkv, lmax, hd = kc.shape
         if vc.shape != kc.shape or not kc.is_contiguous() or not vc.is_contiguous():
             raise ValueError("the caches are two contiguous (NKV, LMAX, HD) tensors: got %s and %s" % (tuple(kc.shape), tuple(vc.shape)))
@@ -973,12 +993,12 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
     if n_heads < 1 or n_heads % nkv or W != (n_heads + 2 * nkv) * hd:
         raise ValueError("rows of %d values are not %d query, %d key and %d value heads of %d" % (W, n_heads, nkv, nkv, hd))
     for name, t in (("cos", cos), ("sin", sin)):
-        _gpu_tensor(name, t, f32, 2)
+        _check_tensor(name, t, f32, 2, dev)
         if t.shape[1] * 2 != hd or t.shape[0] < lmax or not t.is_contiguous():
             raise ValueError("%s is a contiguous (positions, %d) table of at least %d positions: got %s" % (name, hd // 2, lmax, tuple(t.shape)))
     for name, t in (("qn", qn), ("kn", kn)):
         if t is not None:
-            _gpu_tensor(name, t, f32, 1)
+            _check_tensor(name, t, f32, 1, dev)
             if t.shape[0] != hd or not t.is_contiguous():
                 raise ValueError("%s has shape %s: (%d,) is expected" % (name, tuple(t.shape), hd))
     if state.numel() < 1:
@@ -988,28 +1008,29 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
     if out is None:
         out = torch.empty((T, n_heads, hd), dtype=qkv.dtype, device=qkv.device)
     else:
-        _gpu_tensor("out", out, (qkv.dtype,))
+        _check_tensor("out", out, (qkv.dtype,), None, dev)
         if out.numel() != T * n_heads * hd or not out.is_contiguous():
             raise ValueError("out is a contiguous tensor of %d values: got %s" % (T * n_heads * hd, tuple(out.shape)))
     ld = qkv.stride(0) if T > 1 else W
     qp, kp = (None if t is None else t.data_ptr() for t in (qn, kn))
     if four:
         _lib.call("miq_qk_norm_rope_kv4", qkv.data_ptr(), dtype_code(qkv), ld, qp, kp, float(eps), state.data_ptr(), cos.data_ptr(),
-                  sin.data_ptr(), out.data_ptr(), cache.data_ptr(), T, n_heads, nkv, hd, lmax, stream_handle())
+                  sin.data_ptr(), out.data_ptr(), cache.data_ptr(), T, n_heads, nkv, hd, lmax, _raw_stream(dev))
     else:
         _lib.call("miq_qk_norm_rope_kv", qkv.data_ptr(), ld, qp, kp, float(eps), state.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-                  out.data_ptr(), kc.data_ptr(), vc.data_ptr(), T, n_heads, nkv, hd, lmax, stream_handle())
+                  out.data_ptr(), kc.data_ptr(), vc.data_ptr(), T, n_heads, nkv, hd, lmax, _raw_stream(dev))
     return out
 
 
-def attention_kv4(q, cache, state, scale=None, out=None, ws=None):
+def attention_kv4(q, cache, state, scale=None, out=None):
     """Causal grouped-query attention of q (T, NH, HD), fp32 or fp16, over a 4-bit cache: token t, at
     position state[0] + t, attends to positions 0 .. state[0] + t; scale is 1 / sqrt(HD) unless given. A token
     whose position is below 0 gets zeros. Returns (T, NH, HD) in q's dtype. (`KVCache.attn`, `gqa_attention`:
     `webtorch/_core.py:1543-1596, 1319-1340`, which keep the cache in fp32.)"""
-    _gpu_tensor("q", q, (torch.float32, torch.float16), 3)
-    _gpu_tensor("state", state, (torch.int32,))
-    nkv, lmax, hd = _kv4_shape(cache)
+    dev = _gpu_of("q", q)
+    _check_tensor("q", q, (torch.float32, torch.float16), 3, dev)
+    _check_tensor("state", state, (torch.int32,), None, dev)
+    nkv, lmax, hd = _kv4_shape(cache, dev)
     T, nh, qd = q.shape
     if qd != hd or nh < 1 or nh % nkv or state.numel() < 1:
         raise ValueError("q %s does not go with a cache of %d heads of %d" % (tuple(q.shape), nkv, hd))
@@ -1017,14 +1038,12 @@ def attention_kv4(q, cache, state, scale=None, out=None, ws=None):
     if out is None:
         out = torch.empty_like(q)
     else:
-        _gpu_tensor("out", out, (q.dtype,))
+        _check_tensor("out", out, (q.dtype,), None, dev)
         if out.numel() != q.numel() or not out.is_contiguous():
             raise ValueError("out is a contiguous tensor of %d values: got %s" % (q.numel(), tuple(out.shape)))
-    if ws is None:
-        ws = _call_workspace(attention_kv4_workspace_bytes(T, nh, nkv, hd, lmax))
+    wp, wn, _keep = _call_workspace(attention_kv4_workspace_bytes(T, nh, nkv, hd, lmax), dev)
     _lib.call("miq_attention_kv4", q.data_ptr(), dtype_code(q), cache.data_ptr(), state.data_ptr(), out.data_ptr(), T, nh, nkv, hd, lmax,
-              1.0 / math.sqrt(hd) if scale is None else float(scale), None if ws is None else ws.data_ptr(),
-              0 if ws is None else ws.numel(), stream_handle())
+              1.0 / math.sqrt(hd) if scale is None else float(scale), wp, wn, _raw_stream(dev))
     return out
 
 
@@ -1037,8 +1056,9 @@ def token_logprobs(logits, ids, top_k=0):
     likelier), each (T,), and the top_k <= 32 likeliest tokens, top_ids and top_logprobs (T, top_k), of
     equal ones the lower id first. An id outside the vocabulary has log probability 0 and rank -1; logits of
     -inf are tokens of probability 0."""
-    _gpu_tensor("logits", logits, (torch.float32, torch.float16), 2)
-    _gpu_tensor("ids", ids, (torch.int32, torch.int64), 1)
+    dev = _gpu_of("logits", logits)
+    _check_tensor("logits", logits, (torch.float32, torch.float16), 2, dev)
+    _check_tensor("ids", ids, (torch.int32, torch.int64), 1, dev)
     T, V = logits.shape
     if ids.shape[0] != T:
         raise ValueError("%d ids for %d rows of logits" % (ids.shape[0], T))
@@ -1049,12 +1069,15 @@ def token_logprobs(logits, ids, top_k=0):
     if ids.dtype != torch.int32:
         ids = ids.clamp(-1, 0x7FFFFFFF).to(torch.int32)
     ids = ids.contiguous()
-    r = TokenLogprobs(*(torch.empty(s, dtype=d, device=logits.device) for s, d in (
-        (T, torch.float32), (T, torch.float32), (T, torch.int32), ((T, top_k), torch.int32), ((T, top_k), torch.float32))))
+    where, f32, i32 = logits.device, torch.float32, torch.int32
+    lp, ent, rank = (torch.empty(T, dtype=f32, device=where), torch.empty(T, dtype=f32, device=where),
+                     torch.empty(T, dtype=i32, device=where))
+    ti, tl = torch.empty((T, top_k), dtype=i32, device=where), torch.empty((T, top_k), dtype=f32, device=where)
+    ld, code, st = logits.stride(0) if T > 1 else V, dtype_code(logits), _raw_stream(dev)
     for t0 in range(0, T, 65535):  # rows of one launch
         n = min(T - t0, 65535)
-        ws = _call_workspace(token_logprobs_workspace_bytes(n, V, top_k))
-        _lib.call("miq_token_logprobs", logits[t0:].data_ptr(), dtype_code(logits), logits.stride(0) if T > 1 else V,
-                  ids[t0:].data_ptr(), n, V, top_k, *(x[t0:].data_ptr() for x in r), None, n,
-                  None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream_handle())
-    return r
+        wp, wn, _keep = _call_workspace(token_logprobs_workspace_bytes(n, V, top_k), dev)
+        _lib.call("miq_token_logprobs", logits.data_ptr() + t0 * ld * logits.element_size(), code, ld, ids.data_ptr() + 4 * t0, n, V, top_k,
+                  lp.data_ptr() + 4 * t0, ent.data_ptr() + 4 * t0, rank.data_ptr() + 4 * t0, ti.data_ptr() + 4 * top_k * t0,
+                  tl.data_ptr() + 4 * top_k * t0, None, n, wp, wn, st)
+    return TokenLogprobs(lp, ent, rank, ti, tl)

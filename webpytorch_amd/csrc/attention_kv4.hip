@@ -102,7 +102,7 @@ __device__ __forceinline__ void join_slices(const float* p0, size_t step, int sl
     const int row = x / (HD / 2), d = 2 * (x % (HD / 2));
     const float* pr = p0 + (size_t)row * (HD + 4);
     float mx = -INFINITY, sum = 0.f, a[2] = {0.f, 0.f};
-    constexpr int U = 16;
+    constexpr int U = 8;
     for (int k0 = 0; k0 < slices; k0 += U) {
       uint64_t st[U], v[U];
 #pragma unroll
@@ -136,17 +136,20 @@ __device__ __forceinline__ void join_slices(const float* p0, size_t step, int sl
   }
 }
 
-// 8 probabilities as matrix-core operands: rounded towards zero to fp16, and for fp32 rows what that leaves
-// (the sum of probabilities is taken of the operands, by the matrix cores, so that a rounding to one side
-// cancels in the quotient).
+// 8 probabilities as matrix-core operands. fp16 rows: rounded to the nearest (towards zero, one instruction
+// less, leaves the output at 3.3e-4 of float64 instead of 2.7e-4; its own rounding is 2.0e-4). fp32 rows: hi
+// towards zero, and what that leaves. The sum of probabilities is taken of the operands, by the matrix cores.
 template <int P> __device__ __forceinline__ void split_p(const float* p, half8v* ph) {
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    const half2v hi = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(p[2 * x], p[2 * x + 1]));
-    ph[0][2 * x] = hi.x;
-    ph[0][2 * x + 1] = hi.y;
-    if constexpr (P == 2) {
+    if constexpr (P == 1) {
+      ph[0][2 * x] = (_Float16)p[2 * x];
+      ph[0][2 * x + 1] = (_Float16)p[2 * x + 1];
+    } else {
+      const half2v hi = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(p[2 * x], p[2 * x + 1]));
       const half2v lo = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, -1.f, p[2 * x]), fmaf((float)hi.y, -1.f, p[2 * x + 1])));
+      ph[0][2 * x] = hi.x;
+      ph[0][2 * x + 1] = hi.y;
       ph[1][2 * x] = lo.x;
       ph[1][2 * x + 1] = lo.y;
     }
@@ -199,8 +202,8 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
   const int first = (int)min(pos0 + tf, (int64_t)LMAX - 1);                   // the smallest last key
   const int nblk = (S + kKv4Block - 1) / kKv4Block;
   // blocks of a slice: joining costs 3 us or more, so that up to 3 blocks a wave are one slice (700 positions of 2
-  // heads of 64: 8.6 -> 7.5 us), and from 512 blocks on a slice has two a wave (16000 positions: 14.7 -> 12.5 us)
-  const int per = nblk <= 3 * NW ? 3 * NW : max(nblk >= 512 ? 2 * NW : NW, (nblk + (int)gridDim.x - 1) / (int)gridDim.x);
+  // heads of 64: 8.6 -> 7.5 us), and from 256 blocks on a slice has two a wave (16000 positions: 14.7 -> 12.5 us)
+  const int per = nblk <= 3 * NW ? 3 * NW : max(nblk >= 256 ? 2 * NW : NW, (nblk + (int)gridDim.x - 1) / (int)gridDim.x);
   const int slices = max(1, (nblk + per - 1) / per);
   if (slice >= slices) return;
   const int b0 = slice * per, b1 = min(nblk, b0 + per);
