@@ -56,20 +56,16 @@ __device__ __forceinline__ float half_wave_max(float v) {
 __device__ __forceinline__ uint32_t kv4_quantize(float x, uint16_t& S, uint16_t& Z) {
 #pragma clang fp contract(off)
   const uint64_t odd = __ballot(!(fabsf(x) < INFINITY));
-  if ((uint32_t)((threadIdx.x & 32) ? odd >> 32 : odd)) {
-    S = kKv4Bad;
-    Z = kKv4Bad;
-    return 0;
-  }
+  const bool bad = (uint32_t)((threadIdx.x & 32) ? odd >> 32 : odd) != 0;
   x = fminf(fmaxf(x, -kKv4Max), kKv4Max);
   const float hi = half_wave_max(x), lo = -half_wave_max(-x);
   const __half s = __float2half_rn(fmaxf((hi - lo) * 16.f / 15.f, fabsf(lo) * (1.f / 128.f)));
   const float sf = __half2float(s);
   const __half z = __float2half_rn(lo - sf);
-  S = __half_as_ushort(s);
-  Z = __half_as_ushort(z);
-  if (!(sf > 0.f)) return 0;
-  return (uint32_t)fminf(fmaxf(rintf((x - __half2float(z)) / sf * 16.f) - 16.f, 0.f), 15.f);
+  S = bad ? kKv4Bad : __half_as_ushort(s);
+  Z = bad ? kKv4Bad : __half_as_ushort(z);
+  const float c = fminf(fmaxf(rintf((x - __half2float(z)) / sf * 16.f) - 16.f, 0.f), 15.f);
+  return !bad && sf > 0.f ? (uint32_t)c : 0u;  // no branch: calls on several groups overlap
 }
 
 }  // namespace miq

@@ -15,6 +15,11 @@
 namespace miq {
 
 constexpr int kNrWaves = 4;
+constexpr int kNrHeads = 4;  // heads of a wave, where there are enough of them
+
+// One head a wave while that fills the chip's 1024 SIMDs no more than a few times (a token's latency counts), then
+// several, whose loads are all issued first and share the rotation's.
+static int heads_per_wave(int T, int heads) { return (int64_t)T * heads >= 8192 ? kNrHeads : 1; }
 
 template <int CTRL> __device__ __forceinline__ double dpp_d(double v) {
   const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xF, 0xF, false);
@@ -35,173 +40,226 @@ __device__ __forceinline__ double wave_sum_d(double v) {
   return (lane_at_d(v, 0) + lane_at_d(v, 16)) + (lane_at_d(v, 32) + lane_at_d(v, 48));
 }
 
+// The rotation partners, HD / 2 dimensions further, of v[i] = dimension lane + 64 i.
+template <int HD> __device__ __forceinline__ void partners(const float* v, float* o) {
+  if constexpr (HD == 128) {
+    o[0] = v[1];
+    o[1] = v[0];
+  } else if constexpr (HD == 256) {
+    o[0] = v[2];
+    o[1] = v[3];
+    o[2] = v[0];
+    o[3] = v[1];
+  } else if constexpr (HD == 64) {
+    o[0] = __shfl_xor(v[0], 32);
+  }
+}
+
 // The fp32 cache: every product, quotient and sum rounded where miq_head_rmsnorm and miq_rope_kv
-// round theirs, in their order, so that the results are theirs bit for bit.
+// round theirs, in their order, so that the results are theirs bit for bit. A wave takes U heads of one token,
+// all loads first; HDT is the head dimension where a lane's partner is in registers, 0 for any (through LDS).
+template <int HDT, int U>
 __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv_kernel(
     const float* __restrict__ qkv, size_t ld, const float* __restrict__ qn, const float* __restrict__ kn, float eps,
     const int32_t* __restrict__ state, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
-    float* __restrict__ q_out, float* __restrict__ kc, float* __restrict__ vc, int T, int NH, int NKV, int HD,
-    int LMAX) {
-  __shared__ float rows[kNrWaves][256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int heads = NH + 2 * NKV, half = HD / 2;
+    float* __restrict__ q_out, float* __restrict__ kc, float* __restrict__ vc, int T, int NH, int NKV, int HDR, int LMAX) {
+  constexpr int N = HDT ? HDT / 64 : 4;
+  const int HD = HDT ? HDT : HDR;
+  __shared__ float rows[HDT ? 1 : kNrWaves][256];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int heads = NH + 2 * NKV, half = HD / 2, groups = (heads + U - 1) / U;
   const int64_t unit = (int64_t)blockIdx.x * kNrWaves + wave;
-  const bool live = unit < (int64_t)T * heads;
-  const int t = live ? (int)(unit / heads) : 0, h = live ? (int)(unit % heads) : 0;
+  const int t = (int)(unit / groups), h0 = (int)(unit % groups) * U;
+  if (t >= T) return;  // whole waves
+  const float* row = qkv + (size_t)t * ld;
+  float v[U][N], w[2][N], c[N], s[N];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[u][i] = h0 + u < heads && (HDT || lane + 64 * i < HD) ? row[(h0 + u) * HD + lane + 64 * i] : 0.f;
   const int64_t pos = (int64_t)state[0] + t;
   const bool in = pos >= 0 && pos < LMAX;
-  const float* row = qkv + (size_t)t * ld + (size_t)h * HD;
-  float v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = live && lane + 64 * i < HD ? row[lane + 64 * i] : 0.f;
-  const float* w = h < NH ? qn : h < NH + NKV ? kn : nullptr;
-  if (w) {  // whole waves
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s = s + v[i] * v[i];
-    s = wave_sum(s);
-    const float r = sqrtf(s / (float)HD + eps);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < HD) v[i] = (v[i] / r) * w[lane + 64 * i];
+  for (int i = 0; i < N; ++i) {
+    const int d = lane + 64 * i, j = d < half ? d : d - half;
+    const bool has = HDT || d < HD;
+    w[0][i] = qn && has ? qn[d] : 0.f;
+    w[1][i] = kn && has ? kn[d] : 0.f;
+    c[i] = in && has ? cos_t[(size_t)pos * half + j] : 0.f;
+    s[i] = in && has ? sin_t[(size_t)pos * half + j] : 0.f;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) rows[wave][lane + 64 * i] = v[i];
-  __syncthreads();
-  if (!live) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    if (d >= HD) break;
+  for (int u = 0; u < U; ++u) {
+    const int h = h0 + u;
+    if (h >= heads) break;
     if (h >= NH + NKV) {
-      if (in) vc[((size_t)(h - NH - NKV) * LMAX + pos) * HD + d] = v[i];
+      if (in)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (HDT || lane + 64 * i < HD) vc[((size_t)(h - NH - NKV) * LMAX + pos) * HD + lane + 64 * i] = v[u][i];
       continue;
     }
-    const int j = d < half ? d : d - half;
-    float y = 0.f;
-    if (in) {
-      const float rv = d < half ? -rows[wave][d + half] : rows[wave][d - half];
-      y = v[i] * cos_t[(size_t)pos * half + j] + rv * sin_t[(size_t)pos * half + j];
+    if (h < NH ? qn != nullptr : kn != nullptr) {
+      float q = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) q = q + v[u][i] * v[u][i];
+      q = wave_sum(q);
+      const float r = sqrtf(q / (float)HD + eps);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[u][i] = (v[u][i] / r) * (h < NH ? w[0][i] : w[1][i]);
     }
-    if (h < NH) q_out[((size_t)t * NH + h) * HD + d] = y;
-    else if (in) kc[((size_t)(h - NH) * LMAX + pos) * HD + d] = y;
+    float o[N];
+    if constexpr (HDT) {
+      partners<HDT>(v[u], o);
+    } else {
+      float* mine = rows[wave];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int i = 0; i < N; ++i) mine[lane + 64 * i] = v[u][i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int d = lane + 64 * i;
+        o[i] = d < HD ? mine[d < half ? d + half : d - half] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = lane + 64 * i;
+      if (!HDT && d >= HD) break;
+      float y = 0.f;  // a position outside the cache: no key, and zeros for its queries
+      if (in) y = v[u][i] * c[i] + (d < half ? -o[i] : o[i]) * s[i];
+      if (h < NH) q_out[((size_t)t * NH + h) * HD + d] = y;
+      else if (in) kc[((size_t)(h - NH) * LMAX + pos) * HD + d] = y;
+    }
   }
 }
 
 // The 4-bit cache. A key's codes depend on which side of a border its value is, so q and k are computed
-// in fp64 (the vector units' fp64 rate is half the fp32 one, and the pass waits for memory) and rounded once.
-// Waves [0, T (NH + NKV)) take a head of q or k; the ones after them 8 values of each dimension, the 8
-// positions that share words (kv4_key): a word that is not wholly new is read first.
-template <int HD, typename XT>
+// in fp64 (the vector units' fp64 rate is that of fp32) and rounded once. The first waves take 64
+// dimensions of the values of the 8 positions that share words (kv4_key; a word that is not wholly new is read
+// first), the others U heads of q and k of one token.
+template <int HD, typename XT, int U>
 __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv4_kernel(
     const XT* __restrict__ qkv, size_t ld, const float* __restrict__ qn, const float* __restrict__ kn, float eps,
     const int32_t* __restrict__ state, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
     XT* __restrict__ q_out, uint8_t* __restrict__ cache, int T, int NH, int NKV, int LMAX, int vblocks) {
   constexpr int N = HD / 64, NG = HD / 32, HALF = HD / 2;
   const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * kNrWaves + uniform(threadIdx.x >> 6);
-  const int64_t nqk = (int64_t)T * (NH + NKV);
-  const int64_t pos0 = state[0];
+  const int nv = vblocks * NKV * 4 * N, wave = uniform(threadIdx.x >> 6);
+  const int64_t unit = (int64_t)blockIdx.x * kNrWaves + wave - nv;
+  const int heads = NH + NKV, groups = (heads + U - 1) / U;
   const int NB = kv4_blocks(LMAX);
-  if (unit < nqk) {
-    const int t = (int)(unit / (NH + NKV)), h = (int)(unit % (NH + NKV));
-    const int64_t pos = pos0 + t;
+  if (unit >= 0) {
+    if (unit >= (int64_t)T * groups) return;
+    const int t = (int)(unit / groups), h0 = (int)(unit % groups) * U;
+    const XT* row = qkv + (size_t)t * ld;
+    XT x[U][N];
+    float w[2][N], cs[N], sn[N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[u][i] = h0 + u < heads ? row[(h0 + u) * HD + lane + 64 * i] : from_f32<XT>(0.f);
+    const int64_t pos = (int64_t)state[0] + t;
     const bool in = pos >= 0 && pos < LMAX;
-    const XT* row = qkv + (size_t)t * ld + (size_t)h * HD;
-    if (!in) {  // a position outside the cache: no key, and zeros for its queries
-      if (h < NH)
-#pragma unroll
-        for (int i = 0; i < N; ++i) q_out[((size_t)t * NH + h) * HD + lane + 64 * i] = from_f32<XT>(0.f);
-      return;
-    }
-    double v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (double)to_f32<XT>(row[lane + 64 * i]);
-    const float* w = h < NH ? qn : kn;
-    if (w) {
-      double s = 0.0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) s += v[i] * v[i];
-      const double inv = 1.0 / sqrt(wave_sum_d(s) / HD + (double)eps);
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = v[i] * inv * (double)w[lane + 64 * i];
-    }
-    float y[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int d = lane + 64 * i, j = d < HALF ? d : d - HALF;
-      double o;  // the rotation partner
-      if constexpr (HD % 128 == 0) o = v[(i + N / 2) % N];
-      else if constexpr (HD == 64) o = other_half(v[0]);
-      else {  // 192: 96 dimensions further, in lane ^ 32 of the register after next or of the next one
-        double got[3];
+      w[0][i] = qn ? qn[d] : 0.f;
+      w[1][i] = kn ? kn[d] : 0.f;
+      cs[i] = in ? cos_t[(size_t)pos * HALF + j] : 0.f;
+      sn[i] = in ? sin_t[(size_t)pos * HALF + j] : 0.f;
+    }
 #pragma unroll
-        for (int r = 0; r < 3; ++r) got[r] = other_half(v[r]);
-        const int k = (i + (lane < 32 ? 1 : 2)) % 3;
-        o = k == 0 ? got[0] : k == 1 ? got[1] : got[2];
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u;
+      if (h >= heads) break;
+      if (!in) {  // a position outside the cache: no key, and zeros for its queries
+        if (h < NH)
+#pragma unroll
+          for (int i = 0; i < N; ++i) q_out[((size_t)t * NH + h) * HD + lane + 64 * i] = from_f32<XT>(0.f);
+        continue;
       }
-      const double c = (double)cos_t[(size_t)pos * HALF + j], s = (double)sin_t[(size_t)pos * HALF + j];
-      y[i] = (float)(d < HALF ? v[i] * c - o * s : v[i] * c + o * s);
-    }
-    if (h < NH) {
+      double v[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) q_out[((size_t)t * NH + h) * HD + lane + 64 * i] = from_f32<XT>(y[i]);
-      return;
-    }
-    const int key = (int)(pos % kKv4Block);
-    uint8_t* rec = cache + ((size_t)(h - NH) * NB + (size_t)(pos / kKv4Block)) * kv4_record(HD);
+      for (int i = 0; i < N; ++i) v[i] = (double)to_f32<XT>(x[u][i]);
+      if (h < NH ? qn != nullptr : kn != nullptr) {
+        double s = 0.0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      uint16_t S, Z;
-      uint32_t c = kv4_quantize(y[i], S, Z) << kv4_shift(lane & 7);
-      c |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0xB1, 0xF, 0xF, false);
-      c |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0x4E, 0xF, 0xF, false);
-      c |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0x141, 0xF, 0xF, false);
-      const int grp = 2 * i + (lane >> 5);
-      if ((lane & 7) == 0)
-        *reinterpret_cast<uint32_t*>(rec + kv4_word((key >> 4) * NG + grp, (lane & 31) >> 3, key & 15)) = c;
-      if ((lane & 31) == 0)
-        *reinterpret_cast<uint32_t*>(rec + kv4_kmeta(HD) + (key * NG + grp) * 4) = S | ((uint32_t)Z << 16);
+        for (int i = 0; i < N; ++i) s = fma(v[i], v[i], s);
+        const double inv = rsqrt(wave_sum_d(s) * (1.0 / HD) + (double)eps);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] * inv * (double)(h < NH ? w[0][i] : w[1][i]);
+      }
+      float y[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        double o;  // the rotation partner
+        if constexpr (HD % 128 == 0) o = v[(i + N / 2) % N];
+        else if constexpr (HD == 64) o = other_half(v[0]);
+        else {  // 192: 96 dimensions further, in lane ^ 32 of the register after next or of the next one
+          double got[3];
+#pragma unroll
+          for (int r = 0; r < 3; ++r) got[r] = other_half(v[r]);
+          const int k = (i + (lane < 32 ? 1 : 2)) % 3;
+          o = k == 0 ? got[0] : k == 1 ? got[1] : got[2];
+        }
+        const double os = lane + 64 * i < HALF ? -o : o;
+        y[i] = (float)fma(os, (double)sn[i], v[i] * (double)cs[i]);
+      }
+      if (h < NH) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q_out[((size_t)t * NH + h) * HD + lane + 64 * i] = from_f32<XT>(y[i]);
+        continue;
+      }
+      const int key = (int)(pos % kKv4Block);
+      uint8_t* rec = cache + ((size_t)(h - NH) * NB + (size_t)(pos / kKv4Block)) * kv4_record(HD);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        uint16_t S, Z;
+        uint32_t c = kv4_quantize(y[i], S, Z) << kv4_shift(lane & 7);
+        c |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0xB1, 0xF, 0xF, false);
+        c |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0x4E, 0xF, 0xF, false);
+        c |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0x141, 0xF, 0xF, false);
+        const int grp = 2 * i + (lane >> 5);
+        if ((lane & 7) == 0)
+          *reinterpret_cast<uint32_t*>(rec + kv4_word((key >> 4) * NG + grp, (lane & 31) >> 3, key & 15)) = c;
+        if ((lane & 31) == 0)
+          *reinterpret_cast<uint32_t*>(rec + kv4_kmeta(HD) + (key * NG + grp) * 4) = S | ((uint32_t)Z << 16);
+      }
     }
     return;
   }
-  const int64_t vu = unit - nqk;
-  const int g = (int)(vu & 3), kv = (int)((vu >> 2) % NKV);
-  const int64_t first = pos0 > 0 ? pos0 : 0, blk = first / kKv4Block + (vu >> 2) / NKV;
-  if ((vu >> 2) / NKV >= vblocks || blk >= NB) return;
+  const int vu = blockIdx.x * kNrWaves + wave, i = vu % N, g = vu / N & 3, kv = vu / (4 * N) % NKV;
+  const int64_t pos0 = state[0], first = pos0 > 0 ? pos0 : 0, blk = first / kKv4Block + vu / (4 * N * NKV);
+  if (blk >= NB) return;
+  const int d = lane + 64 * i, grp = 2 * i + (lane >> 5);
   uint32_t live = 0;
-  float x[8][N];
+  float x[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int64_t pos = blk * kKv4Block + kv4_key(g, e), t = pos - pos0;
     const bool in = t >= 0 && t < T && pos < LMAX;
     live |= (in ? 15u : 0u) << kv4_shift(e);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      x[e][i] = in ? to_f32<XT>(qkv[(size_t)t * ld + (size_t)(NH + NKV + kv) * HD + lane + 64 * i]) : 0.f;
+    x[e] = in ? to_f32<XT>(qkv[(size_t)t * ld + (size_t)(NH + NKV + kv) * HD + d]) : 0.f;
   }
   if (!live) return;
   uint8_t* rec = cache + ((size_t)kv * NB + (size_t)blk) * kv4_record(HD);
+  uint32_t* word = reinterpret_cast<uint32_t*>(rec + kv4_vcodes(HD) + kv4_word(d >> 4, g, d & 15));
+  uint16_t* meta = reinterpret_cast<uint16_t*>(rec + kv4_vmeta(HD)) + (grp * 4 + g) * 16;
+  uint32_t c = live == 0xFFFFFFFFu ? 0u : *word & ~live;
+  uint16_t S[8], Z[8];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int d = lane + 64 * i, grp = 2 * i + (lane >> 5);
-    uint32_t* word = reinterpret_cast<uint32_t*>(rec + kv4_vcodes(HD) + kv4_word(d >> 4, g, d & 15));
-    uint32_t c = live == 0xFFFFFFFFu ? 0u : *word & ~live;
-    uint16_t* meta = reinterpret_cast<uint16_t*>(rec + kv4_vmeta(HD)) + (grp * 4 + g) * 16;
+  for (int e = 0; e < 8; ++e) c |= (kv4_quantize(x[e], S[e], Z[e]) << kv4_shift(e)) & live;
+  *word = c;
+  if ((lane & 31) == 0)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      uint16_t S, Z;
-      const uint32_t code = kv4_quantize(x[e][i], S, Z);
+    for (int e = 0; e < 8; ++e)
       if ((live >> kv4_shift(e)) & 1) {
-        c |= code << kv4_shift(e);
-        if ((lane & 31) == 0) {
-          meta[e] = S;
-          meta[8 + e] = Z;
-        }
+        meta[e] = S[e];
+        meta[8 + e] = Z[e];
       }
-    }
-    *word = c;
-  }
 }
 
 // fp32 rows of the positions [start, start + n): a thread takes one word, of a key 8 dimensions, of the
@@ -267,10 +325,23 @@ extern "C" int miq_qk_norm_rope_kv(const float* qkv, int64_t ld, const float* qn
   if (int rc = check_norm_rope("qk_norm_rope_kv", qkv, ld, state, cos_tab, sin_tab, q_out, T, NH, NKV, HD, LMAX)) return rc;
   if (T == 0) return MIQ_OK;
   MIQ_REQUIRE(kcache && vcache, MIQ_ERR_INVALID, "qk_norm_rope_kv: null pointer");
-  const int64_t units = (int64_t)T * (NH + 2 * NKV);
-  hipLaunchKernelGGL(norm_rope_kv_kernel, dim3((unsigned)((units + kNrWaves - 1) / kNrWaves)), dim3(64 * kNrWaves), 0,
-                     static_cast<hipStream_t>(stream), qkv, (size_t)ld, qn, kn, eps, state, cos_tab, sin_tab, q_out, kcache,
-                     vcache, T, NH, NKV, HD, LMAX);
+  const int heads = NH + 2 * NKV, U = heads_per_wave(T, heads);
+  const int64_t units = (int64_t)T * ((heads + U - 1) / U);
+  const dim3 grid((unsigned)((units + kNrWaves - 1) / kNrWaves)), block(64 * kNrWaves);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+#define MIQ_NR(HDV, UV)                                                                                                     \
+  hipLaunchKernelGGL((norm_rope_kv_kernel<HDV, UV>), grid, block, 0, st, qkv, (size_t)ld, qn, kn, eps, state, cos_tab, sin_tab, q_out, \
+                     kcache, vcache, T, NH, NKV, HD, LMAX)
+#define MIQ_NR_HD(UV)                     \
+  switch (HD) {                           \
+    case 64: MIQ_NR(64, UV); break;       \
+    case 128: MIQ_NR(128, UV); break;     \
+    case 256: MIQ_NR(256, UV); break;     \
+    default: MIQ_NR(0, UV);               \
+  }
+  if (U == 1) { MIQ_NR_HD(1) } else { MIQ_NR_HD(kNrHeads) }
+#undef MIQ_NR_HD
+#undef MIQ_NR
   return check_launch("qk_norm_rope_kv");
 }
 
@@ -285,20 +356,25 @@ extern "C" int miq_qk_norm_rope_kv4(const void* qkv, int x_dtype, int64_t ld, co
   MIQ_REQUIRE(aligned(cache, 16), MIQ_ERR_ALIGN, "qk_norm_rope_kv4: the cache must be 16-byte aligned");
   // T rows lie in at most this many blocks, wherever the first one is
   const int vblocks = (T + kKv4Block - 2) / kKv4Block + 1;
-  const int64_t units = (int64_t)T * (NH + NKV) + (int64_t)vblocks * NKV * 4;
+  const int U = heads_per_wave(T, NH + NKV);
+  const int64_t units = (int64_t)T * ((NH + NKV + U - 1) / U) + (int64_t)vblocks * NKV * 4 * (HD / 64);
   const dim3 grid((unsigned)((units + kNrWaves - 1) / kNrWaves)), block(64 * kNrWaves);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-#define MIQ_NR(HDV, XT)                                                                                           \
-  hipLaunchKernelGGL((norm_rope_kv4_kernel<HDV, XT>), grid, block, 0, st, static_cast<const XT*>(qkv), (size_t)ld, qn, kn, eps, \
+#define MIQ_NR(HDV, XT, UV)                                                                                       \
+  hipLaunchKernelGGL((norm_rope_kv4_kernel<HDV, XT, UV>), grid, block, 0, st, static_cast<const XT*>(qkv), (size_t)ld, qn, kn, eps, \
                      state, cos_tab, sin_tab, static_cast<XT*>(q_out), static_cast<uint8_t*>(cache), T, NH, NKV, LMAX, vblocks)
-#define MIQ_NR_HD(XT)               \
-  switch (HD) {                     \
-    case 64: MIQ_NR(64, XT); break; \
-    case 128: MIQ_NR(128, XT); break; \
-    case 192: MIQ_NR(192, XT); break; \
-    default: MIQ_NR(256, XT);       \
+#define MIQ_NR_HD(XT, UV)                   \
+  switch (HD) {                             \
+    case 64: MIQ_NR(64, XT, UV); break;     \
+    case 128: MIQ_NR(128, XT, UV); break;   \
+    case 192: MIQ_NR(192, XT, UV); break;   \
+    default: MIQ_NR(256, XT, UV);           \
   }
-  if (x_dtype == MIQ_F32) { MIQ_NR_HD(float) } else { MIQ_NR_HD(__half) }
+  if (x_dtype == MIQ_F32) {
+    if (U == 1) { MIQ_NR_HD(float, 1) } else { MIQ_NR_HD(float, kNrHeads) }
+  } else {
+    if (U == 1) { MIQ_NR_HD(__half, 1) } else { MIQ_NR_HD(__half, kNrHeads) }
+  }
 #undef MIQ_NR_HD
 #undef MIQ_NR
   return check_launch("qk_norm_rope_kv4");
