@@ -57,6 +57,25 @@ __device__ __forceinline__ void lp_merge(LpSum& a, float m, float s0, float s1) 
   a.s0 = fa * a.s0 + fb * s0;
   a.m = mn;
 }
+// over the wave: one exponential a lane, against the wave's maximum
+__device__ __forceinline__ void lp_wave(LpSum& a, int& above) {
+  const float m = wave_max(a.m);
+  if (m == -INFINITY) {
+    a.s0 = wave_sum(a.s0);
+  } else {
+    const float d = fmaxf((a.m - m) * kLog2e, -1e4f), f = __builtin_amdgcn_exp2f(d);
+    a.s1 = wave_sum(f * fmaf(a.s0, d, a.s1));
+    a.s0 = wave_sum(f * a.s0);
+    a.m = m;
+  }
+  int n = above;
+  n += __builtin_amdgcn_update_dpp(0, n, 0xB1, 0xF, 0xF, false);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x4E, 0xF, 0xF, false);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x141, 0xF, 0xF, false);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x140, 0xF, 0xF, false);
+  above = (__builtin_amdgcn_readlane(n, 0) + __builtin_amdgcn_readlane(n, 16)) +
+          (__builtin_amdgcn_readlane(n, 32) + __builtin_amdgcn_readlane(n, 48));
+}
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int s) {
   return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), s) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, s);
 }
@@ -214,11 +233,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
   }
 
   // ---- the lanes' and the waves' parts ----
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    lp_merge(a, __shfl_xor(a.m, s), __shfl_xor(a.s0, s), __shfl_xor(a.s1, s));
-    above += __shfl_xor(above, s);
-  }
+  lp_wave(a, above);
   if (k) lp_keep(list, n, k);
   if (lane == 0) {
     sums[wave] = a;
@@ -288,10 +303,9 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
       above = (int)(w1 >> 32);
     }
     // no key below the best of the segments' k-th keys is among the row's best k
+    lp_wave(a, above);
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
-      lp_merge(a, __shfl_xor(a.m, s), __shfl_xor(a.s0, s), __shfl_xor(a.s1, s));
-      above += __shfl_xor(above, s);
       const uint64_t o = shfl_xor64(lb, s);
       lb = o > lb ? o : lb;
     }
