@@ -124,7 +124,10 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
     float* __restrict__ ent_out, int32_t* __restrict__ rank_out, int32_t* __restrict__ top_ids, float* __restrict__ top_lp,
     const int32_t* __restrict__ state, int out_rows, int* __restrict__ counters, uint64_t* __restrict__ parts) {
   constexpr int VEC = LpLoad<T>::VEC, U = kLpPer / VEC;
-  __shared__ __align__(16) uint64_t lists[kLpWaves][kLpList], join[kLpJoin];
+  __shared__ __align__(16) uint64_t lists[kLpWaves][kLpList], pool[kLpWaves * kLpChunk / 2];
+  float* vals = reinterpret_cast<float*>(pool) + uniform(threadIdx.x >> 6) * kLpChunk;  // a wave's chunk
+  uint64_t* join = pool;  // later: the keys of all segments
+  static_assert(kLpWaves * kLpChunk / 2 >= kLpJoin, "the join's keys fit");
   __shared__ LpSum sums[kLpWaves];
   __shared__ uint64_t bounds[kLpWaves];
   __shared__ int cnts[kLpWaves], njoin, last;
@@ -207,25 +210,35 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
         bv = -wave_max(-g);
       }
       if (__ballot(cm >= bv)) {
-        auto push = [&](float y, uint32_t i, bool valid) __attribute__((always_inline)) {
-          const uint64_t key = lp_key(y, i);
-          const uint64_t mask = __ballot(valid && !(y < bv) && key > kth);
-          if (!mask) return;
-          if ((mask >> lane) & 1) list[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
+        // a bit for each value of the lane that may come in (bit kLpPer: the row's unaligned ends); one of every lane
+        // a round, fetched through LDS, so that the code is short: a row's only chunk pays for each line of it
+        uint32_t bits = ext && !(xe < bv) ? 1u << kLpPer : 0u;
+#pragma unroll
+        for (int e = 0; e < kLpPer; ++e)
+          if (vb + (e / VEC) * 64 + lane < v1 && !(v[e] < bv)) bits |= 1u << e;
+#pragma unroll
+        for (int e = 0; e < kLpPer; e += 4)
+          *reinterpret_cast<float4*>(&vals[(e * 16 + lane) * 4]) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        while (__ballot(bits != 0)) {
+          const int e = __ffs(bits) - 1;
+          uint64_t key = 0;
+          if (bits) {
+            const bool end = e == kLpPer;
+            const float y = end ? xe : vals[((e & ~3) * 16 + lane) * 4 + (e & 3)];
+            key = lp_key(y, (uint32_t)(end ? xi : head + (vb + (e / VEC) * 64 + lane) * VEC + e % VEC));
+            bits &= bits - 1;
+          }
+          const uint64_t mask = __ballot(key > kth);
+          if (key > kth) list[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
           n += __popcll(mask);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           if (n > kLpList - 64) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             lp_keep(list, n, k);
             n = k;
             kth = list[k - 1];
             bv = lp_value(kth);
           }
-        };
-        if (first && seg == 0 && wave == 0) push(xe, xi, ext);
-#pragma unroll
-        for (int e = 0; e < kLpPer; ++e) {
-          const int vi = vb + (e / VEC) * 64 + lane;
-          push(v[e], (uint32_t)(head + vi * VEC + e % VEC), vi < v1);
         }
       }
     }
