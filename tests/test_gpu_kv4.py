@@ -341,6 +341,100 @@ def test_two_threads_two_streams(gpu):
     assert not errors and wrong == [0, 0], (errors, wrong)
 
 
+def _torch_want(q, cache, pos):
+    """float64 on the GPU over what the cache stands for; q (T, NH, HD)."""
+    import torch
+    from webpytorch_amd import core
+    T, NH, HD = q.shape
+    n = max(pos + T, 1)
+    k, v = (t.double() for t in core.kv4_dequant(cache, 0, n))
+    rep = NH // k.shape[0]
+    out = torch.empty(q.shape, dtype=torch.float64, device="cuda")
+    later = torch.arange(n, device="cuda")[None, :] > pos + torch.arange(T, device="cuda")[:, None]
+    for h in range(NH):
+        s = torch.mm(q[:, h].double(), k[h // rep].t().contiguous()) / math.sqrt(HD)
+        s[later] = -math.inf
+        out[:, h] = torch.mm(torch.softmax(s, 1).nan_to_num(0.0), v[h // rep])
+    return out
+
+
+@pytest.mark.parametrize("dt", ["float32", "float16"])
+@pytest.mark.parametrize("NH,NKV,HD", [(2, 1, 64), (3, 1, 128), (2, 2, 192), (4, 1, 256)])
+@pytest.mark.parametrize("T,pos,lmax", [(600, 0, 600), (300, 5, 8192), (90, 4001, 70000), (257, 1000, 40000), (700, -650, 800),
+                                        (700, -20, 8192)])
+def test_many_rows(gpu, NH, NKV, HD, T, pos, lmax, dt):
+    """The many-row kernel at every head dimension, whole and in slices that a second launch joins, a cache
+    whose memory behind the last position is anything, rows before position 0, and a NaN that reaches its tokens."""
+    import torch
+    from webpytorch_amd import core
+    g = torch.Generator().manual_seed(T + HD)
+    n = max(pos + T, 1)
+    q = torch.randn((T, NH, HD), generator=g).to(getattr(torch, dt)).cuda()
+    k, v = (torch.randn((n, NKV, HD), generator=g) for _ in range(2))
+    rnd = torch.randint(0, 256, (NKV, (lmax + 31) // 32, 40 * HD), dtype=torch.uint8, generator=g).cuda()
+    cache = fill(k, v, cache=rnd)
+    got = core.attention_kv4(q, cache, state(torch, pos))
+    want = _torch_want(q, cache, pos)
+    close(got, want.cpu().numpy(), F32_REL if dt == "float32" else F16_REL)
+    assert not got[:max(0, -pos)].any()
+    at = n - min(T, n) // 2 - 1
+    v[at, 0, 40] = float("nan")
+    bad = core.attention_kv4(q, fill(k, v, cache=rnd), state(torch, pos))
+    sees = torch.arange(T) + pos >= at
+    assert torch.equal(bad[~sees], got[~sees]) and torch.isnan(bad[sees][:, :NH // NKV, 32:64]).all()
+    other = [d for d in range(HD) if not 32 <= d < 64]
+    assert torch.equal(bad[sees][..., other], got[sees][..., other])
+
+
+def test_threads_on_one_stream_with_other_products(gpu):
+    """Attention in two launches, log probabilities and a split GEMV share the stream's workspace: each thread
+    gets what it gets alone."""
+    import torch
+    from webpytorch_amd import core, synth
+    q, cache, st = _case(51, T=90, pos=4000, lmax=70000)
+    lg, ids = torch.randn((3, 50000), generator=torch.Generator().manual_seed(5)).cuda(), torch.arange(3, dtype=torch.int32, device="cuda")
+    L = synth.gptq_layer(5, 4096, 1024, 128, 4)
+    lin = core.QuantizedLinear.from_autogptq(L["qweight"], L["qzeros"], L["scales"], None, 128, 4)
+    x = torch.from_numpy(synth.activations(5, 3, 4096, np.float32)).cuda()
+    calls = [lambda: core.attention_kv4(q, cache, st), lambda: core.token_logprobs(lg, ids, 4).top_logprobs, lambda: lin.forward(x)]
+    alone = [c() for c in calls]
+    torch.cuda.synchronize()
+    wrong, errors, start = [torch.zeros((), dtype=torch.int64, device="cuda") for _ in calls], [], threading.Barrier(len(calls))
+
+    def work(i):
+        try:
+            start.wait(30)
+            for _ in range(100):
+                wrong[i] += (calls[i]() != alone[i]).sum()
+        except Exception as e:
+            errors.append(e)
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join(60)
+    torch.cuda.synchronize()
+    assert not errors and [int(w) for w in wrong] == [0, 0, 0], (errors, wrong)
+
+
+def test_many_rows_in_a_graph(gpu):
+    """Two launches and the graph's own workspace, replayed with eager calls between."""
+    import torch
+    from webpytorch_amd import core
+    q, cache, st = _case(52, T=90, pos=4000, lmax=70000)
+    want = core.attention_kv4(q, cache, st)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = core.attention_kv4(q, cache, st)
+    for pos in (4000, 3900, 4000):
+        st[0] = pos
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        eager = core.attention_kv4(q, cache, st)
+        assert torch.equal(out, eager) and (pos != 4000 or torch.equal(out, want))
+
+
 def test_argument_checks(gpu):
     import torch
     from webpytorch_amd import core

@@ -807,8 +807,8 @@ extern "C" int miq_attention_kv4(const void* q, int x_dtype, const void* cache, 
   const dim3 grid = p.few ? dim3((unsigned)p.slices, (unsigned)p.tiles, (unsigned)NKV) : dim3((unsigned)NKV, (unsigned)p.tiles, (unsigned)p.slices);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   // the join reads what the tiles kernel left in the workspace: another thread's call on the stream waits
-  std::unique_lock<std::mutex> lock(stream_lock(st), std::defer_lock);
-  if (!p.few && part) lock.lock();
+  std::unique_lock<std::mutex> whole(stream_lock(st), std::defer_lock);
+  if (part) whole.lock();
 #define MIQ_A4(HDV, XT)                                                                                              \
   if (p.few) {                                                                                                       \
     hipLaunchKernelGGL((attention_kv4_rows_kernel<HDV, XT>), grid, dim3(64 * kA4Waves), lds, st, static_cast<const XT*>(q), \

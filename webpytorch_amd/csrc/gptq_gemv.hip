@@ -622,6 +622,8 @@ extern "C" int miq_gptq_gemv(const void* x, int x_dtype, const int32_t* perm, co
   int rc = gemv_check("gptq_gemv", x, x_dtype, qweight, qzeros, scales, scales_dtype, out, out_dtype, M, K, N,
                       gs, bits);
   if (rc || M == 0) return rc;
+  // one launch, but it writes to the workspace: not between the launches of another thread's call
+  std::lock_guard<std::mutex> whole(stream_lock(static_cast<hipStream_t>(stream)));
   // one row of an int4 layer: the matrix-core GEMV (it declines shapes it does not cover)
   if (M == 1 && bits == 4 && (size_t)K * N / 2 >= kGemvMmaMinBytes &&
       (workspace == nullptr || aligned(workspace, 256))) {
@@ -658,6 +660,7 @@ extern "C" int miq_gptq_gemv_fused(const float* x, int x_mode, const float* norm
   int rc = gemv_check("gptq_gemv_fused", x, MIQ_F32, qweight, qzeros, scales, scales_dtype, out, MIQ_F32, M, K, N, gs,
                       bits);
   if (rc || M == 0) return rc;
+  std::lock_guard<std::mutex> whole(stream_lock(static_cast<hipStream_t>(stream)));  // as in miq_gptq_gemv
   // one row of an int4 layer in k order: the matrix-core GEMV with the transform in its staging
   if (M == 1 && bits == 4 && !perm && (workspace == nullptr || aligned(workspace, 256))) {
     rc = gemv_mma(x, MIQ_F32, nullptr, qweight, qzeros, scales, scales_dtype, bias, out, MIQ_F32, K, N, gs,

@@ -433,6 +433,9 @@ extern "C" int miq_token_logprobs(const void* logits, int x_dtype, int64_t ld, c
   uint64_t* parts = part ? reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + kCounterBytes) : nullptr;
   const dim3 grid((unsigned)segs, (unsigned)T), block(kLpThreads);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  // one launch, but it writes to the workspace: not between the launches of another thread's call
+  std::unique_lock<std::mutex> whole(stream_lock(st), std::defer_lock);
+  if (part) whole.lock();
   if (x_dtype == MIQ_F32)
     hipLaunchKernelGGL(logprobs_kernel<float>, grid, block, 0, st, static_cast<const float*>(logits), (size_t)ld, ids, V, k,
                        logprobs, entropy, ranks, top_ids, top_logprobs, state, out_rows, counters, parts);
