@@ -3,9 +3,10 @@
 // webtorch/_core.py:1504-1540): q_h = rope(x_h / sqrt(mean(x_h^2) + eps) * qn), k likewise, v as it is, k and
 // v into an fp32 cache or into the 4-bit one (kv4.h).
 //
-// A wave takes one head of one token, lane l its dimensions l, l + 64, ..: the mean is a wave sum, a
+// A wave takes heads of one token, lane l the dimensions l, l + 64, ..: the mean is a wave sum, a
 // group of 32 dimensions is half a wave, and a dimension's rotation partner is another register of the lane
-// (HD 128, 256), the lane 32 further (HD 64), or read through LDS.
+// (HD 128, 256), the lane 32 further (HD 64), or read through LDS. Bound: memory for prompts (4001 tokens into the fp32
+// cache: 150 MB in 29.8 us, 5.0 TB/s), the launch and two round trips for a token (2.4 us).
 #include <math.h>
 
 #include "kv4.h"
@@ -15,11 +16,12 @@
 namespace miq {
 
 constexpr int kNrWaves = 4;
-constexpr int kNrHeads = 4;  // heads of a wave, where there are enough of them
-
 // One head a wave while that fills the chip's 1024 SIMDs no more than a few times (a token's latency counts), then
-// several, whose loads are all issued first and share the rotation's.
-static int heads_per_wave(int T, int heads) { return (int64_t)T * heads >= 8192 ? kNrHeads : 1; }
+// several, whose loads are all issued first and share the rotation's: 4001 tokens of 36 heads of 128 without a norm,
+// fp32 cache, 54 us at one head, 30.4 at 2, 29.8 at 4, 30.2 at 8; 700 tokens with norms, 4-bit cache, 19.0 at 4
+// heads of q and k, 16.9 at 4 of q or one of k, 16.1 at 2 of q or one of k (each with the 4.5 us of reading back).
+constexpr int kNrHeads = 4, kNrHeads4 = 2;
+static bool several_heads(int T, int heads) { return (int64_t)T * heads >= 8192; }
 
 template <int CTRL> __device__ __forceinline__ double dpp_d(double v) {
   const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xF, 0xF, false);
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv_kernel(
 // The 4-bit cache. A key's codes depend on which side of a border its value is, so q and k are computed
 // in fp64 (the vector units' fp64 rate is that of fp32) and rounded once. The first waves take 64
 // dimensions of the values of the 8 positions that share words (kv4_key; a word that is not wholly new is read
-// first), the others U heads of q and k of one token.
+// first), the others U heads of q, or one of k, of one token.
 template <int HD, typename XT, int U>
 __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv4_kernel(
     const XT* __restrict__ qkv, size_t ld, const float* __restrict__ qn, const float* __restrict__ kn, float eps,
@@ -149,18 +151,19 @@ __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv4_kernel(
   const int lane = threadIdx.x & 63;
   const int nv = vblocks * NKV * 4 * N, wave = uniform(threadIdx.x >> 6);
   const int64_t unit = (int64_t)blockIdx.x * kNrWaves + wave - nv;
-  const int heads = NH + NKV, groups = (heads + U - 1) / U;
+  const int qgroups = (NH + U - 1) / U, groups = qgroups + NKV;
   const int NB = kv4_blocks(LMAX);
   if (unit >= 0) {
     if (unit >= (int64_t)T * groups) return;
-    const int t = (int)(unit / groups), h0 = (int)(unit % groups) * U;
+    const int t = (int)(unit / groups), group = (int)(unit % groups);
+    const int h0 = group < qgroups ? group * U : NH + group - qgroups, end = group < qgroups ? min(NH, h0 + U) : h0 + 1;
     const XT* row = qkv + (size_t)t * ld;
     XT x[U][N];
     float w[2][N], cs[N], sn[N];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[u][i] = h0 + u < heads ? row[(h0 + u) * HD + lane + 64 * i] : from_f32<XT>(0.f);
+      for (int i = 0; i < N; ++i) x[u][i] = h0 + u < end ? row[(h0 + u) * HD + lane + 64 * i] : from_f32<XT>(0.f);
     const int64_t pos = (int64_t)state[0] + t;
     const bool in = pos >= 0 && pos < LMAX;
 #pragma unroll
@@ -174,7 +177,7 @@ __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv4_kernel(
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int h = h0 + u;
-      if (h >= heads) break;
+      if (h >= end) break;
       if (!in) {  // a position outside the cache: no key, and zeros for its queries
         if (h < NH)
 #pragma unroll
@@ -325,7 +328,7 @@ extern "C" int miq_qk_norm_rope_kv(const float* qkv, int64_t ld, const float* qn
   if (int rc = check_norm_rope("qk_norm_rope_kv", qkv, ld, state, cos_tab, sin_tab, q_out, T, NH, NKV, HD, LMAX)) return rc;
   if (T == 0) return MIQ_OK;
   MIQ_REQUIRE(kcache && vcache, MIQ_ERR_INVALID, "qk_norm_rope_kv: null pointer");
-  const int heads = NH + 2 * NKV, U = heads_per_wave(T, heads);
+  const int heads = NH + 2 * NKV, U = several_heads(T, heads) ? kNrHeads : 1;
   const int64_t units = (int64_t)T * ((heads + U - 1) / U);
   const dim3 grid((unsigned)((units + kNrWaves - 1) / kNrWaves)), block(64 * kNrWaves);
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -356,8 +359,8 @@ extern "C" int miq_qk_norm_rope_kv4(const void* qkv, int x_dtype, int64_t ld, co
   MIQ_REQUIRE(aligned(cache, 16), MIQ_ERR_ALIGN, "qk_norm_rope_kv4: the cache must be 16-byte aligned");
   // T rows lie in at most this many blocks, wherever the first one is
   const int vblocks = (T + kKv4Block - 2) / kKv4Block + 1;
-  const int U = heads_per_wave(T, NH + NKV);
-  const int64_t units = (int64_t)T * ((NH + NKV + U - 1) / U) + (int64_t)vblocks * NKV * 4 * (HD / 64);
+  const int U = several_heads(T, NH + NKV) ? kNrHeads4 : 1;
+  const int64_t units = (int64_t)T * ((NH + U - 1) / U + NKV) + (int64_t)vblocks * NKV * 4 * (HD / 64);
   const dim3 grid((unsigned)((units + kNrWaves - 1) / kNrWaves)), block(64 * kNrWaves);
   const hipStream_t st = static_cast<hipStream_t>(stream);
 #define MIQ_NR(HDV, XT, UV)                                                                                       \
@@ -371,9 +374,9 @@ extern "C" int miq_qk_norm_rope_kv4(const void* qkv, int x_dtype, int64_t ld, co
     default: MIQ_NR(256, XT, UV);           \
   }
   if (x_dtype == MIQ_F32) {
-    if (U == 1) { MIQ_NR_HD(float, 1) } else { MIQ_NR_HD(float, kNrHeads) }
+    if (U == 1) { MIQ_NR_HD(float, 1) } else { MIQ_NR_HD(float, kNrHeads4) }
   } else {
-    if (U == 1) { MIQ_NR_HD(__half, 1) } else { MIQ_NR_HD(__half, kNrHeads) }
+    if (U == 1) { MIQ_NR_HD(__half, 1) } else { MIQ_NR_HD(__half, kNrHeads4) }
   }
 #undef MIQ_NR_HD
 #undef MIQ_NR
