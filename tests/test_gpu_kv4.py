@@ -435,6 +435,65 @@ def test_many_rows_in_a_graph(gpu):
         assert torch.equal(out, eager) and (pos != 4000 or torch.equal(out, want))
 
 
+@pytest.mark.parametrize("size", [2e-6, 3e-5, 1e-3])
+@pytest.mark.parametrize("T", [1, 700])
+def test_values_below_the_normal_fp16_range(gpu, size, T):
+    """Values that stand for fp16 subnormals, and keys of that size under a large scale, are not taken for zero."""
+    import torch
+    from webpytorch_amd import core
+    g = torch.Generator().manual_seed(12)
+    n, HD = 900, 64
+    q = torch.randn((T, 2, HD), generator=g).cuda()
+    k, v = (torch.randn((n, 1, HD), generator=g) * size for _ in range(2))
+    cache = fill(k, v)
+    got = core.attention_kv4(q, cache, state(torch, n - T), scale=0.125 / size)
+    wk, wv = (t.cpu().numpy() for t in core.kv4_dequant(cache, 0, n))
+    want = kv4.attention(q[-40:].cpu().numpy(), wk, wv, n - min(T, 40), float(np.float32(0.125 / size)))
+    close(got[-40:], want, F32_REL)
+
+
+@pytest.mark.parametrize("dt", ["float32", "float16"])
+@pytest.mark.parametrize("T", [1, 3, 700])
+def test_tensors_off_a_16_byte_line(gpu, T, dt):
+    import torch
+    from webpytorch_amd import core
+    q, cache, st = _case(61, T=T, NH=2, NKV=1, pos=33, lmax=800)
+    q = q.to(getattr(torch, dt))
+    want = core.attention_kv4(q, cache, st)
+    off = lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)  # noqa: E731
+    out = off(torch.zeros_like(q))
+    core.attention_kv4(off(q), cache, st, out=out)
+    assert torch.equal(out, want)
+    cos, sin = tables(torch, 800, 64)
+    qkv = torch.randn((T, 4 * 64), generator=torch.Generator().manual_seed(3)).to(q.dtype).cuda()
+    a, b = core.kv4_cache(1, 800, 64), core.kv4_cache(1, 800, 64)
+    assert torch.equal(core.qk_norm_rope(qkv, st, cos, sin, 2, a), core.qk_norm_rope(off(qkv), st, off(cos), off(sin), 2, b)) and torch.equal(a, b)
+    with pytest.raises(ValueError, match="aligned"):
+        core.attention_kv4(q, off(cache), st)
+
+
+@pytest.mark.parametrize("T", [1, 5, 600])
+def test_a_cache_that_ends_inside_a_block(gpu, T):
+    """LMAX 45 through the C calls: positions from 45 on are not written, and tokens there attend up to 44."""
+    import torch
+    from webpytorch_amd import _lib, core
+    g = torch.Generator().manual_seed(13)
+    NH, NKV, HD, LMAX, pos = 4, 2, 64, 45, 30
+    x = torch.randn((LMAX, (NH + 2 * NKV) * HD), generator=g).cuda()
+    cos, sin = tables(torch, LMAX, HD)
+    cache = core.kv4_cache(NKV, LMAX, HD)
+    more = torch.randn((T + 20, (NH + 2 * NKV) * HD), generator=g).cuda()
+    P, q0 = core.ptr, torch.empty((LMAX + T + 20, NH, HD), device="cuda")
+    for rows, at in ((x, 0), (more, LMAX)):  # the second writes nothing
+        _lib.call("miq_qk_norm_rope_kv4", P(rows), 0, rows.shape[1], None, None, 1e-6, P(state(torch, at)), P(cos), P(sin), P(q0), P(cache),
+                  rows.shape[0], NH, NKV, HD, LMAX, None)
+    assert not torch.stack(core.kv4_dequant(cache, LMAX, 64 - LMAX)).any()
+    q, out = torch.randn((T, NH, HD), generator=g).cuda(), torch.empty((T, NH, HD), device="cuda")
+    _lib.call("miq_attention_kv4", P(q), 0, P(cache), P(state(torch, pos)), P(out), T, NH, NKV, HD, LMAX, 0.125, None, 0, None)
+    wk, wv = (t.cpu().numpy() for t in core.kv4_dequant(cache, 0, LMAX))
+    close(out, kv4.attention(q.cpu().numpy(), wk, wv, pos, 0.125), F32_REL)
+
+
 def test_argument_checks(gpu):
     import torch
     from webpytorch_amd import core
@@ -447,6 +506,8 @@ def test_argument_checks(gpu):
         core.attention_kv4(q, cache[:, ::2], st)
     with pytest.raises(ValueError, match="out is"):
         core.attention_kv4(q, cache, st, out=torch.empty((1, 8, 32), device="cuda"))
+    with pytest.raises(ValueError, match="apart from q"):
+        core.attention_kv4(q, cache, st, out=q)
     with pytest.raises(TypeError, match="state"):
         core.attention_kv4(q, cache, st.long())
     cos, sin = tables(torch, 4096, 64)

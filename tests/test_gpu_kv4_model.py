@@ -145,6 +145,28 @@ def test_persistent_step_with_logprobs_and_its_timeout(gpu, monkeypatch):
     assert all(torch.equal(x, y) for x, y in zip(a.generate(ids, 9, logprobs=4).logprobs, ra.logprobs))
 
 
+@pytest.mark.parametrize("mode", ["native", "requant"])
+def test_gguf_model_from_pretrained(gpu, tmp_path, mode):
+    """`kv_bits` through the loaders: a GGUF file in its own blocks (the unfused steps) and requantized, a context
+    that ends inside a block of the cache."""
+    from test_gpu_gguf_model import make_model, oracle_weights
+    from webpytorch_amd import llm
+    path = tmp_path / "m.gguf"
+    mats, floats = make_model(path)[:2]
+    m = llm.AutoModelForCausalLM.from_pretrained(str(path), dtype="auto" if mode == "native" else "int4", lmax=45, weights=mode, kv_bits=4)
+    ids = [int(i) for i in synth.prompt_ids(31, 37, 2048)]
+    tokens = m.generate(ids, 8).tokens
+    o = Kv4Oracle(oracle_weights(mats, floats, mode), lmax=64)
+    o.caches = [kv4.unpack(c.cpu().numpy(), 45) for c in m.kv4]
+    cache, pos, step = [None] * o.L, 0, ids
+    for n in range(1, 9):
+        _, want = o.forward(step, pos, cache)
+        assert m.generate(ids, n).tokens == tokens[:n]
+        lg = m.buf["logits"][0].cpu().numpy()
+        assert np.linalg.norm(lg - want) <= ORACLE_REL * np.linalg.norm(want)
+        pos, step = pos + len(step), tokens[n - 1:n]
+
+
 def test_refusals(gpu):
     w = synth.decoder_weights(27, **SMALL)
     for kw, exc in ((dict(kv_bits=8), ValueError), (dict(kv_bits=4, persistent=True), ValueError)):

@@ -121,6 +121,17 @@ def test_deterministic_in_graphs_and_on_streams(gpu):
         assert all(torch.equal(a, b) for a, b in zip(core.token_logprobs(*cases[1], 20), want[1]))
 
 
+def test_more_rows_than_one_launch_takes(gpu):
+    import torch
+    g = torch.Generator().manual_seed(9)
+    x, ids = torch.randn((70001, 9), generator=g).cuda(), torch.randint(0, 9, (70001,), generator=g, dtype=torch.int32).cuda()
+    from webpytorch_amd import core
+    got = core.token_logprobs(x, ids, 3)
+    want = torch.log_softmax(x.double(), 1)
+    assert float((got.logprobs - want.gather(1, ids.long()[:, None])[:, 0]).abs().max()) < 1e-5
+    assert torch.equal(got.top_ids, torch.sort(x, dim=1, descending=True, stable=True).indices[:, :3].int())
+
+
 def test_row_of_the_decode_state(gpu):
     import torch
     from webpytorch_amd import _lib, core
