@@ -167,6 +167,28 @@ def test_gguf_model_from_pretrained(gpu, tmp_path, mode):
         pos, step = pos + len(step), tokens[n - 1:n]
 
 
+def test_score_of_few_rows_needs_the_heads_workspace(gpu):
+    """2 to 8 rows of the head split K where one row does not: more workspace than the steps ever take."""
+    sh = dict(SMALL, L=1, H=1024, I=256, V=32768)
+    m = model(synth.decoder_weights(29, gaussian=True, **sh), 32)
+    ids = [int(i) for i in synth.prompt_ids(29, 20, sh["V"])]
+    whole = m.score(ids)
+    for n in (2, 3, 6, 9):
+        got = m.score(ids[:n])
+        assert np.allclose(got.logprobs.cpu().numpy(), whole.logprobs[:n - 1].cpu().numpy(), rtol=0, atol=1e-3)
+
+
+@pytest.mark.parametrize("k", [0, 16, 20, 32])
+def test_logprobs_of_a_large_vocabulary(gpu, k):
+    """The workspace holds any number of alternatives: of this vocabulary, 16 need more than 32."""
+    sh = dict(L=1, H=128, NH=2, NKV=1, HD=64, I=128, V=262144, gs=128, bits=4)
+    m = model(synth.decoder_weights(30, gaussian=True, **sh), 16)
+    r = m.generate([5, 6, 7], 4, logprobs=k)
+    assert r.logprobs.top_ids.shape == (4, k) and r.logprobs.ranks.tolist() == [0] * 4
+    if k:
+        assert r.logprobs.top_ids[:, 0].tolist() == r.tokens
+
+
 def test_refusals(gpu):
     w = synth.decoder_weights(27, **SMALL)
     for kw, exc in ((dict(kv_bits=8), ValueError), (dict(kv_bits=4, persistent=True), ValueError)):

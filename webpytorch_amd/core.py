@@ -296,8 +296,9 @@ def _gptq_matmul(xf, qweight, qzeros, scales, K, N, gs, bits, zoff=0.0, *, bias=
                   dtype_code(scales), ptr(bias), ptr(out), dtype_code(out), M, K, N, gs, bits,
                   float(zoff), ptr(ws), ws.numel(), stream_handle())
         return out
-    if ws is None:
-        ws = workspace(gemv_workspace_bytes(M, K, N, gs, bits, xd))
+    need = gemv_workspace_bytes(M, K, N, gs, bits, xd)
+    if ws is None or ws.numel() < need:
+        ws = workspace(need)
     _lib.call("miq_gptq_gemv", ptr(xf), xd, ptr(perm), ptr(qweight), ptr(qzeros),
               ptr(scales), dtype_code(scales), ptr(bias), ptr(out), dtype_code(out), M, K, N, gs,
               bits, float(zoff), ptr(ws), 0 if ws is None else ws.numel(), stream_handle())

@@ -347,14 +347,15 @@ class CausalLM:
             if "moe" in lay:
                 lins["router"] = lay["moe"]["router"]
         lins = {k: q for k, q in lins.items() if isinstance(q, _Lin)}  # GGUF kernels need no workspace
-        for M in range(1, T + 1):  # the head only ever sees the last token
+        for M in range(1, T + 1):  # of the head, a step only sees the last token
             for lin in lins.values():
                 need = max(need, core.gemv_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits, _lib.MIQ_F32))
                 if M > core.GEMV_MAX_M:  # prefill rows on the matrix cores
                     need = max(need, core.gemm_f32x_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits))
             if self.kv_bits == 4:
                 need = max(need, core.attention_kv4_workspace_bytes(M, self.NH, self.NKV, self.HD, self.lmax))
-        need = max(need, core.token_logprobs_workspace_bytes(1, self.V, min(self.V, core.MAX_TOP_LOGPROBS)))
+        for k in range(min(self.V, core.MAX_TOP_LOGPROBS) + 1):  # fewer alternatives may meet from more segments
+            need = max(need, core.token_logprobs_workspace_bytes(1, self.V, k))
         self.ws = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=dev)
         self._alloc_persistent()
 
