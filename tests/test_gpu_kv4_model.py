@@ -126,6 +126,39 @@ def test_context_past_the_fp32_attention(gpu):
     assert float((m.buf["logits"] - one).norm()) <= MODEL_REL * float(one.norm())
 
 
+@pytest.mark.parametrize("kv_bits", [None, 4])
+def test_prompts_in_pieces(gpu, kv_bits, monkeypatch):
+    """A prompt of several pieces (the last of one token, of some, whole) against the same in one."""
+    from webpytorch_amd import llm
+    sh = dict(SMALL, L=1)
+    w = synth.decoder_weights(32, gaussian=True, **sh)
+    ids = [int(i) for i in synth.prompt_ids(32, 48, sh["V"])]
+    a = model(w, 64, kv_bits=kv_bits)
+    monkeypatch.setattr(llm.CausalLM, "PREFILL_ROWS", 16)
+    b = model(w, 64, kv_bits=kv_bits)
+    assert b.buf["h"].shape[0] == 16 and b.history.shape[0] == 64
+    for n in (15, 16, 17, 33, 40, 48):
+        for m in (a, b):
+            m.generate(ids[:n], 3, use_graph=False)
+        assert int(b.state[0]) == n + 2
+        la, lb = a.buf["logits"], b.buf["logits"]
+        assert float((la - lb).norm()) <= MODEL_REL * float(la.norm())
+    sa, sb = a.score(ids, 2), b.score(ids, 2)
+    tol = MODEL_REL * float(la.norm())
+    assert sb.logprobs.shape == (47,) and float((sa.logprobs - sb.logprobs).abs().max()) < tol
+
+
+def test_long_context_of_wide_layers(gpu):
+    """40000 positions of a layer of 37888 columns: more rows at a time than its products are made for."""
+    sh = dict(SMALL, L=1, I=18944)
+    w = synth.decoder_weights(33, gaussian=True, **sh)
+    ids = [int(i) for i in synth.prompt_ids(33, 20, sh["V"])]
+    a, b = model(w, 40000, kv_bits=4), model(w, 64, kv_bits=4)
+    assert a.generate(ids, 5).tokens == b.generate(ids, 5).tokens
+    # 16384 rows of 18944 values as two fp16 numbers (1.24e9 bytes), not the GEMV's sums of as many rows (35e9)
+    assert a.ws.numel() < 1.3e9
+
+
 def test_persistent_step_with_logprobs_and_its_timeout(gpu, monkeypatch):
     import torch
     w = synth.decoder_weights(26, gaussian=True, **SMALL)

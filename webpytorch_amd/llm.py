@@ -183,6 +183,9 @@ class CausalLM:
     contexts past the fp32 attention's 16384 positions); the steps are then launch sequences."""
 
     SCORE_ROWS = 256  # rows of logits that `score` holds at a time
+    # tokens that go through the layers at a time (a longer prompt goes in pieces): the products' offsets and grids
+    # are made for these, and the activations of 131072 tokens of the 7B shape would take 50 GB
+    PREFILL_ROWS = 16384
 
     def __init__(self, weights, lmax=256, fused=True, persistent=None, kv_bits=None):
         c = weights["cfg"]
@@ -310,7 +313,7 @@ class CausalLM:
         return _Lin({"qweight": qw, "qzeros": qz, "scales": sc}, K, self.gs, self.bits, 0.0)
 
     def _alloc(self):
-        dev, f32, T = core.device(), torch.float32, self.lmax
+        dev, f32, T = core.device(), torch.float32, min(self.lmax, self.PREFILL_ROWS)
         z = lambda *s: torch.zeros(s, dtype=f32, device=dev)  # noqa: E731
         qkvd = (self.NH + 2 * self.NKV) * self.HD
         self.buf = {"h": z(T, self.H), "xn": z(T, self.H), "qkv": z(T, qkvd), "q": z(T, self.NH * self.HD),
@@ -327,14 +330,15 @@ class CausalLM:
             self.vc = torch.zeros_like(self.kc)
         # RoPE tables exactly as `_rope_np` builds them (float64 angles, rounded once to fp32)
         inv = 1.0 / (self.theta ** (np.arange(0, self.HD, 2, dtype=np.float64) / self.HD))
-        ang = np.arange(0, T, dtype=np.float64)[:, None] * inv[None, :]
+        ang = np.arange(0, self.lmax, dtype=np.float64)[:, None] * inv[None, :]
         self.cos_t = core.to_device(np.cos(ang).astype(np.float32))
         self.sin_t = core.to_device(np.sin(ang).astype(np.float32))
         self.ids = torch.zeros(T, dtype=torch.int32, device=dev)
-        self.history = torch.zeros(T, dtype=torch.int32, device=dev)
+        self.history = torch.zeros(self.lmax, dtype=torch.int32, device=dev)
         self.state = torch.zeros(_lib.lib().miq_decode_state_words(), dtype=torch.int32, device=dev)
         # one split-K workspace sized for every projection at T = 1 and at the largest prefill
-        # (the need is not monotonic in the row count: wide enough layers stop splitting K)
+        # (the need is not monotonic in the row count: wide enough layers stop splitting K; a product that
+        # needs more, as prompts off the matrix cores do, takes the stream's workspace)
         need = 0
         if isinstance(self.head, _Lin):
             need = core.gemv_workspace_bytes(1, self.head.K, self.head.N, self.gs, self.bits, _lib.MIQ_F32)
@@ -349,8 +353,9 @@ class CausalLM:
         lins = {k: q for k, q in lins.items() if isinstance(q, _Lin)}  # GGUF kernels need no workspace
         for M in range(1, T + 1):  # of the head, a step only sees the last token
             for lin in lins.values():
-                need = max(need, core.gemv_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits, _lib.MIQ_F32))
-                if M > core.GEMV_MAX_M:  # prefill rows on the matrix cores
+                if M <= core.GEMV_MAX_M:
+                    need = max(need, core.gemv_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits, _lib.MIQ_F32))
+                else:  # prefill rows on the matrix cores
                     need = max(need, core.gemm_f32x_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits))
             if self.kv_bits == 4:
                 need = max(need, core.attention_kv4_workspace_bytes(M, self.NH, self.NKV, self.HD, self.lmax))
@@ -629,6 +634,22 @@ class CausalLM:
         if self.pws is not None:
             self.pws.zero_()  # epoch and every exchange tag back to zero (never a valid tag)
 
+    def _place(self, ids, pos):
+        """Tokens for the layers, at positions from pos on."""
+        self.ids[:len(ids)].copy_(torch.tensor(ids, dtype=torch.int32))
+        if pos:
+            self.state[:1].fill_(pos)
+
+    def _lead(self, ids):
+        """The layers over the pieces of a prompt ahead of its last one (the first is in place): their keys and
+        values. Returns how many tokens the last one has, in place for a step."""
+        rows, pos = int(self.ids.shape[0]), 0
+        while len(ids) - pos > rows:
+            self._layers(rows)
+            pos += rows
+            self._place(ids[pos:pos + rows], pos)
+        return len(ids) - pos
+
     def _plan_length(self, n_prompt, max_new):
         """Refuse sequences that do not fit the KV cache (`webtorch/llm.py:1397-1429`)."""
         if n_prompt < 1 or max_new < 1:
@@ -681,17 +702,20 @@ class CausalLM:
             raise ValueError("score takes 2 .. lmax (%d) tokens, got %d" % (self.lmax, len(ids)))
         self._logprob_rows(top_k)
         self.reset()
-        self.ids[:n + 1].copy_(torch.tensor(ids, dtype=torch.int32))
-        given = self.ids[1:n + 1].clone()
-        self._layers(n)
-        parts, rows = [], self.SCORE_ROWS
+        given = core.to_device(np.asarray(ids[1:], dtype=np.int32))
+        parts, rows, piece = [], self.SCORE_ROWS, int(self.ids.shape[0])
         logits = torch.empty((min(n, rows), self.V), dtype=torch.float32, device=core.device())
-        for t0 in range(0, n, rows):
-            m = min(rows, n - t0)
-            h = self.buf["h"][t0:t0 + m]
-            _lib.call("miq_rmsnorm", ptr(h), ptr(self.final_norm), ptr(self.buf["xn"]), m, self.H, self.eps, stream_handle())
-            self._linear(self.head, self.buf["xn"][:m], logits[:m])
-            parts.append(core.token_logprobs(logits[:m], given[t0:t0 + m], top_k))
+        for p0 in range(0, n, piece):
+            p1 = min(n, p0 + piece)
+            self._place(ids[p0:p1], p0)
+            self._layers(p1 - p0)
+            for t0 in range(p0, p1, rows):
+                m = min(rows, p1 - t0)
+                h = self.buf["h"][t0 - p0:t0 - p0 + m]
+                _lib.call("miq_rmsnorm", ptr(h), ptr(self.final_norm), ptr(self.buf["xn"]), m, self.H, self.eps,
+                          stream_handle())
+                self._linear(self.head, self.buf["xn"][:m], logits[:m])
+                parts.append(core.token_logprobs(logits[:m], given[t0:t0 + m], top_k))
         return parts[0] if len(parts) == 1 else core.TokenLogprobs(*(torch.cat(p) for p in zip(*parts)))
 
     def generate(self, ids, max_new, use_graph=True, logprobs=None):
@@ -709,10 +733,10 @@ class CausalLM:
 
     def _generate(self, ids, max_new, use_graph):
         self.reset()
-        self.ids[:len(ids)].copy_(torch.tensor(ids, dtype=torch.int32))
+        self._place(ids[:int(self.ids.shape[0])], 0)
         torch.cuda.synchronize()
         t0 = time.perf_counter()
-        self._step(len(ids))
+        self._step(self._lead(ids))
         torch.cuda.synchronize()
         ttft = time.perf_counter() - t0
         chunks = self._chunks(max_new - 1)
