@@ -31,6 +31,8 @@ def call(name, **over):
     ("miq_qk_norm_rope_kv", dict(ld=255), ValueError, "255 values|rows 255"),
     ("miq_qk_norm_rope_kv", dict(kc=None), ValueError, "null"),
     ("miq_qk_norm_rope_kv", dict(T=-1), ValueError, "T=-1"),
+    ("miq_qk_norm_rope_kv", dict(T=1 << 26), NotImplementedError, "past the grid"),
+    ("miq_qk_norm_rope_kv4", dict(T=1 << 26), NotImplementedError, "past the grid"),
     ("miq_qk_norm_rope_kv4", dict(HD=80, ld=4096), NotImplementedError, "HD=80"),
     ("miq_qk_norm_rope_kv4", dict(dt=2), NotImplementedError, "dtype 2"),
     ("miq_qk_norm_rope_kv4", dict(cache=264), ValueError, "aligned"),

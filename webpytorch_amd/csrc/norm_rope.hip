@@ -310,6 +310,9 @@ extern "C" int miq_kv4_cache_bytes(int NKV, int LMAX, int HD, size_t* bytes) {
   return MIQ_OK;
 }
 
+// a launch has fewer than 2^32 threads
+static bool grid_holds(int64_t units) { return units <= (int64_t)kNrWaves * ((1 << 24) - 1); }
+
 static int check_norm_rope(const char* what, const void* qkv, int64_t ld, const int32_t* state, const float* cos_tab,
                            const float* sin_tab, const void* q_out, int T, int NH, int NKV, int HD, int LMAX) {
   MIQ_REQUIRE(T >= 0 && NH > 0 && NKV > 0 && NH % NKV == 0 && NH <= (1 << 16) && HD > 0 && HD % 2 == 0 && HD <= 256 && LMAX > 0 &&
@@ -317,7 +320,6 @@ static int check_norm_rope(const char* what, const void* qkv, int64_t ld, const 
               MIQ_ERR_INVALID, "%s: T=%d NH=%d NKV=%d HD=%d LMAX=%d", what, T, NH, NKV, HD, LMAX);
   MIQ_REQUIRE(ld >= (int64_t)(NH + 2 * NKV) * HD, MIQ_ERR_INVALID, "%s: rows %lld apart hold %lld values", what, (long long)ld,
               (long long)(NH + 2 * NKV) * HD);
-  MIQ_REQUIRE((int64_t)T * (NH + 2 * NKV) / kNrWaves < 0x7FFFFFFF - 1, MIQ_ERR_UNSUPPORTED, "%s: T=%d is past the grid", what, T);
   MIQ_REQUIRE(T == 0 || (qkv && state && cos_tab && sin_tab && q_out), MIQ_ERR_INVALID, "%s: null pointer", what);
   return MIQ_OK;
 }
@@ -330,6 +332,7 @@ extern "C" int miq_qk_norm_rope_kv(const float* qkv, int64_t ld, const float* qn
   MIQ_REQUIRE(kcache && vcache, MIQ_ERR_INVALID, "qk_norm_rope_kv: null pointer");
   const int heads = NH + 2 * NKV, U = several_heads(T, heads) ? kNrHeads : 1;
   const int64_t units = (int64_t)T * ((heads + U - 1) / U);
+  MIQ_REQUIRE(grid_holds(units), MIQ_ERR_UNSUPPORTED, "qk_norm_rope_kv: T=%d is past the grid", T);
   const dim3 grid((unsigned)((units + kNrWaves - 1) / kNrWaves)), block(64 * kNrWaves);
   const hipStream_t st = static_cast<hipStream_t>(stream);
 #define MIQ_NR(HDV, UV)                                                                                                     \
@@ -358,9 +361,10 @@ extern "C" int miq_qk_norm_rope_kv4(const void* qkv, int x_dtype, int64_t ld, co
   MIQ_REQUIRE(cache, MIQ_ERR_INVALID, "qk_norm_rope_kv4: null pointer");
   MIQ_REQUIRE(aligned(cache, 16), MIQ_ERR_ALIGN, "qk_norm_rope_kv4: the cache must be 16-byte aligned");
   // T rows lie in at most this many blocks, wherever the first one is
-  const int vblocks = (T + kKv4Block - 2) / kKv4Block + 1;
+  const int vblocks = (int)(((int64_t)T + kKv4Block - 2) / kKv4Block) + 1;
   const int U = several_heads(T, NH + NKV) ? kNrHeads4 : 1;
   const int64_t units = (int64_t)T * ((NH + U - 1) / U + NKV) + (int64_t)vblocks * NKV * 4 * (HD / 64);
+  MIQ_REQUIRE(grid_holds(units), MIQ_ERR_UNSUPPORTED, "qk_norm_rope_kv4: T=%d is past the grid", T);
   const dim3 grid((unsigned)((units + kNrWaves - 1) / kNrWaves)), block(64 * kNrWaves);
   const hipStream_t st = static_cast<hipStream_t>(stream);
 #define MIQ_NR(HDV, XT, UV)                                                                                       \
