@@ -13,8 +13,8 @@
 // Bound and measured (us in graph replay; the floor is the larger of the bytes at a large copy's 4.8 TB/s and the
 // operations at a large fp16 product's 1180 TFLOP/s, twice for fp32 rows): one token of 32 / 8 heads of 128 behind
 // 131000 positions 42 (168 MB, 4.0 TB/s; floor 35: 80 KB in flight a CU); behind 700 positions of 14 / 2 heads of 64
-// 7.5 (round trips); 2000 fp32 rows of 28 / 4 heads of 128 from an empty cache 84 (floor 49), 6001 fp16 rows 323
-// (floor 219), 77 fp16 tokens of 32 / 8 heads behind 30000 72 and 9 to join 21 slices (floor 32): the vector units
+// 7.5 (round trips); 2000 fp32 rows of 28 / 4 heads of 128 from an empty cache 85 (floor 49), 6001 fp16 rows 328
+// (floor 219), 77 fp16 tokens of 32 / 8 heads behind 30000 59 and 9 to join 21 slices (floor 32): the vector units
 // (exponentials at a quarter of their rate, maxima, rounding, unpacking: half of the time) and the matrix cores (a
 // third) overlap little with two or three waves a SIMD.
 #include <math.h>
@@ -606,6 +606,17 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
     fetch_k(s0 + 2);
     refer(s0);
     __syncthreads();
+  }
+  if (rw >= R) {  // a wave without rows only unpacks (77 tokens of 4 heads a kv head behind 30000: 81 -> 76.5 us)
+    for (int step = s0; step < s1; ++step) {
+      check_v(step + 1);
+      stage_k(step + 2);
+      stage_v(step + 1);
+      fetch_k(step + 3);
+      fetch_v(step + 2);
+      __syncthreads();
+    }
+    return;
   }
   for (int step = s0; step < s1; ++step) {
     check_v(step + 1);
