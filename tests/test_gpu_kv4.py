@@ -435,6 +435,21 @@ def test_many_rows_in_a_graph(gpu):
         assert torch.equal(out, eager) and (pos != 4000 or torch.equal(out, want))
 
 
+@pytest.mark.parametrize("dt", ["float32", "float16"])
+@pytest.mark.parametrize("T", [5, 40, 700])
+def test_a_token_does_not_depend_on_its_neighbours(gpu, T, dt):
+    """Other tokens' queries, steep ones that raise their references often, leave a token's bits as they are."""
+    import torch
+    from webpytorch_amd import core
+    q, cache, st = _case(71, T=T, NH=4, NKV=2, pos=500, lmax=2048)
+    q = q.to(getattr(torch, dt))
+    steep = q.clone()
+    steep[::2] *= 40
+    a, b = (core.attention_kv4(x, cache, st) for x in (q, steep))
+    assert torch.equal(a[1::2], b[1::2]) and torch.isfinite(b).all()
+    close(b, _torch_want(steep, cache, 500).cpu().numpy(), 1e-4 if dt == "float32" else 2 * F16_REL)
+
+
 @pytest.mark.parametrize("size", [2e-6, 3e-5, 1e-3])
 @pytest.mark.parametrize("T", [1, 700])
 def test_values_below_the_normal_fp16_range(gpu, size, T):

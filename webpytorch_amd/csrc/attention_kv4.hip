@@ -7,12 +7,12 @@
 // words of the cache are unpacked in registers, in operand order (kv4.h), and no value moves between lanes
 // from the scores to the output. K and V are exact fp16; fp32 rows take q and p as two fp16 numbers each
 // (hi + lo: 22 bits; q scaled by a power of two per row), fp16 rows take one (q is exact, p rounded to
-// fp16: 2^-12 of a probability). Sums and softmax statistics are fp32. p is held times 2^14, so that its
+// fp16: 2^-12 of a probability). Sums and softmax statistics are fp32. p is held times 2^7 or more, so that its
 // lower part stays in fp16's normal range.
 //
 // Bound and measured (us in graph replay; the floor is the larger of the bytes at a large copy's 4.8 TB/s and the
 // operations at a large fp16 product's 1180 TFLOP/s, twice for fp32 rows): one token of 32 / 8 heads of 128 behind
-// 131000 positions 42 (168 MB, 4.0 TB/s; floor 35: 80 KB in flight a CU); behind 700 positions of 14 / 2 heads of 64
+// 131000 positions 41 (168 MB, 4.1 TB/s; floor 35: 80 KB in flight a CU); behind 700 positions of 14 / 2 heads of 64
 // 7.5 (round trips); 2000 fp32 rows of 28 / 4 heads of 128 from an empty cache 85 (floor 49), 6001 fp16 rows 328
 // (floor 219), 77 fp16 tokens of 32 / 8 heads behind 30000 59 and 9 to join 21 slices (floor 32): the vector units
 // (exponentials at a quarter of their rate, maxima, rounding, unpacking: half of the time) and the matrix cores (a
@@ -25,7 +25,10 @@ namespace miq {
 
 constexpr int kA4Waves = 8;
 constexpr int kA4Rows = 16;
-constexpr float kA4Unit = 16384.f;  // a probability of 1
+// The reference of the exponentials is raised only when a score passes it by more than 2^8 (a probability, 2^7 at the
+// reference, then stays below 2^15), so that the output is seldom rescaled (131000 positions 50 -> 47 us a replay); each
+// row by its own scores alone, so that a token's bits do not depend on its neighbours' queries.
+constexpr float kA4UnitLog2 = 7.f, kA4Slack = 8.f;
 constexpr int kA4CtrStride = 32;    // ints between arrival counters: a 128-byte line each
 constexpr int kA4MaxSlices = 64;
 constexpr int kA4MinSteps = 8;      // key steps of a slice of many rows, at least
@@ -247,7 +250,7 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
 
   float4v o[NT];
   float4v l = (float4v){0.f, 0.f, 0.f, 0.f};  // the sum of probabilities, in every row of the product
-  float m = -INFINITY;
+  float m = -INFINITY, neg = kA4UnitLog2;  // the reference, and what is added to a score for the exponent
 #pragma unroll
   for (int i = 0; i < NT; ++i) o[i] = (float4v){0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](Raw& w, int blk) __attribute__((always_inline)) {
@@ -273,25 +276,26 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        float v = s[b][x] * back;
-        if (masked && blk * kKv4Block + 16 * b + 4 * g + x > lim) v = -INFINITY;
-        s[b][x] = v;
-        mx = fmaxf(mx, v);
+        if (masked && blk * kKv4Block + 16 * b + 4 * g + x > lim) s[b][x] = -INFINITY;
+        mx = fmaxf(mx, s[b][x]);
       }
-    const float mn = fmaxf(m, rows_max(mx));
-    const float ref = mn == -INFINITY ? 0.f : mn;  // no key yet: every probability is 0
-    const float alpha = __builtin_amdgcn_exp2f(m - ref);
-    m = mn;
+    mx = rows_max(mx) * back;
+    if (__ballot(mx > m + kA4Slack)) {
+      const float mn = mx > m + kA4Slack ? mx : m;
+      const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      neg = kA4UnitLog2 - (mn == -INFINITY ? 0.f : mn);  // no key yet: every probability is 0
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[i] *= alpha;
+    }
     half8v ph[P];
     float p8[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - ref) * kA4Unit;
+    for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], back, neg));
     split_p<P>(p8, ph);
-    l *= alpha;
 #pragma unroll
     for (int p = P - 1; p >= 0; --p) l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones(), ph[p], l, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) o[i] *= alpha;
 
     // ---- values ----
     // keys behind the last one hold anything: their S and Z are cleared. A group with a NaN or an
@@ -400,11 +404,7 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
 // them), 32 at a time (64 for HD 64). The waves unpack the records' words together, once for all rows, into
 // operands in LDS, in operand order: each write and read is 16 consecutive bytes a lane. Two buffers, one
 // barrier a step: while a step's products run, the next step's words, loaded a step before that, are unpacked.
-// The reference of the exponentials is raised only when a score passes it by more than 2^8 (p then stays
-// below 2^15), so that the output is seldom rescaled.
 constexpr int kA4TileWaves = 4;
-constexpr float kA4TileUnitLog2 = 7.f;  // a probability of 1 is 2^7 at the reference
-constexpr float kA4Slack = 8.f;
 // blocks of a step and 16-row tiles of a wave: what the registers hold (fp32 rows take twice the operands)
 __host__ __device__ constexpr int kv4_step_blocks(int HD, bool f32) { return HD == 64 ? 2 : HD == 128 && !f32 ? 2 : 1; }
 __host__ __device__ constexpr int kv4_tile_qt(int HD, bool f32) { return HD <= 128 && !f32 ? 2 : 1; }
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     m[i] = -INFINITY;
-    neg[i] = kA4TileUnitLog2;
+    neg[i] = kA4UnitLog2;
     l[i] = (float4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[i][n] = (float4v){0.f, 0.f, 0.f, 0.f};
@@ -579,10 +579,10 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
     if (__ballot(raise)) {
 #pragma unroll
       for (int i = 0; i < QT; ++i) {
-        const float mn = fmaxf(m[i], mx[i]);
+        const float mn = mx[i] > m[i] + kA4Slack ? mx[i] : m[i];
         const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i] - mn);
         m[i] = mn;
-        neg[i] = kA4TileUnitLog2 - (mn == -INFINITY ? 0.f : mn);  // no key yet: every probability is 0
+        neg[i] = kA4UnitLog2 - (mn == -INFINITY ? 0.f : mn);  // no key yet: every probability is 0
         l[i] *= alpha;
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[i][n] *= alpha;
