@@ -962,7 +962,7 @@ def kv4_dequant(cache, start=0, n=None):
     n = lmax - start if n is None else n
     if start < 0 or n < 0 or start + n > lmax:
         raise ValueError("positions %d .. %d of a cache of %d" % (start, start + n - 1, lmax))
-    k = torch.empty((nkv, n, hd), dtype=torch.float32, device=cache.device)
+    k = torch.empty(nkv, n, hd, dtype=torch.float32, device=dev)
     v = torch.empty_like(k)
     _lib.call("miq_kv4_dequant_f32", cache.data_ptr(), k.data_ptr(), v.data_ptr(), nkv, lmax, hd, start, n, _raw_stream(dev))
     return k, v
@@ -1007,7 +1007,7 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
     if qkv.stride(1) != 1 or (T > 1 and qkv.stride(0) < W):
         qkv = qkv.contiguous()
     if out is None:
-        out = torch.empty((T, n_heads, hd), dtype=qkv.dtype, device=qkv.device)
+        out = torch.empty(T, n_heads, hd, dtype=qkv.dtype, device=dev)
     else:
         _check_tensor("out", out, (qkv.dtype,), None, dev)
         if out.numel() != T * n_heads * hd or not out.is_contiguous() or out.data_ptr() == qkv.data_ptr() != 0:
@@ -1070,10 +1070,10 @@ def token_logprobs(logits, ids, top_k=0):
     if ids.dtype != torch.int32:
         ids = ids.clamp(-1, 0x7FFFFFFF).to(torch.int32)
     ids = ids.contiguous()
-    where, f32, i32 = logits.device, torch.float32, torch.int32
-    lp, ent, rank = (torch.empty(T, dtype=f32, device=where), torch.empty(T, dtype=f32, device=where),
-                     torch.empty(T, dtype=i32, device=where))
-    ti, tl = torch.empty((T, top_k), dtype=i32, device=where), torch.empty((T, top_k), dtype=f32, device=where)
+    f32, i32 = torch.float32, torch.int32
+    lp, rank = torch.empty(T, dtype=f32, device=dev), torch.empty(T, dtype=i32, device=dev)
+    tl, ti = torch.empty(T, top_k, dtype=f32, device=dev), torch.empty(T, top_k, dtype=i32, device=dev)
+    ent = torch.empty_like(lp)
     ld, code, st = logits.stride(0) if T > 1 else V, dtype_code(logits), _raw_stream(dev)
     for t0 in range(0, T, 65535):  # rows of one launch
         n = min(T - t0, 65535)
