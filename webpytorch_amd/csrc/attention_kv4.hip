@@ -14,9 +14,9 @@
 // operations at a large fp16 product's 1180 TFLOP/s, twice for fp32 rows): one token of 32 / 8 heads of 128 behind
 // 131000 positions 41 (168 MB, 4.1 TB/s; floor 35: 80 KB in flight a CU); behind 700 positions of 14 / 2 heads of 64
 // 7.5 (round trips); 2000 fp32 rows of 28 / 4 heads of 128 from an empty cache 85 (floor 49), 6001 fp16 rows 328
-// (floor 219), 77 fp16 tokens of 32 / 8 heads behind 30000 59 and 9 to join 21 slices (floor 32): the vector units
-// (exponentials at a quarter of their rate, maxima, rounding, unpacking: half of the time) and the matrix cores (a
-// third) overlap little with two or three waves a SIMD.
+// (floor 219), 77 fp16 tokens of 32 / 8 heads behind 30000 59 and 9 to join 21 slices (floor 32): bound by
+// the issue of instructions (2000 rows: a wave and step of 32 keys have 160 vector and 34 matrix instructions, 2700 of
+// the 3200 cycles that three waves of a SIMD take; a third of the vector instructions unpack).
 #include <math.h>
 
 #include "kv4.h"
