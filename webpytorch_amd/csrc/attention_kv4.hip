@@ -12,9 +12,9 @@
 //
 // Bound and measured (us in graph replay; the floor is the larger of the bytes at a large copy's 4.8 TB/s and the
 // operations at a large fp16 product's 1180 TFLOP/s, twice for fp32 rows): one token of 32 / 8 heads of 128 behind
-// 131000 positions 41 (168 MB, 4.1 TB/s; floor 35: 80 KB in flight a CU); behind 700 positions of 14 / 2 heads of 64
-// 7.5 (round trips); 2000 fp32 rows of 28 / 4 heads of 128 from an empty cache 85 (floor 49), 6001 fp16 rows 328
-// (floor 219), 77 fp16 tokens of 32 / 8 heads behind 30000 59 and 9 to join 21 slices (floor 32): bound by
+// 131000 positions 42 (168 MB, 4.0 TB/s; floor 35: 80 KB in flight a CU); behind 700 positions of 14 / 2 heads of 64
+// 7.5 (round trips); 2000 fp32 rows of 28 / 4 heads of 128 from an empty cache 83 (floor 49), 6001 fp16 rows 321
+// (floor 219), 77 fp16 tokens of 32 / 8 heads behind 30000 56 and 9 to join 21 slices (floor 32): bound by
 // the issue of instructions (2000 rows: a wave and step of 32 keys have 160 vector and 34 matrix instructions, 2700 of
 // the 3200 cycles that three waves of a SIMD take; a third of the vector instructions unpack).
 #include <math.h>
@@ -53,7 +53,7 @@ __device__ __forceinline__ half8v unpack_key(uint32_t w, uint32_t meta) {
               fma2(kv4_pair<3>(w), S, Z));
 }
 // of a value word: S and Z of its 8 keys in pairs
-__device__ __forceinline__ half8v unpack_value(uint32_t w, const uint32_t* S, const uint32_t* Z) {
+__device__ __forceinline__ half8v unpack_value(uint32_t w, miq_u32x4 S, miq_u32x4 Z) {
   return cat4(fma2(kv4_pair<0>(w), as_h2(S[0]), as_h2(Z[0])), fma2(kv4_pair<1>(w), as_h2(S[1]), as_h2(Z[1])),
               fma2(kv4_pair<2>(w), as_h2(S[2]), as_h2(Z[2])), fma2(kv4_pair<3>(w), as_h2(S[3]), as_h2(Z[3])));
 }
@@ -170,7 +170,7 @@ __device__ __forceinline__ half8v ones() { return (half8v){1, 1, 1, 1, 1, 1, 1, 
 
 // Groups with a NaN or an infinity (S negative) among a lane's 8 keys: their S and Z are cleared; the
 // return value has a bit for each such key of the block (all lanes together).
-__device__ __forceinline__ uint32_t clear_bad(uint32_t* S, uint32_t* Z) {
+__device__ __forceinline__ uint32_t clear_bad(miq_u32x4& S, miq_u32x4& Z) {
   uint32_t hit = 0;
   const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
@@ -222,7 +222,8 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
   // ---- a block's words: the next one's are loaded while one is multiplied, where the registers hold both ----
   constexpr int NR = HD <= 128 ? 2 : 1;
   struct Raw {
-    uint32_t kw[NT], vw[NT], km[2][NJ], vm[NJ][8];
+    uint32_t kw[NT], vw[NT], km[2][NJ];
+    miq_u32x4 vs[NJ], vz[NJ];
   } raw[NR];
   auto load = [&](Raw& x, int blk) __attribute__((always_inline)) {
     const uint8_t* rec = C + (size_t)blk * kv4_record(HD);
@@ -237,10 +238,10 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
     for (int u = 0; u < NT / 4; ++u)
       *reinterpret_cast<uint4*>(&x.vw[4 * u]) = *reinterpret_cast<const uint4*>(rec + kv4_vcodes(HD) + (u * 64 + lane) * 16);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        *reinterpret_cast<uint4*>(&x.vm[j][4 * u]) = *reinterpret_cast<const uint4*>(rec + kv4_vmeta(HD) + (j * 4 + g) * 32 + 16 * u);
+    for (int j = 0; j < NJ; ++j) {
+      x.vs[j] = *reinterpret_cast<const miq_u32x4*>(rec + kv4_vmeta(HD) + (j * 4 + g) * 32);
+      x.vz[j] = *reinterpret_cast<const miq_u32x4*>(rec + kv4_vmeta(HD) + (j * 4 + g) * 32 + 16);
+    }
   };
   const bool work = b0 + wave < b1;  // wave-uniform
   if (work) load(raw[0], b0 + wave);
@@ -257,7 +258,8 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
     auto& kw = w.kw;
     auto& vw = w.vw;
     auto& km = w.km;
-    auto& vm = w.vm;
+    auto& vs = w.vs;
+    auto& vz = w.vz;
     // ---- scores ----
     float4v s[2];
 #pragma unroll
@@ -306,8 +308,8 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
         const uint32_t keep = keep_pair(blk * kKv4Block + kv4_key(g, 2 * p), S);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          vm[j][p] &= keep;
-          vm[j][4 + p] &= keep;
+          vs[j][p] &= keep;
+          vz[j][p] &= keep;
         }
       }
     }
@@ -315,15 +317,15 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int p = 0; p < 4; ++p) odd |= vm[j][p];
+      for (int p = 0; p < 4; ++p) odd |= vs[j][p];
     const bool bad = __ballot((odd & 0x80008000u) != 0) != 0ull;
     uint32_t hit[NJ] = {};  // keys whose group j is bad
     if (bad)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) hit[j] = clear_bad(&vm[j][0], &vm[j][4]);
+      for (int j = 0; j < NJ; ++j) hit[j] = clear_bad(vs[j], vz[j]);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const half8v v = unpack_value(vw[i], &vm[i >> 1][0], &vm[i >> 1][4]);
+      const half8v v = unpack_value(vw[i], vs[i >> 1], vz[i >> 1]);
 #pragma unroll
       for (int p = P - 1; p >= 0; --p) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[p], o[i], 0, 0, 0);
     }
@@ -445,7 +447,8 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
 
   // ---- words on their way: numbers n0 .. of a step's K and V words ----
   const int n0 = wave * WPW % NT, bo = wave * WPW / NT;
-  uint32_t kw[WPW], km[WPW], vw[WPW], vm[NM][8];
+  uint32_t kw[WPW], km[WPW], vw[WPW];
+  miq_u32x4 vs[NM], vz[NM];  // vectors: the loads of arrays of words were merged across S and Z and waited for at once (+1.5 %)
   auto words = [&](const uint8_t* part, uint32_t* w) __attribute__((always_inline)) {
     const uint8_t* at = part + kv4_word(n0, g, c);
     if constexpr (WPW == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(at);
@@ -465,11 +468,11 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
     const uint8_t* rec = C + (size_t)min(step * NBK + bo, nblk - 1) * kv4_record(HD);
     words(rec + kv4_vcodes(HD), vw);
 #pragma unroll
-    for (int x = 0; x < NM; ++x)
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-        *reinterpret_cast<uint4*>(&vm[x][4 * y]) =
-            *reinterpret_cast<const uint4*>(rec + kv4_vmeta(HD) + (((n0 + x * (WPW / NM)) / 2 * 4 + g) * 2 + y) * 16);
+    for (int x = 0; x < NM; ++x) {
+      const miq_u32x4* at = reinterpret_cast<const miq_u32x4*>(rec + kv4_vmeta(HD) + ((n0 + x * (WPW / NM)) / 2 * 4 + g) * 32);
+      vs[x] = at[0];
+      vz[x] = at[1];
+    }
   };
   // S and Z of step's values made fit: keys behind the last one hold anything and are cleared; so are groups
   // with a NaN or an infinity, which are noted for the rows
@@ -481,8 +484,8 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
         const uint32_t keep = keep_pair(k0 + kv4_key(g, 2 * p), S);
 #pragma unroll
         for (int x = 0; x < NM; ++x) {
-          vm[x][p] &= keep;
-          vm[x][4 + p] &= keep;
+          vs[x][p] &= keep;
+          vz[x][p] &= keep;
         }
       }
     }
@@ -490,12 +493,12 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
 #pragma unroll
     for (int x = 0; x < NM; ++x)
 #pragma unroll
-      for (int p = 0; p < 4; ++p) neg |= vm[x][p];
+      for (int p = 0; p < 4; ++p) neg |= vs[x][p];
     const bool bad = __ballot((neg & 0x80008000u) != 0) != 0ull;
     uint32_t hit[NM] = {};
     if (bad)
 #pragma unroll
-      for (int x = 0; x < NM; ++x) hit[x] = clear_bad(&vm[x][0], &vm[x][4]);
+      for (int x = 0; x < NM; ++x) hit[x] = clear_bad(vs[x], vz[x]);
     if (lane == 0) {
       flags[step & 1][wave] = bad;
 #pragma unroll
@@ -510,7 +513,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
   auto stage_v = [&](int step) __attribute__((always_inline)) {
     half8v* dst = ops + ((size_t)(2 + (step & 1)) * NBK * NT + wave * WPW) * 64 + lane;
 #pragma unroll
-    for (int x = 0; x < WPW; ++x) dst[x * 64] = unpack_value(vw[x], &vm[x * NM / WPW][0], &vm[x * NM / WPW][4]);
+    for (int x = 0; x < WPW; ++x) dst[x * 64] = unpack_value(vw[x], vs[x * NM / WPW], vz[x * NM / WPW]);
   };
 
   // ---- q as matrix-core operands; scores in units of log 2, their factor positive ----
