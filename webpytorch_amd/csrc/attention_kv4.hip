@@ -5,10 +5,11 @@
 // A kv head's queries are rows r = t rep + hh (rep = NH / NKV heads share its keys and values), 16
 // to a tile. A wave multiplies transposed on the fp16 matrix cores: S^T = K Q^T, then O^T = V^T P^T; the
 // words of the cache are unpacked in registers, in operand order (kv4.h), and no value moves between lanes
-// from the scores to the output. K and V are exact fp16; fp32 rows take q and p as two fp16 numbers each
-// (hi + lo: 22 bits; q scaled by a power of two per row), fp16 rows take one (q is exact, p rounded to
-// fp16: 2^-12 of a probability). Sums and softmax statistics are fp32. p is held times 2^7 or more, so that its
-// lower part stays in fp16's normal range.
+// from the scores to the output. K and V are exact fp16; p is two fp16 numbers (hi + lo: 22 bits), and so is q of
+// fp32 rows (scaled by a power of two per row); q of fp16 rows is exact. Sums and softmax statistics are fp32. p is held
+// times 2^7 or more, so that its lower part stays in fp16's normal range. (p of fp16 rows as one number cost the output as
+// much again as its own rounding, 2.7e-4 of float64 instead of 2.0e-4, and saved a third of the matrix instructions:
+// 6001 rows of 28 / 4 heads of 128 326 us instead of 425.)
 //
 // Bound and measured (us in graph replay; the floor is the larger of the bytes at a large copy's 4.8 TB/s and the
 // operations at a large fp16 product's 1180 TFLOP/s, twice for fp32 rows): one token of 32 / 8 heads of 128 behind
@@ -147,23 +148,17 @@ __device__ __forceinline__ void join_slices(const float* p0, size_t step, int sl
   }
 }
 
-// 8 probabilities as matrix-core operands. fp16 rows: rounded to the nearest (towards zero, one instruction
-// less, leaves the output at 3.3e-4 of float64 instead of 2.7e-4; its own rounding is 2.0e-4). fp32 rows: hi
-// towards zero, and what that leaves. The sum of probabilities is taken of the operands, by the matrix cores.
-template <int P> __device__ __forceinline__ void split_p(const float* p, half8v* ph) {
+// 8 probabilities as matrix-core operands: hi towards zero, and what that leaves. The sum of probabilities is taken
+// of the operands, by the matrix cores.
+__device__ __forceinline__ void split_p(const float* p, half8v* ph) {
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    if constexpr (P == 1) {
-      ph[0][2 * x] = (_Float16)p[2 * x];
-      ph[0][2 * x + 1] = (_Float16)p[2 * x + 1];
-    } else {
-      const half2v hi = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(p[2 * x], p[2 * x + 1]));
-      const half2v lo = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, -1.f, p[2 * x]), fmaf((float)hi.y, -1.f, p[2 * x + 1])));
-      ph[0][2 * x] = hi.x;
-      ph[0][2 * x + 1] = hi.y;
-      ph[1][2 * x] = lo.x;
-      ph[1][2 * x + 1] = lo.y;
-    }
+    const half2v hi = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(p[2 * x], p[2 * x + 1]));
+    const half2v lo = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, -1.f, p[2 * x]), fmaf((float)hi.y, -1.f, p[2 * x + 1])));
+    ph[0][2 * x] = hi.x;
+    ph[0][2 * x + 1] = hi.y;
+    ph[1][2 * x] = lo.x;
+    ph[1][2 * x + 1] = lo.y;
   }
 }
 __device__ __forceinline__ half8v ones() { return (half8v){1, 1, 1, 1, 1, 1, 1, 1}; }
@@ -291,13 +286,13 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
     }
-    half8v ph[P];
+    half8v ph[2];
     float p8[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], back, neg));
-    split_p<P>(p8, ph);
+    split_p(p8, ph);
 #pragma unroll
-    for (int p = P - 1; p >= 0; --p) l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones(), ph[p], l, 0, 0, 0);
+    for (int p = 1; p >= 0; --p) l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones(), ph[p], l, 0, 0, 0);
 
     // ---- values ----
     // keys behind the last one hold anything: their S and Z are cleared. A group with a NaN or an
@@ -327,7 +322,7 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
     for (int i = 0; i < NT; ++i) {
       const half8v v = unpack_value(vw[i], vs[i >> 1], vz[i >> 1]);
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[p], o[i], 0, 0, 0);
+      for (int p = 1; p >= 0; --p) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[p], o[i], 0, 0, 0);
     }
     if (bad)
 #pragma unroll
@@ -407,9 +402,10 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
 // operands in LDS, in operand order: each write and read is 16 consecutive bytes a lane. Two buffers, one
 // barrier a step: while a step's products run, the next step's words, loaded a step before that, are unpacked.
 constexpr int kA4TileWaves = 4;
-// blocks of a step and 16-row tiles of a wave: what the registers hold (fp32 rows take twice the operands)
+// blocks of a step and 16-row tiles of a wave: what the registers hold (fp32 rows take twice the operands of q; 3000
+// fp16 rows of 14 / 2 heads of 64: 56 us at one tile a wave, 75 at two, which leave a SIMD two waves)
 __host__ __device__ constexpr int kv4_step_blocks(int HD, bool f32) { return HD == 64 ? 2 : HD == 128 && !f32 ? 2 : 1; }
-__host__ __device__ constexpr int kv4_tile_qt(int HD, bool f32) { return HD <= 128 && !f32 ? 2 : 1; }
+__host__ __device__ constexpr int kv4_tile_qt(int HD, bool f32) { return HD == 128 && !f32 ? 2 : 1; }
 __host__ __device__ constexpr int kv4_tile_rows(int HD, bool f32) { return kA4TileWaves * 16 * kv4_tile_qt(HD, f32); }
 
 // Slices of `steps` key steps, of `per` steps each
@@ -624,7 +620,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
   for (int step = s0; step < s1; ++step) {
     check_v(step + 1);
     const half8v* vf = ops + (size_t)(2 + (step & 1)) * NBK * NT * 64 + lane;
-    half8v ph[QT][NBK][P];
+    half8v ph[QT][NBK][2];
 #pragma unroll
     for (int i = 0; i < QT; ++i)
 #pragma unroll
@@ -632,7 +628,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[i][2 * b + (e >> 2)][e & 3], back[i], neg[i]));
-        split_p<P>(p, ph[i][b]);
+        split_p(p, ph[i][b]);
       }
     scores(step + 1);
     stage_k(step + 2);
@@ -642,7 +638,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
 #pragma unroll
     for (int b = 0; b < NBK; ++b)
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p)
+      for (int p = 1; p >= 0; --p)
 #pragma unroll
         for (int i = 0; i < QT; ++i) l[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones(), ph[i][b][p], l[i], 0, 0, 0);
 #pragma unroll
@@ -651,7 +647,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
       for (int b = 0; b < NBK; ++b) {
         const half8v v = vf[(b * NT + n) * 64];
 #pragma unroll
-        for (int p = P - 1; p >= 0; --p)
+        for (int p = 1; p >= 0; --p)
 #pragma unroll
           for (int i = 0; i < QT; ++i) o[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[i][b][p], o[i][n], 0, 0, 0);
       }
