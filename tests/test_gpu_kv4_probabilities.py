@@ -1,4 +1,5 @@
-"""GPU: the bits that the probabilities of attention over the 4-bit cache carry."""
+"""GPU: the probabilities of attention over the 4-bit cache. Small ones count too: a first key that takes most of the
+softmax and has a small value (an attention sink) leaves the output to many small probabilities."""
 import math
 
 import pytest
@@ -6,6 +7,30 @@ import pytest
 from test_gpu_kv4 import fill, state
 
 pytestmark = pytest.mark.gpu
+
+# A probability is held as two fp16 numbers of 2^11 p, to 2^-25 at the least: of 16000 keys that share 1 % it is 2^11 x 6e-7
+# = 2^-9.6, so 2^-15 of each, at random, 2^-22 of their sum. The scores are exact where they are large (the sink's), and
+# fp32 sums of 500 steps stay within 500 x 2^-24 / 6.
+SINK_REL = 5e-6
+
+
+def sink(n, nkv, HD, share, g):
+    """Keys and values (n, nkv, HD): position 0 takes `share` of every query that `queries` makes."""
+    import torch
+    k, v = torch.randn((n, nkv, HD), generator=g), 1 + torch.randn((n, nkv, HD), generator=g)
+    k[:, :, :32] = 0
+    # e^score of the others sums to n e^(1/2 (HD - 32) / HD): the queries' scores are N(0, (HD - 32) / HD)
+    k[0] = 0
+    k[0, :, :32] = (math.log(n) + 0.5 * (HD - 32) / HD + math.log(share / (1 - share))) * math.sqrt(HD) / 32
+    v[0] *= 0.01
+    return k, v
+
+
+def queries(T, NH, HD, g):
+    import torch
+    q = torch.randn((T, NH, HD), generator=g)
+    q[:, :, :32] = 1
+    return q
 
 
 def last_rows(q, cache, pos, rows):
@@ -22,6 +47,23 @@ def last_rows(q, cache, pos, rows):
         s[later] = -math.inf
         out[:, h] = torch.mm(torch.softmax(s, 1), v[h // (NH // k.shape[0])])
     return out
+
+
+@pytest.mark.parametrize("share", [0.9, 0.99, 0.999])
+@pytest.mark.parametrize("T,n,NH,NKV,HD", [(1, 16000, 4, 2, 64), (30, 16000, 2, 1, 64), (4096, 6000, 8, 8, 64), (4096, 16000, 8, 8, 64),
+                                           (2048, 16000, 16, 16, 128), (100, 100000, 4, 4, 64)])
+def test_sink_keys(gpu, T, n, NH, NKV, HD, share):
+    import torch
+    from webpytorch_amd import core
+    g = torch.Generator().manual_seed(n)
+    k, v = sink(n, NKV, HD, share, g)
+    q = queries(T, NH, HD, g).cuda()
+    cache = fill(k, v)
+    rows = min(T, 16)
+    got = core.attention_kv4(q, cache, state(torch, n - T))[-rows:].double()
+    want = last_rows(q, cache, n - T, rows)
+    err = float((got - want).norm() / want.norm())
+    assert err <= SINK_REL, err
 
 
 @pytest.mark.parametrize("NH,NKV,HD", [(4, 2, 64), (4, 1, 128), (2, 1, 192), (2, 1, 256)])

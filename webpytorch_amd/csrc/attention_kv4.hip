@@ -7,7 +7,7 @@
 // words of the cache are unpacked in registers, in operand order (kv4.h), and no value moves between lanes
 // from the scores to the output. K and V are exact fp16; p is two fp16 numbers (hi + lo: 22 bits), and so is q of
 // fp32 rows (scaled by a power of two per row); q of fp16 rows is exact. Sums and softmax statistics are fp32. p is held
-// times 2^7 or more, so that its lower part stays in fp16's normal range. (p of fp16 rows as one number cost the output as
+// times 2^11 or more, so that its lower part stays in fp16's normal range. (p of fp16 rows as one number cost the output as
 // much again as its own rounding, 2.7e-4 of float64 instead of 2.0e-4, and saved a third of the matrix instructions:
 // 6001 rows of 28 / 4 heads of 128 326 us instead of 425.)
 //
@@ -26,10 +26,12 @@ namespace miq {
 
 constexpr int kA4Waves = 8;
 constexpr int kA4Rows = 16;
-// The reference of the exponentials is raised only when a score passes it by more than 2^8 (a probability, 2^7 at the
+// The reference of the exponentials is raised only when a score passes it by more than 2^4 (a probability, 2^11 at the
 // reference, then stays below 2^15), so that the output is seldom rescaled (131000 positions 50 -> 47 us a replay); each
-// row by its own scores alone, so that a token's bits do not depend on its neighbours' queries.
-constexpr float kA4UnitLog2 = 7.f, kA4Slack = 8.f;
+// row by its own scores alone, so that a token's bits do not depend on its neighbours' queries. The unit is as high as
+// that and fp16's range allow: two fp16 numbers hold it to 2^-25, so that of 100000 keys that share 0.1 % beside one the sum
+// is right to 4e-7 (5e-6 at 2^7; a slack of 2^8 takes the same time).
+constexpr float kA4UnitLog2 = 11.f, kA4Slack = 4.f;
 constexpr int kA4CtrStride = 32;    // ints between arrival counters: a 128-byte line each
 constexpr int kA4MaxSlices = 64;
 constexpr int kA4MinSteps = 8;      // key steps of a slice of many rows, at least
@@ -148,17 +150,17 @@ __device__ __forceinline__ void join_slices(const float* p0, size_t step, int sl
   }
 }
 
-// 8 probabilities as matrix-core operands: hi towards zero, and what that leaves. The sum of probabilities is taken
-// of the operands, by the matrix cores.
+// 8 probabilities as matrix-core operands: the nearest fp16 number, and the one nearest to what that leaves (to 2^-25 at
+// the least). Both to the nearest: towards zero, all small probabilities shrink alike beside a large one (of 16000 keys that
+// share 1 % by a part in 6000). The sum of probabilities is taken of the operands, by the matrix cores.
 __device__ __forceinline__ void split_p(const float* p, half8v* ph) {
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    const half2v hi = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(p[2 * x], p[2 * x + 1]));
-    const half2v lo = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, -1.f, p[2 * x]), fmaf((float)hi.y, -1.f, p[2 * x + 1])));
+    const half2v hi = {(_Float16)p[2 * x], (_Float16)p[2 * x + 1]};
     ph[0][2 * x] = hi.x;
     ph[0][2 * x + 1] = hi.y;
-    ph[1][2 * x] = lo.x;
-    ph[1][2 * x + 1] = lo.y;
+    ph[1][2 * x] = (_Float16)fmaf((float)hi.x, -1.f, p[2 * x]);
+    ph[1][2 * x + 1] = (_Float16)fmaf((float)hi.y, -1.f, p[2 * x + 1]);
   }
 }
 __device__ __forceinline__ half8v ones() { return (half8v){1, 1, 1, 1, 1, 1, 1, 1}; }
