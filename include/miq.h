@@ -413,7 +413,8 @@ int miq_kv4_dequant_f32(const void* cache, float* k_out, float* v_out, int NKV, 
 /* miq_attention over a 4-bit cache: q and out [T][NH][HD] fp32 or fp16 (x_dtype); token t of head h
  * attends to positions 0 .. min(state[0] + t, LMAX - 1) of kv head h / (NH / NKV); a token whose
  * position is below 0 attends to nothing and gets zeros. The probabilities, and q of fp32 rows, enter the
- * fp16 matrix cores as two numbers each (22 bits). A value that reads as NaN reaches
+ * fp16 matrix cores as two numbers each (22 bits). Scores may be as large as fp32 holds (past it, and where all
+ * of a token's scores are -inf, its output is NaN). A value that reads as NaN reaches
  * exactly the tokens that attend to it, and what positions behind the last one hold does not matter.
  * out must not overlap q. workspace: as miq_gptq_gemv's (counters zero before the first call and left zero; not shared by calls
  * that run concurrently; null where miq_attention_kv4_workspace says 0). Results do not depend on the order of

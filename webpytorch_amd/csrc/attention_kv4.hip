@@ -49,6 +49,32 @@ __device__ __forceinline__ int row_shift(float mx) {
   return (e == 0 || e == 255) ? 0 : 13 + 127 - e;
 }
 
+// A row's reference: a score s (the matrix cores' sum) has the probability 2^((s - shift) back + neg), a fused product
+// and sum. Scores below kA4Far units of log 2 have shift 0 and a whole reference, neg = kA4UnitLog2 - rint(the highest),
+// which is exact, so that rescaling is by powers of two. Past it no fp32 number lies near enough to all scores: the
+// highest is taken off in the matrix cores' units first, where it leaves an exact 0 for its own key. (A reference
+// rounded in units of log 2 is off by its last place, 2^7 at 2^30, and takes the exponentials of every key to 0 or
+// to infinity.)
+constexpr float kA4Far = 4194304.f, kA4NoKey = 3.402823466e38f;  // 2^22; neg of a row that has met no key
+struct Ref {
+  float shift, neg;
+};
+// the exponent that the row's highest score (-inf: none) has now
+__device__ __forceinline__ float ref_exponent(const Ref& r, float mx, float back) { return fmaf(mx - r.shift, back, r.neg); }
+// Takes mx as the reference where the exponent is past the slack; returns what the row's sums are rescaled by.
+__device__ __forceinline__ float ref_raise(Ref& r, float mx, float back) {
+  if (!(ref_exponent(r, mx, back) > kA4UnitLog2 + kA4Slack)) return 1.f;
+  const float top = mx * back;  // past fp32's range: NaN, as the difference of two such scores is
+  const Ref n = fabsf(top) < kA4Far ? Ref{0.f, kA4UnitLog2 - rintf(top)} : Ref{mx, kA4UnitLog2 + (top - top)};
+  const float f = __builtin_amdgcn_exp2f(fmaf(r.shift - n.shift, back, n.neg - r.neg));
+  r = n;
+  return f;
+}
+// the reference in units of log 2, -inf for none
+__device__ __forceinline__ float ref_log2(const Ref& r, float back) {
+  return r.neg == kA4NoKey ? -INFINITY : fmaf(r.shift, back, kA4UnitLog2 - r.neg);
+}
+
 // the 8 numbers S (1 + c / 16) + Z of a key word: one S and Z
 __device__ __forceinline__ half8v unpack_key(uint32_t w, uint32_t meta) {
   const half2v m = as_h2(meta), S = (half2v){m.x, m.x}, Z = (half2v){m.y, m.y};
@@ -111,7 +137,8 @@ __device__ __forceinline__ bool last_slice(int* ctr, int slices, int* last) {
 // out rows r0 .. r0 + nr - 1 from the slices' parts ([row][HD + 4]: the output, the maximum and the sum), in
 // slice order
 template <int HD, typename XT, int THREADS>
-__device__ __forceinline__ void join_slices(const float* p0, size_t step, int slices, XT* out, int r0, int nr, int rep, int kv, int NH) {
+__device__ __forceinline__ void join_slices(const float* p0, size_t step, int slices, XT* out, int64_t pos0, int r0, int nr, int rep, int kv,
+                                            int NH) {
   for (int x = threadIdx.x; x < nr * (HD / 2); x += THREADS) {
     const int row = x / (HD / 2), d = 2 * (x % (HD / 2));
     const float* pr = p0 + (size_t)row * (HD + 4);
@@ -145,8 +172,9 @@ __device__ __forceinline__ void join_slices(const float* p0, size_t step, int sl
     }
     const int rr = r0 + row;
     XT* orow = out + ((size_t)(rr / rep) * NH + kv * rep + rr % rep) * HD + d;
-    orow[0] = from_f32<XT>(sum == 0.f ? 0.f : a[0] / sum);
-    orow[1] = from_f32<XT>(sum == 0.f ? 0.f : a[1] / sum);
+    const bool none = pos0 + rr / rep < 0;  // a row without keys: zeros
+    orow[0] = from_f32<XT>(none ? 0.f : a[0] / sum);
+    orow[1] = from_f32<XT>(none ? 0.f : a[1] / sum);
   }
 }
 
@@ -248,7 +276,8 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
 
   float4v o[NT];
   float4v l = (float4v){0.f, 0.f, 0.f, 0.f};  // the sum of probabilities, in every row of the product
-  float m = -INFINITY, neg = kA4UnitLog2;  // the reference, and what is added to a score for the exponent
+  Ref ref = {0.f, kA4NoKey};
+  bool far = false;  // wave-uniform: a row of the wave has a shift
 #pragma unroll
   for (int i = 0; i < NT; ++i) o[i] = (float4v){0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](Raw& w, int blk) __attribute__((always_inline)) {
@@ -278,20 +307,21 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
         if (masked && blk * kKv4Block + 16 * b + 4 * g + x > lim) s[b][x] = -INFINITY;
         mx = fmaxf(mx, s[b][x]);
       }
-    mx = rows_max(mx) * back;
-    if (__ballot(mx > m + kA4Slack)) {
-      const float mn = mx > m + kA4Slack ? mx : m;
-      const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      neg = kA4UnitLog2 - (mn == -INFINITY ? 0.f : mn);  // no key yet: every probability is 0
+    mx = rows_max(mx);
+    if (__ballot(ref_exponent(ref, mx, back) > kA4UnitLog2 + kA4Slack)) {
+      const float alpha = ref_raise(ref, mx, back);
+      far = __ballot(ref.shift != 0.f) != 0ull;
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
     }
+    if (far)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) s[b] -= ref.shift;
     half8v ph[2];
     float p8[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], back, neg));
+    for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], back, ref.neg));
     split_p(p8, ph);
 #pragma unroll
     for (int p = 1; p >= 0; --p) l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones(), ph[p], l, 0, 0, 0);
@@ -357,7 +387,7 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
   const int nr = min(QR, R - r0);
   if (wave < nw) {
     if (g == 0) {
-      ms[wave][c] = m;
+      ms[wave][c] = ref_log2(ref, back);
       ls[wave][c] = l[0];
     }
     if (c < nr)
@@ -390,13 +420,13 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
     const int rr = r0 + row;
     XT* orow = out + ((size_t)(rr / rep) * NH + kv * rep + rr % rep) * HD + d;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) orow[e] = from_f32<XT>(sum == 0.f ? 0.f : a[e] / sum);  // a row without keys: zeros
+    for (int e = 0; e < 4; ++e) orow[e] = from_f32<XT>(pos0 + rr / rep < 0 ? 0.f : a[e] / sum);  // a row without keys: zeros
   }
   if (slices == 1) return;
 
   if (!last_slice(counters + (kv * gridDim.y + tile) * kA4CtrStride, slices, &last)) return;
   join_slices<HD, XT, 64 * NW>(parts + (size_t)(kv * gridDim.y + tile) * gridDim.x * QR * (HD + 4), (size_t)QR * (HD + 4), slices,
-                               out, r0, nr, rep, kv, NH);
+                               out, pos0, r0, nr, rep, kv, NH);
 }
 
 // Many rows: a workgroup takes 4 x 16 QT of them, every wave its own, and all their keys (or a slice of
@@ -528,11 +558,11 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
 
   float4v o[QT][NT], s[QT][2 * NBK];
   float4v l[QT];  // the sum of probabilities, in every row of the product
-  float m[QT], neg[QT];  // the reference, and what is added to a score for the exponent
+  Ref ref[QT];
+  bool far = false;  // wave-uniform: a row of the wave has a shift
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    m[i] = -INFINITY;
-    neg[i] = kA4UnitLog2;
+    ref[i] = {0.f, kA4NoKey};
     l[i] = (float4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[i][n] = (float4v){0.f, 0.f, 0.f, 0.f};
@@ -553,7 +583,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
       }
     }
   };
-  // masks the scores of `step` and raises the references they need
+  // masks the scores of `step`, raises the references they need and takes the shifts off
   auto refer = [&](int step) __attribute__((always_inline)) {
     const int k0 = step * NBK * kKv4Block;
     if (k0 + NBK * kKv4Block - 1 > first) {  // wave-uniform
@@ -574,21 +604,26 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
       for (int b = 0; b < 2 * NBK; ++b)
 #pragma unroll
         for (int x = 0; x < 4; ++x) mx[i] = fmaxf(mx[i], s[i][b][x]);
-      mx[i] = rows_max(mx[i]) * back[i];
-      raise |= mx[i] > m[i] + kA4Slack;  // m = -inf: any score
+      mx[i] = rows_max(mx[i]);
+      raise |= ref_exponent(ref[i], mx[i], back[i]) > kA4UnitLog2 + kA4Slack;
     }
     if (__ballot(raise)) {
+      bool shifted = false;
 #pragma unroll
       for (int i = 0; i < QT; ++i) {
-        const float mn = mx[i] > m[i] + kA4Slack ? mx[i] : m[i];
-        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i] - mn);
-        m[i] = mn;
-        neg[i] = kA4UnitLog2 - (mn == -INFINITY ? 0.f : mn);  // no key yet: every probability is 0
+        const float alpha = ref_raise(ref[i], mx[i], back[i]);
+        shifted |= ref[i].shift != 0.f;
         l[i] *= alpha;
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[i][n] *= alpha;
       }
+      far = __ballot(shifted) != 0ull;
     }
+    if (far)
+#pragma unroll
+      for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int b = 0; b < 2 * NBK; ++b) s[i][b] -= ref[i].shift;
   };
 
   // K runs a step ahead of V: in step t the waves multiply K(t + 1) and V(t), unpack K(t + 2) and V(t + 1), and
@@ -629,7 +664,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
       for (int b = 0; b < NBK; ++b) {
         float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[i][2 * b + (e >> 2)][e & 3], back[i], neg[i]));
+        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[i][2 * b + (e >> 2)][e & 3], back[i], ref[i].neg));
         split_p(p, ph[i][b]);
       }
     scores(step + 1);
@@ -679,7 +714,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
       float4v* part = parts + (((size_t)(kv * gridDim.y + tile) * (QR / 16) + wave * QT + i) * gridDim.z + slice) * kv4_part_unit(HD);
 #pragma unroll
       for (int n = 0; n < NT; ++n) part[n * 64 + lane] = o[i][n];
-      if (g == 0) reinterpret_cast<float2*>(part + NT * 64)[c] = make_float2(m[i], sum);
+      if (g == 0) reinterpret_cast<float2*>(part + NT * 64)[c] = make_float2(ref_log2(ref[i], back[i]), sum);
       continue;
     }
     if (r >= R) continue;
@@ -687,7 +722,7 @@ __global__ __launch_bounds__(64 * kA4TileWaves, HD <= 128 && sizeof(XT) == 4 ? 3
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) orow[16 * n + e] = from_f32<XT>(sum == 0.f ? 0.f : o[i][n][e] / sum);  // a row without keys: zeros
+      for (int e = 0; e < 4; ++e) orow[16 * n + e] = from_f32<XT>(lim[i] < 0 ? 0.f : o[i][n][e] / sum);  // a row without keys: zeros
   }
 }
 
@@ -744,7 +779,7 @@ __global__ __launch_bounds__(256) void attention_kv4_join_kernel(const int32_t* 
 #pragma unroll
   for (int n = 0; n < NW; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) orow[16 * (wave * NW + n) + e] = from_f32<XT>(sum == 0.f ? 0.f : a[n][e] / sum);
+    for (int e = 0; e < 4; ++e) orow[16 * (wave * NW + n) + e] = from_f32<XT>(pos0 + r / rep < 0 ? 0.f : a[n][e] / sum);
 }
 
 // Up to kA4FewRows rows of a kv head go by the rows kernel, and up to kA4SomeRows where the cache is short: it unpacks
