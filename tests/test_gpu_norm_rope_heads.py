@@ -64,3 +64,26 @@ def test_kv4_write_matches_float64(gpu, NH, NKV, HD, norm, more, dt):
             assert np.array_equal(now[part][i][:, at], want[i], equal_nan=i > 0)
             view = (lambda t: t) if i == 0 else (lambda t: np.ascontiguousarray(t).view(np.uint16))
             assert np.array_equal(view(now[part][i])[:, rest], view(was[part][i])[:, rest])
+
+
+@pytest.mark.parametrize("HD,T", [(64, 2000), (128, 1000), (192, 30), (256, 700)])
+def test_fp16_queries_are_rounded_once(gpu, HD, T):
+    """Without a norm a query is two fp64 products and their sum: the fp16 number next to it, not that of its fp32
+    number (a value in 2^13 or so lies between the two roundings)."""
+    import torch
+    from webpytorch_amd import core
+    g = torch.Generator().manual_seed(HD)
+    NH, lmax = 8, (T + 31) // 32 * 32
+    qkv = torch.randn((T, (NH + 2) * HD), generator=g).half()
+    cache = core.kv4_cache(1, lmax, HD)
+    cos, sin = tables(torch, lmax, HD)
+    q = core.qk_norm_rope(qkv.cuda(), state(torch, 0), cos, sin, NH, cache)
+    x = qkv.numpy().reshape(T, -1, HD)[:, :NH].astype(np.longdouble)
+    c, s = (t[:T].cpu().numpy().astype(np.longdouble)[:, None] for t in (cos, sin))
+    h = HD // 2  # 11 x 24 bits a product: 64 bits hold the sum but for cancellation's last ones
+    want = np.concatenate([x[..., :h] * c - x[..., h:] * s, x[..., h:] * c + x[..., :h] * s], -1)
+    lo, hi = (np.nextafter(want.astype(np.float16), np.float16(d)).astype(np.longdouble) for d in (-np.inf, np.inf))
+    got = q.cpu().numpy().astype(np.longdouble)
+    # the nearest: no neighbour is nearer by more than fp64's own rounding of the sum
+    err, slack = np.abs(got - want), np.abs(want) * 2.0 ** -50 + 2.0 ** -60
+    assert (err <= np.minimum(np.abs(lo - want), np.abs(hi - want)) + slack).all()

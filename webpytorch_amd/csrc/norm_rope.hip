@@ -42,6 +42,17 @@ __device__ __forceinline__ double wave_sum_d(double v) {
   return (lane_at_d(v, 0) + lane_at_d(v, 16)) + (lane_at_d(v, 32) + lane_at_d(v, 48));
 }
 
+// An fp64 number rounded once to a query's type. fp16: by way of the fp32 number next to it towards zero with its last bit
+// set where something is left ("to odd"), so that it is on the same side of every border of fp16 as v is.
+template <typename T> __device__ __forceinline__ T from_f64(double v);
+template <> __device__ __forceinline__ float from_f64<float>(double v) { return (float)v; }
+template <> __device__ __forceinline__ __half from_f64<__half>(double v) {
+  const float f = (float)v;
+  uint32_t b = __float_as_uint(f) - (fabs((double)f) > fabs(v) ? 1u : 0u);
+  if ((double)f != v) b |= 1u;
+  return __float2half_rn(__uint_as_float(b));
+}
+
 // The rotation partners, HD / 2 dimensions further, of v[i] = dimension lane + 64 i.
 template <int HD> __device__ __forceinline__ void partners(const float* v, float* o) {
   if constexpr (HD == 128) {
@@ -195,7 +206,7 @@ __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv4_kernel(
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = v[i] * inv * (double)(h < NH ? w[0][i] : w[1][i]);
       }
-      float y[N];
+      double y[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         double o;  // the rotation partner
@@ -209,11 +220,11 @@ __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv4_kernel(
           o = k == 0 ? got[0] : k == 1 ? got[1] : got[2];
         }
         const double os = lane + 64 * i < HALF ? -o : o;
-        y[i] = (float)fma(os, (double)sn[i], v[i] * (double)cs[i]);
+        y[i] = fma(os, (double)sn[i], v[i] * (double)cs[i]);
       }
       if (h < NH) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) q_out[((size_t)t * NH + h) * HD + lane + 64 * i] = from_f32<XT>(y[i]);
+        for (int i = 0; i < N; ++i) q_out[((size_t)t * NH + h) * HD + lane + 64 * i] = from_f64<XT>(y[i]);
         continue;
       }
       const int key = (int)(pos % kKv4Block);
@@ -221,7 +232,7 @@ __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv4_kernel(
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         uint16_t S, Z;
-        uint32_t c = kv4_quantize(y[i], S, Z) << kv4_shift(lane & 7);
+        uint32_t c = kv4_quantize((float)y[i], S, Z) << kv4_shift(lane & 7);
         c |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0xB1, 0xF, 0xF, false);
         c |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0x4E, 0xF, 0xF, false);
         c |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0x141, 0xF, 0xF, false);
