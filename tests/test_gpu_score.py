@@ -1,0 +1,35 @@
+"""GPU: what `score` leaves behind."""
+import pytest
+
+from webpytorch_amd import synth
+
+pytestmark = pytest.mark.gpu
+
+SMALL = dict(L=1, H=256, NH=4, NKV=2, HD=64, I=512, V=2048, gs=128, bits=4)
+
+
+def model(w, lmax, **kw):
+    from webpytorch_amd import llm
+    return llm.CausalLM.from_weights(w, lmax=lmax, **kw)
+
+
+@pytest.mark.parametrize("kv_bits", [None, 4])
+def test_score_leaves_the_sequence_reset(gpu, kv_bits, monkeypatch):
+    """After a text of several pieces, and after an error between two of them."""
+    from webpytorch_amd import core, llm
+    monkeypatch.setattr(llm.CausalLM, "PREFILL_ROWS", 16)
+    ids = [int(i) for i in synth.prompt_ids(41, 40, SMALL["V"])]
+    m = model(synth.decoder_weights(41, **SMALL), 64, kv_bits=kv_bits)
+    m.score(ids)
+    assert not m.state.any()
+    calls, run = [], core.token_logprobs
+
+    def second_fails(*a):
+        calls.append(0)
+        if len(calls) == 2:
+            raise RuntimeError("planted")
+        return run(*a)
+    monkeypatch.setattr(core, "token_logprobs", second_fails)
+    with pytest.raises(RuntimeError, match="planted"):
+        m.score(ids)
+    assert not m.state.any()

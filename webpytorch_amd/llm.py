@@ -705,17 +705,20 @@ class CausalLM:
         given = core.to_device(np.asarray(ids[1:], dtype=np.int32))
         parts, rows, piece = [], self.SCORE_ROWS, int(self.ids.shape[0])
         logits = torch.empty((min(n, rows), self.V), dtype=torch.float32, device=core.device())
-        for p0 in range(0, n, piece):
-            p1 = min(n, p0 + piece)
-            self._place(ids[p0:p1], p0)
-            self._layers(p1 - p0)
-            for t0 in range(p0, p1, rows):
-                m = min(rows, p1 - t0)
-                h = self.buf["h"][t0 - p0:t0 - p0 + m]
-                _lib.call("miq_rmsnorm", ptr(h), ptr(self.final_norm), ptr(self.buf["xn"]), m, self.H, self.eps,
-                          stream_handle())
-                self._linear(self.head, self.buf["xn"][:m], logits[:m])
-                parts.append(core.token_logprobs(logits[:m], given[t0:t0 + m], top_k))
+        try:
+            for p0 in range(0, n, piece):
+                p1 = min(n, p0 + piece)
+                self._place(ids[p0:p1], p0)
+                self._layers(p1 - p0)
+                for t0 in range(p0, p1, rows):
+                    m = min(rows, p1 - t0)
+                    h = self.buf["h"][t0 - p0:t0 - p0 + m]
+                    _lib.call("miq_rmsnorm", ptr(h), ptr(self.final_norm), ptr(self.buf["xn"]), m, self.H, self.eps,
+                              stream_handle())
+                    self._linear(self.head, self.buf["xn"][:m], logits[:m])
+                    parts.append(core.token_logprobs(logits[:m], given[t0:t0 + m], top_k))
+        finally:
+            self.reset()  # pieces behind the first have moved the position
         return parts[0] if len(parts) == 1 else core.TokenLogprobs(*(torch.cat(p) for p in zip(*parts)))
 
     def generate(self, ids, max_new, use_graph=True, logprobs=None):
