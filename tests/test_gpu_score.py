@@ -33,3 +33,14 @@ def test_score_leaves_the_sequence_reset(gpu, kv_bits, monkeypatch):
     with pytest.raises(RuntimeError, match="planted"):
         m.score(ids)
     assert not m.state.any()
+
+
+def test_score_keeps_no_buffers_of_alternatives(gpu):
+    """The rows that `generate(logprobs=k)` keeps for its graphs are not made for `score`, whose results are its own."""
+    ids = [int(i) for i in synth.prompt_ids(42, 20, SMALL["V"])]
+    m = model(synth.decoder_weights(42, **SMALL), 64)
+    assert m.score(ids, 7).top_ids.shape == (19, 7)
+    for bad in (33, -1):
+        with pytest.raises(ValueError, match="alternatives"):
+            m.score(ids, bad)
+    assert not m._lp_rows

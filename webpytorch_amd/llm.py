@@ -682,11 +682,14 @@ class CausalLM:
             self.pws = pws
         return left
 
+    def _check_alternatives(self, name, k):
+        if not 0 <= k <= min(self.V, core.MAX_TOP_LOGPROBS):
+            raise ValueError("%s=%d (0 .. %d alternatives)" % (name, k, min(self.V, core.MAX_TOP_LOGPROBS)))
+
     def _logprob_rows(self, k):
         """The buffers that steps with k alternatives write, a row per generated token: kept for the captured
         graphs that hold their addresses."""
-        if not 0 <= k <= min(self.V, core.MAX_TOP_LOGPROBS):
-            raise ValueError("logprobs=%d (0 .. %d alternatives)" % (k, min(self.V, core.MAX_TOP_LOGPROBS)))
+        self._check_alternatives("logprobs", k)
         if k not in self._lp_rows:
             n, dev = self.lmax, core.device()
             self._lp_rows[k] = core.TokenLogprobs(*(torch.zeros(s, dtype=d, device=dev) for s, d in (
@@ -700,7 +703,7 @@ class CausalLM:
         n = len(ids) - 1
         if n < 1 or len(ids) > self.lmax:
             raise ValueError("score takes 2 .. lmax (%d) tokens, got %d" % (self.lmax, len(ids)))
-        self._logprob_rows(top_k)
+        self._check_alternatives("top_k", top_k)
         self.reset()
         given = core.to_device(np.asarray(ids[1:], dtype=np.int32))
         parts, rows, piece = [], self.SCORE_ROWS, int(self.ids.shape[0])
