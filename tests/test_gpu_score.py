@@ -1,4 +1,4 @@
-"""GPU: what `score` leaves behind."""
+"""GPU: what `score` leaves behind, and the workspace of prompts through layers off the matrix cores."""
 import pytest
 
 from webpytorch_amd import synth
@@ -44,3 +44,21 @@ def test_score_keeps_no_buffers_of_alternatives(gpu):
         with pytest.raises(ValueError, match="alternatives"):
             m.score(ids, bad)
     assert not m._lp_rows
+
+
+def test_layers_off_the_matrix_cores_have_their_workspace_from_the_start(gpu):
+    """A zero offset that is no whole number keeps a prompt's products on the GEMV, whose sums of many rows are more
+    than the matrix-core product takes: all allocated with the engine, none during a prompt."""
+    from webpytorch_amd import core
+    sh = dict(SMALL, H=1024, NH=16, I=9728)
+    w = synth.decoder_weights(43, **sh)
+    for lay in w["layers"]:
+        for name in ("q", "k", "v", "o", "gate", "up", "down"):
+            lay[name]["zoff"] = 0.5
+    m = model(w, 520, persistent=False)
+    ids = [int(i) for i in synth.prompt_ids(43, 500, sh["V"])]
+    m.generate(ids[:20], 2)  # the first-use checks have the stream's workspace
+    before = {k: t.numel() for k, t in core._WORKSPACE.items()}
+    for n in (100, 333, 500):
+        m.generate(ids[:n], 2)
+    assert {k: t.numel() for k, t in core._WORKSPACE.items()} == before

@@ -261,6 +261,12 @@ def gptq_dequant(qweight, qzeros, scales, K, N, gs, bits, zoff=0.0, g_idx=None):
     return out
 
 
+def f32_rows_on_matrix_cores(K, zoff):
+    """Whether more than GEMV_MAX_M fp32 rows run the matrix-core GEMM: the zero points are whole numbers in its
+    operands, and K fits its rows. The GEMV takes the others."""
+    return float(zoff).is_integer() and 0 <= zoff <= 8 and K <= 32768
+
+
 def _gptq_matmul(xf, qweight, qzeros, scales, K, N, gs, bits, zoff=0.0, *, bias=None, perm=None,
                  out_dtype=None, out=None, ws=None, _check=True):
     """xf (M, K) @ dequant(W) (+ bias) -> (M, N) on the current stream
@@ -288,7 +294,7 @@ def _gptq_matmul(xf, qweight, qzeros, scales, K, N, gs, bits, zoff=0.0, *, bias=
                   dtype_code(scales), ptr(bias), ptr(out), dtype_code(out), M, K, N, gs, bits,
                   float(zoff), ptr(ws), 0 if ws is None else ws.numel(), stream_handle())
         return out
-    if M > GEMV_MAX_M and float(zoff).is_integer() and 0 <= zoff <= 8 and K <= 32768:
+    if M > GEMV_MAX_M and f32_rows_on_matrix_cores(K, zoff):
         need = gemm_f32x_workspace_bytes(M, K, N, gs, bits)
         if ws is None or ws.numel() < need:
             ws = workspace(need)

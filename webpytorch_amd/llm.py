@@ -337,8 +337,7 @@ class CausalLM:
         self.history = torch.zeros(self.lmax, dtype=torch.int32, device=dev)
         self.state = torch.zeros(_lib.lib().miq_decode_state_words(), dtype=torch.int32, device=dev)
         # one split-K workspace sized for every projection at T = 1 and at the largest prefill
-        # (the need is not monotonic in the row count: wide enough layers stop splitting K; a product that
-        # needs more, as prompts off the matrix cores do, takes the stream's workspace)
+        # (the need is not monotonic in the row count: wide enough layers stop splitting K)
         need = 0
         if isinstance(self.head, _Lin):
             need = core.gemv_workspace_bytes(1, self.head.K, self.head.N, self.gs, self.bits, _lib.MIQ_F32)
@@ -353,10 +352,10 @@ class CausalLM:
         lins = {k: q for k, q in lins.items() if isinstance(q, _Lin)}  # GGUF kernels need no workspace
         for M in range(1, T + 1):  # of the head, a step only sees the last token
             for lin in lins.values():
-                if M <= core.GEMV_MAX_M:
-                    need = max(need, core.gemv_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits, _lib.MIQ_F32))
-                else:  # prefill rows on the matrix cores
+                if M > core.GEMV_MAX_M and core.f32_rows_on_matrix_cores(lin.K, lin.zoff):
                     need = max(need, core.gemm_f32x_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits))
+                else:
+                    need = max(need, core.gemv_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits, _lib.MIQ_F32))
             if self.kv_bits == 4:
                 need = max(need, core.attention_kv4_workspace_bytes(M, self.NH, self.NKV, self.HD, self.lmax))
         for k in range(min(self.V, core.MAX_TOP_LOGPROBS) + 1):  # fewer alternatives may meet from more segments
