@@ -372,8 +372,8 @@ int miq_attention(const float* q, const float* kcache, const float* vcache, cons
 
 /* QK-norm, RoPE and the cache write in one launch: miq_head_rmsnorm (a null weight leaves its part
  * alone) followed by miq_rope_kv, bit for bit, with qkv left as it is. Rows lie ld >= (NH + 2 NKV) HD values
- * apart. A position below 0 or from LMAX on writes nothing to the caches and zeros to its row of q_out, which
- * must not overlap qkv. HD even, <= 256.
+ * apart. A position below 0 or from LMAX on writes nothing to the caches and zeros to its row of q_out. q_out
+ * and the caches must not overlap each other or the rows (refused). HD even, <= 256.
  * Replaces: `self._rms(q, lay["qn"])`, `self._rms(k, lay["kn"])` and `_rope_np` of `CausalLM._qkv`
  * with `kv_write` (webtorch/llm.py:1498-1519, 1259-1304; webtorch/_core.py:1504-1540). */
 int miq_qk_norm_rope_kv(const float* qkv, int64_t ld, const float* qn, const float* kn, float eps,
@@ -416,7 +416,7 @@ int miq_kv4_dequant_f32(const void* cache, float* k_out, float* v_out, int NKV, 
  * fp16 matrix cores as two numbers each (22 bits). Scores may be as large as fp32 holds (past it, and where all
  * of a token's scores are -inf, its output is NaN). A value that reads as NaN reaches
  * exactly the tokens that attend to it, and what positions behind the last one hold does not matter.
- * out must not overlap q. workspace: as miq_gptq_gemv's (counters zero before the first call and left zero; not shared by calls
+ * out must not overlap q or the cache (refused). workspace: as miq_gptq_gemv's (counters zero before the first call and left zero; not shared by calls
  * that run concurrently; null where miq_attention_kv4_workspace says 0). Results do not depend on the order of
  * arrival. LMAX up to 2^30. */
 int miq_attention_kv4_workspace(int T, int NH, int NKV, int HD, int LMAX, size_t* bytes);

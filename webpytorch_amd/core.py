@@ -1016,8 +1016,8 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
         out = torch.empty(T, n_heads, hd, dtype=qkv.dtype, device=dev)
     else:
         _check_tensor("out", out, (qkv.dtype,), None, dev)
-        if out.numel() != T * n_heads * hd or not out.is_contiguous() or out.data_ptr() == qkv.data_ptr() != 0:
-            raise ValueError("out is a contiguous tensor of %d values apart from qkv: got %s" % (T * n_heads * hd, tuple(out.shape)))
+        if out.numel() != T * n_heads * hd or not out.is_contiguous():
+            raise ValueError("out is a contiguous tensor of %d values: got %s" % (T * n_heads * hd, tuple(out.shape)))
     ld = qkv.stride(0) if T > 1 else W
     qp, kp = (None if t is None else t.data_ptr() for t in (qn, kn))
     if four:
@@ -1046,8 +1046,8 @@ def attention_kv4(q, cache, state, scale=None, out=None):
         out = torch.empty_like(q)
     else:
         _check_tensor("out", out, (q.dtype,), None, dev)
-        if out.numel() != q.numel() or not out.is_contiguous() or out.data_ptr() == q.data_ptr() != 0:
-            raise ValueError("out is a contiguous tensor of %d values apart from q: got %s" % (q.numel(), tuple(out.shape)))
+        if out.numel() != q.numel() or not out.is_contiguous():
+            raise ValueError("out is a contiguous tensor of %d values: got %s" % (q.numel(), tuple(out.shape)))
     wp, wn, _keep = _call_workspace(attention_kv4_workspace_bytes(T, nh, nkv, hd, lmax), dev)
     _lib.call("miq_attention_kv4", q.data_ptr(), dtype_code(q), cache.data_ptr(), state.data_ptr(), out.data_ptr(), T, nh, nkv, hd, lmax,
               1.0 / math.sqrt(hd) if scale is None else float(scale), wp, wn, _raw_stream(dev))

@@ -854,6 +854,10 @@ extern "C" int miq_attention_kv4(const void* q, int x_dtype, const void* cache, 
   MIQ_REQUIRE(!part || (workspace && ws_bytes >= kCounterBytes + part), MIQ_ERR_INVALID,
               "attention_kv4: workspace of %zu bytes, %zu needed", workspace ? ws_bytes : (size_t)0, kCounterBytes + part);
   MIQ_REQUIRE(!part || aligned(workspace, 256), MIQ_ERR_ALIGN, "attention_kv4: the workspace must be 256-byte aligned");
+  const size_t io = (size_t)T * NH * HD * (f32 ? 4 : 2);  // one tile's rows are written while another's are read
+  MIQ_REQUIRE(!share_bytes(out, io, q, io), MIQ_ERR_INVALID, "attention_kv4: out must lie apart from q");
+  MIQ_REQUIRE(!share_bytes(out, io, cache, (size_t)NKV * kv4_blocks(LMAX) * kv4_record(HD)), MIQ_ERR_INVALID,
+              "attention_kv4: out must lie apart from the cache");
   int* counters = static_cast<int*>(workspace);
   float* parts = part ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes) : nullptr;
   const size_t lds = p.few ? (size_t)kA4Waves * kA4Rows * (HD + 4) * 4

@@ -30,6 +30,12 @@ __host__ __device__ constexpr int kv4_shift(int e) { return 4 * (e >> 1) + 16 * 
 // position within its block of key e of lane group g
 __host__ __device__ constexpr int kv4_key(int g, int e) { return 16 * (e >> 2) + 4 * g + (e & 3); }
 
+// whether two ranges of bytes share any
+inline bool share_bytes(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + nb && y < x + na;
+}
+
 inline bool kv4_head(int HD) { return HD == 64 || HD == 128 || HD == 192 || HD == 256; }
 
 // The fp16 numbers 1 + c / 16 of code pair p of a word.

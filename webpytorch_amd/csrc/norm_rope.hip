@@ -335,6 +335,25 @@ static int check_norm_rope(const char* what, const void* qkv, int64_t ld, const 
   return MIQ_OK;
 }
 
+// Whether a range of n bytes at o meets any of T rows of w bytes that lie ld bytes apart from x on.
+static bool meets_rows(const void* o, size_t n, const void* x, int T, size_t w, size_t ld) {
+  if (!share_bytes(o, n, x, (size_t)(T - 1) * ld + w)) return false;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(o), b = reinterpret_cast<uintptr_t>(x);
+  return a < b || (a - b) % ld < w || (a - b) % ld + n > ld;  // behind a row: the range reaches the next one
+}
+// What a wave writes must not be what another still reads: the caches (two of fp32, or one and null) and q_out
+// lie apart from each other and from the rows.
+static int check_apart(const char* what, const void* qkv, size_t size, int64_t ld, const void* q_out, const void* c0, const void* c1,
+                       size_t cache_bytes, int T, int NH, int NKV, int HD) {
+  const size_t w = (size_t)(NH + 2 * NKV) * HD * size, q = (size_t)T * NH * HD * size;
+  MIQ_REQUIRE(!c1 || !share_bytes(c0, cache_bytes, c1, cache_bytes), MIQ_ERR_INVALID, "%s: the caches overlap", what);
+  MIQ_REQUIRE(!meets_rows(q_out, q, qkv, T, w, (size_t)ld * size), MIQ_ERR_INVALID, "%s: q_out must lie apart from qkv", what);
+  for (const void* c : {c0, c1})
+    MIQ_REQUIRE(!c || (!share_bytes(c, cache_bytes, q_out, q) && !meets_rows(c, cache_bytes, qkv, T, w, (size_t)ld * size)), MIQ_ERR_INVALID,
+                "%s: the cache must lie apart from qkv and q_out", what);
+  return MIQ_OK;
+}
+
 extern "C" int miq_qk_norm_rope_kv(const float* qkv, int64_t ld, const float* qn, const float* kn, float eps,
                                    const int32_t* state, const float* cos_tab, const float* sin_tab, float* q_out,
                                    float* kcache, float* vcache, int T, int NH, int NKV, int HD, int LMAX, void* stream) {
@@ -344,6 +363,7 @@ extern "C" int miq_qk_norm_rope_kv(const float* qkv, int64_t ld, const float* qn
   const int heads = NH + 2 * NKV, U = several_heads(T, heads) ? kNrHeads : 1;
   const int64_t units = (int64_t)T * ((heads + U - 1) / U);
   MIQ_REQUIRE(grid_holds(units), MIQ_ERR_UNSUPPORTED, "qk_norm_rope_kv: T=%d is past the grid", T);
+  if (int rc = check_apart("qk_norm_rope_kv", qkv, 4, ld, q_out, kcache, vcache, (size_t)NKV * LMAX * HD * 4, T, NH, NKV, HD)) return rc;
   const dim3 grid((unsigned)((units + kNrWaves - 1) / kNrWaves)), block(64 * kNrWaves);
   const hipStream_t st = static_cast<hipStream_t>(stream);
 #define MIQ_NR(HDV, UV)                                                                                                     \
@@ -376,6 +396,9 @@ extern "C" int miq_qk_norm_rope_kv4(const void* qkv, int x_dtype, int64_t ld, co
   const int U = several_heads(T, NH + NKV) ? kNrHeads4 : 1;
   const int64_t units = (int64_t)T * ((NH + U - 1) / U + NKV) + (int64_t)vblocks * NKV * 4 * (HD / 64);
   MIQ_REQUIRE(grid_holds(units), MIQ_ERR_UNSUPPORTED, "qk_norm_rope_kv4: T=%d is past the grid", T);
+  if (int rc = check_apart("qk_norm_rope_kv4", qkv, x_dtype == MIQ_F32 ? 4 : 2, ld, q_out, cache, nullptr,
+                           (size_t)NKV * kv4_blocks(LMAX) * kv4_record(HD), T, NH, NKV, HD))
+    return rc;
   const dim3 grid((unsigned)((units + kNrWaves - 1) / kNrWaves)), block(64 * kNrWaves);
   const hipStream_t st = static_cast<hipStream_t>(stream);
 #define MIQ_NR(HDV, XT, UV)                                                                                       \
