@@ -418,7 +418,8 @@ int miq_kv4_dequant_f32(const void* cache, float* k_out, float* v_out, int NKV, 
  * exactly the tokens that attend to it, and what positions behind the last one hold does not matter.
  * out must not overlap q or the cache (refused). workspace: as miq_gptq_gemv's (counters zero before the first call and left zero; not shared by calls
  * that run concurrently; null where miq_attention_kv4_workspace says 0). Results do not depend on the order of
- * arrival. LMAX up to 2^30. */
+ * arrival. LMAX up to 2^30. A scale that is not finite in units of
+ * log 2 is refused. */
 int miq_attention_kv4_workspace(int T, int NH, int NKV, int HD, int LMAX, size_t* bytes);
 int miq_attention_kv4(const void* q, int x_dtype, const void* cache, const int32_t* state, void* out, int T, int NH,
                       int NKV, int HD, int LMAX, float scale, void* workspace, size_t ws_bytes, void* stream);

@@ -845,6 +845,7 @@ extern "C" int miq_attention_kv4(const void* q, int x_dtype, const void* cache, 
                                  void* stream) {
   if (int rc = check_attention_kv4("attention_kv4", T, NH, NKV, HD, LMAX)) return rc;
   MIQ_REQUIRE(x_dtype == MIQ_F32 || x_dtype == MIQ_F16, MIQ_ERR_UNSUPPORTED, "attention_kv4: x dtype %d", x_dtype);
+  MIQ_REQUIRE(isfinite(scale * 1.44269504088896340736f), MIQ_ERR_INVALID, "attention_kv4: scale=%g", (double)scale);
   if (T == 0) return MIQ_OK;
   MIQ_REQUIRE(q && cache && state && out, MIQ_ERR_INVALID, "attention_kv4: null pointer");
   MIQ_REQUIRE(aligned(cache, 16), MIQ_ERR_ALIGN, "attention_kv4: the cache must be 16-byte aligned");
