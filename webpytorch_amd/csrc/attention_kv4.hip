@@ -125,7 +125,7 @@ __device__ __forceinline__ uint64_t get2(const float* p) {
 }
 // Whether this workgroup is the last of the `slices` that stored their parts (the counter is left zero).
 __device__ __forceinline__ bool last_slice(int* ctr, int slices, int* last) {
-  __builtin_amdgcn_s_waitcnt(0);
+  parts_stored();
   __syncthreads();
   if (threadIdx.x == 0) {
     *last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == slices - 1;

@@ -288,7 +288,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(
         put(part + 1, (uint64_t)__float_as_uint(a.s1) | ((uint64_t)(uint32_t)above << 32));
       }
       if (lane < k) put(part + 2 + lane, list[lane]);
-      __builtin_amdgcn_s_waitcnt(0);
+      parts_stored();
       if (lane == 0) {
         int* ctr = counters + (size_t)t * kLpCtrStride;
         last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == segs - 1;
