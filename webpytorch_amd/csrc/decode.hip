@@ -480,7 +480,7 @@ __global__ __launch_bounds__(256) void argmax_kernel(const float* __restrict__ l
     int32_t* part = state + 4 + 2 * blockIdx.x;
     __hip_atomic_store(part, __float_as_int(bv), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store(part + 1, bi, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __builtin_amdgcn_s_waitcnt(0);
+    parts_stored();
     is_last = __hip_atomic_fetch_add(state + 2, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
   }
   __syncthreads();

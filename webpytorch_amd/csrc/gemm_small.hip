@@ -201,7 +201,7 @@ __global__ __launch_bounds__(NWV * 64) void gemm_small_kernel(const __half* __re
                            (uint64_t)__float_as_uint(ys[u]) | ((uint64_t)__float_as_uint(ys[u + 1]) << 32),
                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    __builtin_amdgcn_s_waitcnt(0);
+    parts_stored();
     int* ctr = counters + (tile * NWV + wave) * kCtrStride;
     int seen = 0;
     if (lane == 0) seen = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

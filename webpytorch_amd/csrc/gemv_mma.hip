@@ -253,7 +253,7 @@ __global__ __launch_bounds__(kThreadsG) void gemv_mma_kernel(const XT* __restric
 #pragma unroll
     for (int t = 0; t < 4; ++t)
       __hip_atomic_store(partials + (size_t)sl * N + c + t, acc[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __builtin_amdgcn_s_waitcnt(0);
+  parts_stored();
   __syncthreads();
   if (threadIdx.x == 0)
     is_last = __hip_atomic_fetch_add(counters + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == kslices - 1;

@@ -533,7 +533,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(1, TM * CB <= 4 ? 768 : 51
         }
       }
   }
-  __builtin_amdgcn_s_waitcnt(0);
+  parts_stored();
   __syncthreads();
   int* ctr = counters + (size_t)ntile * mtiles + mtile;
   if (tid == 0) is_last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ksplit - 1;

@@ -374,7 +374,7 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void gptq_gemv_kernel(
     for (int w = 0; w < W; ++w) s += red[(w * MR + m) * 256 + q];
     __hip_atomic_store(ws + ((size_t)ks * M + m0 + m) * N + n, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  __builtin_amdgcn_s_waitcnt(0);
+  parts_stored();
   __syncthreads();
   int* ctr = counters + (size_t)blockIdx.z * gridDim.x + tile;
   if (threadIdx.x == 0)
