@@ -9,7 +9,7 @@
 // fp32 rows (scaled by a power of two per row); q of fp16 rows is exact. Sums and softmax statistics are fp32. p is held
 // times 2^11 or more, so that its lower part stays in fp16's normal range. (p of fp16 rows as one number cost the output as
 // much again as its own rounding, 2.7e-4 of float64 instead of 2.0e-4, and saved a third of the matrix instructions:
-// 6001 rows of 28 / 4 heads of 128 326 us instead of 425.)
+// 6001 rows of 28 / 4 heads of 128 326 us instead of 410.)
 //
 // Bound and measured (us in graph replay; the floor is the larger of the bytes at a large copy's 4.8 TB/s and the
 // operations at a large fp16 product's 1180 TFLOP/s, twice for fp32 rows): one token of 32 / 8 heads of 128 behind
@@ -182,13 +182,15 @@ __device__ __forceinline__ void join_slices(const float* p0, size_t step, int sl
 // the least). Both to the nearest: towards zero, all small probabilities shrink alike beside a large one (of 16000 keys that
 // share 1 % by a part in 6000). The sum of probabilities is taken of the operands, by the matrix cores.
 __device__ __forceinline__ void split_p(const float* p, half8v* ph) {
+  typedef float float2v __attribute__((ext_vector_type(2)));
+  const float minus = __uint_as_float(opaque(0xBF800000u));  // -1: a difference would take a conversion of hi of its own
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    const half2v hi = {(_Float16)p[2 * x], (_Float16)p[2 * x + 1]};
+    const half2v hi = __builtin_convertvector((float2v){p[2 * x], p[2 * x + 1]}, half2v);
     ph[0][2 * x] = hi.x;
     ph[0][2 * x + 1] = hi.y;
-    ph[1][2 * x] = (_Float16)fmaf((float)hi.x, -1.f, p[2 * x]);
-    ph[1][2 * x + 1] = (_Float16)fmaf((float)hi.y, -1.f, p[2 * x + 1]);
+    ph[1][2 * x] = (_Float16)fmaf((float)hi.x, minus, p[2 * x]);
+    ph[1][2 * x + 1] = (_Float16)fmaf((float)hi.y, minus, p[2 * x + 1]);
   }
 }
 __device__ __forceinline__ half8v ones() { return (half8v){1, 1, 1, 1, 1, 1, 1, 1}; }
@@ -434,10 +436,11 @@ __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
 // operands in LDS, in operand order: each write and read is 16 consecutive bytes a lane. Two buffers, one
 // barrier a step: while a step's products run, the next step's words, loaded a step before that, are unpacked.
 constexpr int kA4TileWaves = 4;
-// blocks of a step and 16-row tiles of a wave: what the registers hold (fp32 rows take twice the operands of q; 3000
-// fp16 rows of 14 / 2 heads of 64: 56 us at one tile a wave, 75 at two, which leave a SIMD two waves)
+// blocks of a step and 16-row tiles of a wave: what the registers hold (fp32 rows take twice the operands of q). fp16
+// rows of heads of 64 at one tile a wave, which leaves a SIMD four waves instead of two, are faster over short contexts
+// (3000 tokens of 14 / 2 heads 56 us instead of 72) and slower over long ones (500 behind 30000 161 instead of 118).
 __host__ __device__ constexpr int kv4_step_blocks(int HD, bool f32) { return HD == 64 ? 2 : HD == 128 && !f32 ? 2 : 1; }
-__host__ __device__ constexpr int kv4_tile_qt(int HD, bool f32) { return HD == 128 && !f32 ? 2 : 1; }
+__host__ __device__ constexpr int kv4_tile_qt(int HD, bool f32) { return HD <= 128 && !f32 ? 2 : 1; }
 __host__ __device__ constexpr int kv4_tile_rows(int HD, bool f32) { return kA4TileWaves * 16 * kv4_tile_qt(HD, f32); }
 
 // Slices of `steps` key steps, of `per` steps each
