@@ -126,3 +126,21 @@ def test_rows_whose_scores_are_all_minus_infinity(gpu, T, pos, lmax):
     assert torch.isnan(got[::3, 0]).all() and torch.isfinite(got[:, 1]).all()
     rest = torch.arange(T) % 3 != 0
     assert torch.isfinite(got[rest]).all()
+
+
+@pytest.mark.parametrize("size,scale", [(3e-39, 3e37), (2e-42, 2e37), (1e-37, 1e36)])
+@pytest.mark.parametrize("T", [1, 700])
+def test_queries_below_the_normal_fp32_range(gpu, T, size, scale):
+    """Under a scale that makes scores of them (the second pair: queries of some thousand steps of 2^-149)."""
+    import torch
+    from test_gpu_kv4_probabilities import last_rows
+    from webpytorch_amd import core
+    g = torch.Generator().manual_seed(T)
+    HD, pos = 64, 600
+    q = (torch.randn((T, 2, HD), generator=g) * size).cuda()
+    k, v = (torch.randn((pos + T, 1, HD), generator=g) for _ in range(2))
+    cache = fill(k, v)
+    rows = min(T, 32)
+    got = core.attention_kv4(q, cache, state(torch, pos), scale=scale)[-rows:].double()
+    want = last_rows(q.double() * (scale * math.sqrt(HD)), cache, pos, rows)  # which divides by sqrt(HD)
+    assert float((got - want).norm() / want.norm()) <= 5e-6

@@ -43,10 +43,10 @@ __device__ __forceinline__ float rows_max(float v) {
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-// 2^n of a row: q 2^n has its largest magnitude in [2^13, 2^14); 1 for zero and non-finite rows
+// 2^n of a row: q 2^n has its largest magnitude in [2^13, 2^14) (less below fp32's normal range); 1 for non-finite rows
 __device__ __forceinline__ int row_shift(float mx) {
   const int e = (int)((__float_as_uint(mx) >> 23) & 255);
-  return (e == 0 || e == 255) ? 0 : 13 + 127 - e;
+  return e == 255 ? 0 : 13 + 127 - max(e, 1);
 }
 
 // A row's reference: a score s (the matrix cores' sum) has the probability 2^((s - shift) back + neg), a fused product
