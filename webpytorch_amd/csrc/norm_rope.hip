@@ -281,8 +281,8 @@ __global__ __launch_bounds__(64 * kNrWaves) void norm_rope_kv4_kernel(
 __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restrict__ cache, float* __restrict__ k_out,
                                                           float* __restrict__ v_out, int HD, int NB, int start, int n) {
   const int NT = HD / 16, NG = HD / 32;
-  const int x = blockIdx.x * 256 + threadIdx.x;  // word of a block: [n][g][i]
-  const int kv = blockIdx.z, blk = start / kKv4Block + blockIdx.y;
+  const int x = blockIdx.y * 256 + threadIdx.x;  // word of a block: [n][g][i]
+  const int kv = blockIdx.z, blk = start / kKv4Block + blockIdx.x;
   if (x >= NT * 64) return;
   const uint8_t* rec = cache + ((size_t)kv * NB + blk) * kv4_record(HD);
   const int i = x & 15, g = (x >> 4) & 3, wn = x >> 6;
@@ -430,8 +430,8 @@ extern "C" int miq_kv4_dequant_f32(const void* cache, float* k_out, float* v_out
   MIQ_REQUIRE(cache, MIQ_ERR_INVALID, "kv4_dequant: null pointer");
   MIQ_REQUIRE(aligned(cache, 16), MIQ_ERR_ALIGN, "kv4_dequant: the cache must be 16-byte aligned");
   const int blocks = (start + n - 1) / kKv4Block - start / kKv4Block + 1;
-  MIQ_REQUIRE(blocks <= 65535, MIQ_ERR_UNSUPPORTED, "kv4_dequant: n=%d positions are past the grid", n);
-  hipLaunchKernelGGL(kv4_dequant_kernel, dim3((HD / 16 * 64 + 255) / 256, blocks, NKV), dim3(256), 0, static_cast<hipStream_t>(stream),
+  MIQ_REQUIRE(blocks < (1 << 24), MIQ_ERR_UNSUPPORTED, "kv4_dequant: n=%d positions are past the grid", n);
+  hipLaunchKernelGGL(kv4_dequant_kernel, dim3(blocks, (HD / 16 * 64 + 255) / 256, NKV), dim3(256), 0, static_cast<hipStream_t>(stream),
                      static_cast<const uint8_t*>(cache), k_out, v_out, HD, kv4_blocks(LMAX), start, n);
   return check_launch("kv4_dequant");
 }
