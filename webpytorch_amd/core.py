@@ -980,7 +980,7 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
     the fp32 tables `cos` / `sin` (positions, HD / 2), and k and v written into `cache`: a pair of fp32
     caches (NKV, LMAX, HD), or a 4-bit cache (`kv4_cache`). Returns q (T, NH, HD) in qkv's dtype. With fp32
     caches qkv is fp32, and the results are those of the library's separate norm and RoPE. Rows whose position
-    is outside the cache write nothing, and their q is zero. (`CausalLM._qkv`, `_rope_np`, `kv_write`:
+    is outside the cache (or, in a 4-bit cache's last block, behind the tables) write nothing, and their q is zero. (`CausalLM._qkv`, `_rope_np`, `kv_write`:
     `webtorch/llm.py:1498-1519, 1270-1304`, `webtorch/_core.py:1504-1540`.)"""
     four = isinstance(cache, torch.Tensor)
     f32 = (torch.float32,)
@@ -999,9 +999,10 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
     T, W = qkv.shape
     if n_heads < 1 or n_heads % nkv or W != (n_heads + 2 * nkv) * hd:
         raise ValueError("rows of %d values are not %d query, %d key and %d value heads of %d" % (W, n_heads, nkv, nkv, hd))
+    least = lmax - KV4_BLOCK + 1 if four else lmax  # a 4-bit cache has whole blocks, whatever its context is
     for name, t in (("cos", cos), ("sin", sin)):
         _check_tensor(name, t, f32, 2, dev)
-        if t.shape[1] * 2 != hd or t.shape[0] < lmax or not t.is_contiguous():
+        if t.shape[1] * 2 != hd or t.shape[0] < least or not t.is_contiguous():
             raise ValueError("%s is a contiguous (positions, %d) table of at least %d positions: got %s" % (name, hd // 2, lmax, tuple(t.shape)))
     for name, t in (("qn", qn), ("kn", kn)):
         if t is not None:
@@ -1021,6 +1022,7 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
     ld = qkv.stride(0) if T > 1 else W
     qp, kp = (None if t is None else t.data_ptr() for t in (qn, kn))
     if four:
+        lmax = min(lmax, cos.shape[0], sin.shape[0])
         _lib.call("miq_qk_norm_rope_kv4", qkv.data_ptr(), dtype_code(qkv), ld, qp, kp, float(eps), state.data_ptr(), cos.data_ptr(),
                   sin.data_ptr(), out.data_ptr(), cache.data_ptr(), T, n_heads, nkv, hd, lmax, _raw_stream(dev))
     else:
