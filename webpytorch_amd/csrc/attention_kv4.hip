@@ -9,15 +9,15 @@
 // fp32 rows (scaled by a power of two per row); q of fp16 rows is exact. Sums and softmax statistics are fp32. p is held
 // times 2^11 or more, so that its lower part stays in fp16's normal range. (p of fp16 rows as one number cost the output as
 // much again as its own rounding, 2.7e-4 of float64 instead of 2.0e-4, and saved a third of the matrix instructions:
-// 6001 rows of 28 / 4 heads of 128 326 us instead of 410.)
+// 6001 rows of 28 / 4 heads of 128 326 us instead of 400.)
 //
-// Bound and measured (us in graph replay; the floor is the larger of the bytes at a large copy's 4.8 TB/s and the
-// operations at a large fp16 product's 1180 TFLOP/s, twice for fp32 rows): one token of 32 / 8 heads of 128 behind
-// 131000 positions 42 (168 MB, 4.0 TB/s; floor 35: 80 KB in flight a CU); behind 700 positions of 14 / 2 heads of 64
-// 7.5 (round trips); 2000 fp32 rows of 28 / 4 heads of 128 from an empty cache 83 (floor 49), 6001 fp16 rows 321
-// (floor 219), 77 fp16 tokens of 32 / 8 heads behind 30000 56 and 9 to join 21 slices (floor 32): bound by
-// the issue of instructions (2000 rows: a wave and step of 32 keys have 160 vector and 34 matrix instructions, 2700 of
-// the 3200 cycles that three waves of a SIMD take; a third of the vector instructions unpack).
+// Bound and measured (us a pass; the floor is the larger of the bytes at a large copy's 4.8 TB/s and the operations at a
+// large fp16 product's 1180 TFLOP/s, twice for fp32 rows and one and a half times for fp16 rows): one token of 32 / 8 heads
+// of 128 behind 131000 positions 41 (168 MB, 4.1 TB/s; floor 35: 80 KB in flight a CU); behind 700 positions of 14 / 2
+// heads of 64 7.2 (round trips); 2000 fp32 rows of 28 / 4 heads of 128 from an empty cache 81 (floor 49), 6001 fp16 rows
+// 400 (floor 328), 77 fp16 tokens of 32 / 8 heads behind 30000 71 and 9 to join 21 slices (floor 48): bound by
+// the issue of instructions (2000 rows: a wave and step of 32 keys have 154 vector and 34 matrix instructions; the vector
+// units are busy 44 % and the matrix cores 30 % of the time; a third of the vector instructions unpack).
 #include <math.h>
 
 #include "kv4.h"
@@ -217,7 +217,8 @@ __device__ __forceinline__ uint32_t keep_pair(int k, int end) { return (k < end 
 
 // Rows that fit a few tiles: the waves of a workgroup share a tile's 16 rows and split its keys, and so do
 // the slices (blockIdx.x) of one tile and kv head. A slice's result (maximum, sum, output) goes to the
-// workspace; the last slice of a tile to arrive adds them in slice order.
+// workspace; the last slice of a tile to arrive adds them in slice order. (fp32 rows of 256 dimensions are more than the
+// registers hold: 92 of them go through scratch memory, one token of 8 / 2 heads behind 120000 positions 86 us; fp16 39.)
 template <int HD, typename XT>
 __global__ __launch_bounds__(64 * kA4Waves) void attention_kv4_rows_kernel(
     const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ state, XT* __restrict__ out,
@@ -787,8 +788,10 @@ __global__ __launch_bounds__(256) void attention_kv4_join_kernel(const int32_t* 
 
 // Up to kA4FewRows rows of a kv head go by the rows kernel, and up to kA4SomeRows where the cache is short: it unpacks
 // a block for 16 rows where the tiles kernel does for 64 or 128, but starts sooner and needs no second launch
-// (32 / 8 heads of 128, us, rows / tiles kernel: 64 rows, 8000 positions 21 / 29, 60000 70 / 70; 256 rows,
-// 0 positions 5.5 / 9.9, 1000 16 / 20, 8000 44 / 42, 60000 230 / 168). The position is the device's, so the rule goes by LMAX. Each tile's keys are
+// (us, rows / tiles kernel: 32 / 8 heads of 128, 64 rows, 8000 positions 21 / 28, 60000 65 / 66; 256 rows,
+// 0 positions 6.1 / 9.9, 1000 17 / 20, 8000 43 / 42, 60000 214 / 164; 14 / 2 heads of 64, 63 rows, 8000 positions
+// 13 / 19, 60000 21 / 38; 252 rows, 8000 14 / 20, 60000 43 / 47; 8 / 2 heads of 256 are the exception, 64 rows, 8000 positions
+// 43 / 32, 256 rows 57 / 39). The position is the device's, so the rule goes by LMAX. Each tile's keys are
 // split into as many slices as give every CU a workgroup (two of the tiles kernel's), of at least a block a
 // wave (8 steps) of a full cache.
 constexpr int kA4FewRows = 64, kA4SomeRows = 512;

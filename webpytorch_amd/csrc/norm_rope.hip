@@ -6,7 +6,7 @@
 // A wave takes heads of one token, lane l the dimensions l, l + 64, ..: the mean is a wave sum, a
 // group of 32 dimensions is half a wave, and a dimension's rotation partner is another register of the lane
 // (HD 128, 256), the lane 32 further (HD 64), or read through LDS. Bound: memory for prompts (4001 tokens into the fp32
-// cache: 150 MB in 29.8 us, 5.0 TB/s), the launch and two round trips for a token (2.4 us).
+// cache: 150 MB in 29.8 us, 5.0 TB/s), the launch and two round trips for a token (2.5 us a replay).
 #include <math.h>
 
 #include "kv4.h"
