@@ -980,7 +980,8 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
     the fp32 tables `cos` / `sin` (positions, HD / 2), and k and v written into `cache`: a pair of fp32
     caches (NKV, LMAX, HD), or a 4-bit cache (`kv4_cache`). Returns q (T, NH, HD) in qkv's dtype. With fp32
     caches qkv is fp32, and the results are those of the library's separate norm and RoPE. Rows whose position
-    is outside the cache (or, in a 4-bit cache's last block, behind the tables) write nothing, and their q is zero. (`CausalLM._qkv`, `_rope_np`, `kv_write`:
+    is outside the cache (or, in a 4-bit cache's last block, behind the tables) write nothing, and their q is
+    zero. `out`, if given, and the caches may not overlap each other or qkv. (`CausalLM._qkv`, `_rope_np`, `kv_write`:
     `webtorch/llm.py:1498-1519, 1270-1304`, `webtorch/_core.py:1504-1540`.)"""
     four = isinstance(cache, torch.Tensor)
     f32 = (torch.float32,)
@@ -1034,7 +1035,8 @@ def qk_norm_rope(qkv, state, cos, sin, n_heads, cache, qn=None, kn=None, eps=1e-
 def attention_kv4(q, cache, state, scale=None, out=None):
     """Causal grouped-query attention of q (T, NH, HD), fp32 or fp16, over a 4-bit cache: token t, at
     position state[0] + t, attends to positions 0 .. state[0] + t; scale is 1 / sqrt(HD) unless given. A token
-    whose position is below 0 gets zeros. Returns (T, NH, HD) in q's dtype. (`KVCache.attn`, `gqa_attention`:
+    whose position is below 0 gets zeros. `out`, if given, may not overlap q or the cache. Returns (T, NH, HD) in
+    q's dtype. (`KVCache.attn`, `gqa_attention`:
     `webtorch/_core.py:1543-1596, 1319-1340`, which keep the cache in fp32.)"""
     dev = _gpu_of("q", q)
     _check_tensor("q", q, (torch.float32, torch.float16), 3, dev)
