@@ -62,3 +62,25 @@ def test_layers_off_the_matrix_cores_have_their_workspace_from_the_start(gpu):
     for n in (100, 333, 500):
         m.generate(ids[:n], 2)
     assert {k: t.numel() for k, t in core._WORKSPACE.items()} == before
+
+
+def test_rows_past_the_gemvs_workspace_go_in_pieces(gpu, monkeypatch):
+    """The products of the test above with 16 MB for them: a prompt of 500 rows takes several calls, and no more memory."""
+    from webpytorch_amd import core
+    sh = dict(SMALL, H=1024, NH=16, I=9728)
+    w = synth.decoder_weights(43, **sh)
+    for lay in w["layers"]:
+        for name in ("q", "k", "v", "o", "gate", "up", "down"):
+            lay[name]["zoff"] = 0.5
+    ids = [int(i) for i in synth.prompt_ids(43, 500, sh["V"])]
+    a = model(w, 520, persistent=False)
+    monkeypatch.setattr(core, "GEMV_ROWS_BYTES", 16 << 20)
+    b = model(w, 520, persistent=False)
+    assert b.ws.numel() <= 16 << 20 < a.ws.numel()
+    for m in (a, b):
+        m.generate(ids[:20], 2)
+    before = {k: t.numel() for k, t in core._WORKSPACE.items()}
+    for n in (9, 100, 500):
+        la, lb = [(m.generate(ids[:n], 1), m.buf["logits"].clone())[1] for m in (a, b)]
+        assert float((la - lb).norm()) <= 1e-5 * float(la.norm())
+    assert {k: t.numel() for k, t in core._WORKSPACE.items()} == before

@@ -261,6 +261,19 @@ def gptq_dequant(qweight, qzeros, scales, K, N, gs, bits, zoff=0.0, g_idx=None):
     return out
 
 
+# workspace that rows of one GEMV call may take with a workspace handed in: its sums are fp32 numbers of every row, column
+# and slice of K, 0.1 TB for 16384 rows of 53248 -> 16384, so that more rows go in pieces
+GEMV_ROWS_BYTES = 1 << 30
+
+
+def gemv_rows(M, K, N, gs, bits, x_dtype, nbytes):
+    """How many of M rows a GEMV call takes at a time with nbytes of workspace: halved until they fit, GEMV_MAX_M
+    at the least."""
+    while M > GEMV_MAX_M and gemv_workspace_bytes(M, K, N, gs, bits, x_dtype) > nbytes:
+        M = (M + 15) // 16 * 8
+    return M
+
+
 def f32_rows_on_matrix_cores(K, zoff):
     """Whether more than GEMV_MAX_M fp32 rows run the matrix-core GEMM: the zero points are whole numbers in its
     operands, and K fits its rows. The GEMV takes the others."""
@@ -303,6 +316,13 @@ def _gptq_matmul(xf, qweight, qzeros, scales, K, N, gs, bits, zoff=0.0, *, bias=
                   float(zoff), ptr(ws), ws.numel(), stream_handle())
         return out
     need = gemv_workspace_bytes(M, K, N, gs, bits, xd)
+    if ws is not None and ws.numel() < need and M > GEMV_MAX_M:
+        rows = gemv_rows(M, K, N, gs, bits, xd, max(ws.numel(), GEMV_ROWS_BYTES))
+        if rows < M:
+            for r in range(0, M, rows):
+                _gptq_matmul(xf[r:r + rows], qweight, qzeros, scales, K, N, gs, bits, zoff, bias=bias, perm=perm,
+                             out=out[r:r + rows], ws=ws, _check=False)
+            return out
     if ws is None or ws.numel() < need:
         ws = workspace(need)
     _lib.call("miq_gptq_gemv", ptr(xf), xd, ptr(perm), ptr(qweight), ptr(qzeros),

@@ -354,7 +354,7 @@ class CausalLM:
             for lin in lins.values():
                 if M > core.GEMV_MAX_M and core.f32_rows_on_matrix_cores(lin.K, lin.zoff):
                     need = max(need, core.gemm_f32x_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits))
-                else:
+                elif M <= core.gemv_rows(M, lin.K, lin.N, lin.gs, lin.bits, _lib.MIQ_F32, core.GEMV_ROWS_BYTES):
                     need = max(need, core.gemv_workspace_bytes(M, lin.K, lin.N, lin.gs, lin.bits, _lib.MIQ_F32))
             if self.kv_bits == 4:
                 need = max(need, core.attention_kv4_workspace_bytes(M, self.NH, self.NKV, self.HD, self.lmax))
