@@ -439,6 +439,74 @@ int miq_token_logprobs(const void* logits, int x_dtype, int64_t ld, const int32_
                        float* logprobs, float* entropy, int32_t* ranks, int32_t* top_ids, float* top_logprobs,
                        const int32_t* state, int out_rows, void* workspace, size_t ws_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Serving a batch of sequences: position rotation, a paged key-value cache with its append and its
+ * attention, and the verification of drafted tokens.
+ * ------------------------------------------------------------------------------------- */
+
+/* Position rotation of x [T][H] rows of HD values (fp32 or fp16; tokens ld, heads lh values apart) to out (the same
+ * type; out_ld, out_lh): of each head's first rot dimensions the pairs (i, i + rot / 2), or with pairs = 1 (2 i, 2 i + 1),
+ *   y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin
+ * with row positions[t] of the fp32 tables cos_tab / sin_tab [rows][rot / 2]; the other dimensions are copied. transpose = 1
+ * takes -sin: the gradient with respect to x of a gradient of out. A position below 0 or from rows on makes zeros.
+ * fp32 arithmetic, one rounding to out's type. out may be x itself; any other overlap is refused. HD even, <= 1024.
+ * Replaces: `_rope_np`, `_rot` (webtorch/llm.py:1270-1304) and `rope_decode` (webtorch/_core.py:2302-2330), which rotate
+ * whole heads in halves. */
+int miq_rope(const void* x, int x_dtype, int64_t ld, int64_t lh, const int32_t* positions, const float* cos_tab,
+             const float* sin_tab, int rows, int rot, int pairs, int transpose, void* out, int64_t out_ld, int64_t out_lh,
+             int T, int H, int HD, void* stream);
+
+/* A paged cache is [num_pages][2][NKV][page][HD] of fp16 or fp32 (cache_dtype), 16-byte aligned: keys, then values, of
+ * each page; page a power of two from 16 to 4096, HD 64, 128, 192 or 256. Position n of sequence s is slot n % page of
+ * page pages[s][n / page] (int32 [S][max_pages]; an entry outside 0 .. num_pages - 1 is no page). A batch has T tokens of each
+ * of S sequences at positions[s][t] (int32; below 0: no token).
+ *
+ * miq_paged_append: of the q|k|v rows qkv [S T][(NH + 2 NKV) HD] (fp32 or fp16, ld values apart) RMSNorm of the query and key
+ * heads (weights qn, kn fp32 [HD]; null: none), rotation of both as miq_rope's (rot = 0: none, the tables may be null),
+ * queries to q_out [S T][NH][HD] in qkv's type, keys and values to their slots. A token without a position, page or table row
+ * writes nothing, and its q is zero. fp32 arithmetic, one rounding. NH may be 0 (rows of k|v alone). Of two tokens of one
+ * call at one slot either one's values may stay. qkv, q_out and the cache may not overlap.
+ * Replaces: `CausalLM._qkv`, `_rope_np` and `kv_write` (webtorch/llm.py:1498-1519, 1270-1304; webtorch/_core.py:1504-1540), one
+ * sequence into a contiguous fp32 cache. */
+int miq_paged_append(const void* qkv, int x_dtype, int64_t ld, const float* qn, const float* kn, float eps, const int32_t* positions,
+                     const int32_t* pages, int max_pages, const float* cos_tab, const float* sin_tab, int rows, int rot, int pairs,
+                     void* q_out, void* cache, int cache_dtype, int num_pages, int page, int S, int T, int NH, int NKV, int HD,
+                     void* stream);
+
+/* Attention over a paged cache: q and out [S][T][NH][HD] (fp32 or fp16); token t of sequence s attends to the positions
+ * 0 .. positions[s][t] (those of the table at the most) that have a page, query head h to kv head h / (NH / NKV). A token without
+ * a position or with nothing to attend to gets zeros. Values of an fp16 cache are exact in the products; probabilities, and q of fp32
+ * rows, are two fp16 numbers each (22 bits). fp32 caches: fp32 products. Sums are fp32. An infinity or NaN among the values reaches
+ * exactly the tokens that attend to it, and makes NaN or infinity of them. Made for few tokens of each sequence; any T is right.
+ * workspace: as miq_gptq_gemv's (counters zero before the first call and left zero; not shared by calls that run
+ * concurrently; null where miq_paged_attention_workspace says 0). Results do not depend on the order of arrival; their last bits
+ * depend on the batch's lengths, by which the work is split. out must not overlap q or the cache (refused).
+ * Replaces: `KVCache.attn` + `gqa_attention` (webtorch/_core.py:1543-1596, 1319-1340) for one sequence and a contiguous cache. */
+int miq_paged_attention_workspace(int S, int T, int NH, int NKV, int HD, int page, int max_pages, int cache_dtype, size_t* bytes);
+int miq_paged_attention(const void* q, int x_dtype, const void* cache, int cache_dtype, int num_pages, int page,
+                        const int32_t* positions, const int32_t* pages, int max_pages, void* out, int S, int T, int NH, int NKV,
+                        int HD, float scale, void* workspace, size_t ws_bytes, void* stream);
+
+/* Verification of D drafted tokens of each of S sequences, and the token behind the accepted ones. logits: the target's rows
+ * [S][D + 1] of V (row i judges draft i, row D follows the last one), draft_logits: the draft's rows [S][D] of the same type, or
+ * null for drafts that were not drawn (looked up, or the likeliest): q_i(x_i) = 1. Sequences and rows lie ld_seq, ld_row values
+ * apart. drafts int32 [S][D]: a sequence's end at the first id below 0. With p, q the softmaxes of rows over the temperature
+ * (temperatures fp32 [S], or null: `temperature`) draft i is accepted while uniforms[s][i] q_i(x_i) < p_i(x_i); behind
+ * n accepted ones a token is drawn from max(p_n - q_n, 0), or from p_n if none was refused: the lowest index whose running sum of
+ * weights passes uniforms[s][D] times their total. Temperature 0 (or below, or NaN): a draft is accepted if it is the largest logit's
+ * index (the lowest of equal ones; NaN counts as -inf), which is the token too.
+ * tokens int32 [S][D + 1]: the accepted drafts, the token, then -1; accepted int32 [S]: n. Logits of -inf are tokens of
+ * probability 0. A target row without a distribution (NaN, +inf at a temperature above 0, nothing above -inf) accepts nothing and
+ * its token is -1; without one a draft's row is refused and p drawn from; so is a draft from V on. Where max(p - q, 0) has no weight
+ * the token is the draft. fp64 exponentials and sums (3e-13). D <= 32, S (2 D + 1) <= 65535. workspace as for
+ * miq_paged_attention (always needed).
+ * Replaces: the host's draw from logits read back, one token a pass (`_pick`: webtorch/llm.py:1309-1336). */
+int miq_verify_drafts_workspace(int S, int D, int V, size_t* bytes);
+int miq_verify_drafts(const void* logits, int x_dtype, int64_t ld_seq, int64_t ld_row, const int32_t* drafts,
+                      const void* draft_logits, int64_t draft_ld_seq, int64_t draft_ld_row, const float* uniforms,
+                      const float* temperatures, float temperature, int32_t* tokens, int32_t* accepted, int S, int D, int V,
+                      void* workspace, size_t ws_bytes, void* stream);
+
 /* out[t][i] = silu(gu[t][i]) * gu[t][I + i] for the fused gate|up rows.
  * Replaces: `silu(gate(x)) * up(x)` of `CausalLM._mlp` (webtorch/llm.py:1489-1496,
  * webtorch/_core.py:503-504). */

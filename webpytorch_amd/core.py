@@ -1112,3 +1112,257 @@ def token_logprobs(logits, ids, top_k=0):
                   lp.data_ptr() + 4 * t0, ent.data_ptr() + 4 * t0, rank.data_ptr() + 4 * t0, ti.data_ptr() + 4 * top_k * t0,
                   tl.data_ptr() + 4 * top_k * t0, None, n, wp, wn, st)
     return TokenLogprobs(lp, ent, rank, ti, tl)
+
+
+# ---- serving a batch: position rotation, a paged cache with its append and attention, drafted tokens ----
+PAGE_SIZES = (16, 4096)  # least and most positions of a page, a power of two
+MAX_DRAFTS = 32
+Rope = collections.namedtuple("Rope", "cos sin interleaved")
+
+
+def rope_tables(n, rot, theta=10000.0, scaling=None, interleaved=False):
+    """The rotation tables of positions 0 .. n - 1 over `rot` dimensions as a `Rope` (cos and sin fp32 (n, rot / 2), from
+    float64 angles rounded once, as `_rope_np` builds them: `webtorch/llm.py:1270-1304`). `interleaved` pairs dimensions
+    (2 i, 2 i + 1) instead of (i, i + rot / 2). `scaling` stretches the angles to a longer context than the one trained
+    with; with f_i = theta^(-2 i / rot) it is None or a dict whose "rope_type" is
+      "linear": f_i / factor;
+      "dynamic": theta grows by (factor n / original - factor + 1)^(rot / (rot - 2)) where n is past `original`;
+      "yarn": f_i where a pair turns more than beta_fast (32) times in `original` positions, f_i / factor where fewer than
+        beta_slow (1), a linear ramp over i between; cos and sin times attention_factor (0.1 ln factor + 1);
+      "wavelength": f_i where 2 pi / f_i < original / high_freq_factor (4), f_i / factor where it is above original /
+        low_freq_factor (1), and between them the two mixed linearly in original f_i / 2 pi;
+    with "factor" and (but for linear) "original_max_position_embeddings"."""
+    n, rot = int(n), int(rot)
+    if n < 1 or rot < 2 or rot % 2:
+        raise ValueError("rope_tables: n=%d rot=%d" % (n, rot))
+    i2 = np.arange(0, rot, 2, dtype=np.float64)
+    sc = dict(scaling or {})
+    kind = sc.get("rope_type", sc.get("type", "default"))
+    factor, mul = float(sc.get("factor", 1.0)), 1.0
+    original = float(sc.get("original_max_position_embeddings", 0) or 0)
+    if kind not in ("default", "linear", "dynamic", "yarn", "wavelength"):
+        raise NotImplementedError("rope_type %r (linear, dynamic, yarn or wavelength)" % (kind,))
+    if not factor > 0 or not theta > 0 or (kind in ("dynamic", "yarn", "wavelength") and not original > 0):
+        raise ValueError("rope_tables: theta=%g factor=%g original_max_position_embeddings=%g" % (theta, factor, original))
+    if kind == "dynamic" and n > original and rot > 2:
+        theta = theta * (factor * n / original - factor + 1.0) ** (rot / (rot - 2.0))
+    inv = 1.0 / (float(theta) ** (i2 / rot))
+    if kind == "linear":
+        inv = inv / factor
+    elif kind == "yarn":
+        at = lambda turns: rot * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))  # noqa: E731
+        lo = max(math.floor(at(float(sc.get("beta_fast", 32.0)))), 0)
+        hi = min(math.ceil(at(float(sc.get("beta_slow", 1.0)))), rot - 1)
+        slow = np.clip((np.arange(rot // 2, dtype=np.float64) - lo) / max(hi - lo, 1e-3), 0.0, 1.0)
+        inv = inv * (1.0 - slow) + inv / factor * slow
+        mul = sc.get("attention_factor")
+        mul = 0.1 * math.log(factor) + 1.0 if mul is None and factor > 1 else 1.0 if mul is None else float(mul)
+    elif kind == "wavelength":
+        low, high = float(sc.get("low_freq_factor", 1.0)), float(sc.get("high_freq_factor", 4.0))
+        if not high > low:
+            raise ValueError("rope_tables: high_freq_factor=%g is not above low_freq_factor=%g" % (high, low))
+        plain = np.clip((original * inv / (2.0 * math.pi) - low) / (high - low), 0.0, 1.0)
+        inv = inv * plain + inv / factor * (1.0 - plain)
+    ang = np.arange(0, n, dtype=np.float64)[:, None] * inv[None, :]
+    return Rope(to_device((np.cos(ang) * mul).astype(np.float32)), to_device((np.sin(ang) * mul).astype(np.float32)), bool(interleaved))
+
+
+def _rope_arg(rope, hd, dev):
+    """(cos address, sin address, rows, rot, pairs) of a `Rope` for heads of hd."""
+    cos, sin, pairs = rope
+    for name, t in (("cos", cos), ("sin", sin)):
+        _check_tensor(name, t, (torch.float32,), 2, dev)
+        if t.shape != cos.shape or not 2 <= 2 * t.shape[1] <= hd or t.shape[0] < 1 or not t.is_contiguous():
+            raise ValueError("cos and sin are two contiguous (positions, rot / 2) tables, rot at most %d: got %s and %s"
+                             % (hd, tuple(cos.shape), tuple(sin.shape)))
+    return cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], int(bool(pairs))
+
+
+def _int32(name, t, shape, dev):
+    """A contiguous int32 tensor of this shape."""
+    _check_tensor(name, t, (torch.int32,), len(shape), dev)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s has shape %s: %s is expected" % (name, tuple(t.shape), tuple(shape)))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def rope(x, positions, rope, transpose=False, out=None):
+    """Rotates x (T, H, HD), fp32 or fp16, by the rows of `rope` (`Rope`, `rope_tables`) at `positions` (T,) int32: of each
+    head's first 2 rope.cos.shape[1] dimensions; the others are copied. `transpose` turns the other way: the gradient with respect
+    to x of a gradient of the output. Tokens and heads of x may lie further apart (a slice of fused q|k|v rows). A
+    position outside the tables makes zeros. `out`, if given, is of x's type and shape; it may be x itself, but not overlap it
+    otherwise. (`_rope_np`, `_rot`: `webtorch/llm.py:1270-1304`.)"""
+    dev = _gpu_of("x", x)
+    _check_tensor("x", x, (torch.float32, torch.float16), 3, dev)
+    T, H, hd = x.shape
+    if hd % 2 or not 2 <= hd <= 1024:
+        raise ValueError("heads of %d dimensions (even, 2 .. 1024)" % hd)
+    cp, sp, rows, rot, pairs = _rope_arg(rope, hd, dev)
+    positions = _int32("positions", positions, (T,), dev)
+    same = out is x
+    if x.stride(2) != 1 or (H > 1 and x.stride(1) < hd) or (T > 1 and x.stride(0) < hd):
+        if same:
+            raise ValueError("x is rotated in place where its heads are contiguous and apart: strides %s" % (x.stride(),))
+        x = x.contiguous()
+    if out is None:
+        out = torch.empty(T, H, hd, dtype=x.dtype, device=dev)
+    elif not same:
+        _check_tensor("out", out, (x.dtype,), 3, dev)
+        if out.shape != x.shape or (out.numel() and out.stride(2) != 1):
+            raise ValueError("out has shape %s, strides %s: %s with contiguous heads is expected" % (tuple(out.shape), out.stride(), tuple(x.shape)))
+    _lib.call("miq_rope", x.data_ptr(), dtype_code(x), x.stride(0), x.stride(1), positions.data_ptr(), cp, sp, rows, rot, pairs,
+              int(bool(transpose)), out.data_ptr(), out.stride(0), out.stride(1), T, H, hd, _raw_stream(dev))
+    return out
+
+
+def paged_cache(num_pages, nkv, page, hd, dtype=torch.float16):
+    """An empty paged key-value cache of one layer: (num_pages, 2, nkv, page, hd), zeros; keys at [:, 0], values at [:, 1].
+    `page` positions a page, a power of two from 16 to 4096."""
+    if hd not in KV4_HEADS:
+        raise NotImplementedError("a paged cache holds heads of 64, 128, 192 or 256 dimensions, not %d" % hd)
+    if num_pages < 1 or nkv < 1 or not PAGE_SIZES[0] <= page <= PAGE_SIZES[1] or page & (page - 1):
+        raise ValueError("paged_cache: num_pages=%d nkv=%d page=%d (a power of two from %d to %d)" % ((num_pages, nkv, page) + PAGE_SIZES))
+    if dtype not in (torch.float16, torch.float32):
+        raise TypeError("a paged cache is float16 or float32, not %s" % dtype)
+    return torch.zeros((num_pages, 2, nkv, page, hd), dtype=dtype, device=device())
+
+
+def _paged(cache, positions, pages, dev):
+    """Checks a paged cache with a batch's positions (S, T) and pages (S, most): (num_pages, nkv, page, hd, positions, pages)."""
+    _check_tensor("the cache", cache, (torch.float16, torch.float32), 5, dev)
+    num, two, nkv, page, hd = cache.shape
+    if two != 2 or hd not in KV4_HEADS or num < 1 or nkv < 1 or not PAGE_SIZES[0] <= page <= PAGE_SIZES[1] or page & (page - 1) \
+            or not cache.is_contiguous():
+        raise ValueError("a paged cache is a contiguous (pages, 2, NKV, page, HD) tensor, page a power of two from %d to %d, HD 64, 128, 192 or "
+                         "256: got %s" % (PAGE_SIZES + (tuple(cache.shape),)))
+    _check_tensor("positions", positions, (torch.int32,), 2, dev)
+    _check_tensor("pages", pages, (torch.int32,), 2, dev)
+    if pages.shape[0] != positions.shape[0]:
+        raise ValueError("pages of %d sequences, positions of %d" % (pages.shape[0], positions.shape[0]))
+    return num, nkv, page, hd, positions if positions.is_contiguous() else positions.contiguous(), pages if pages.is_contiguous() else pages.contiguous()
+
+
+def paged_append(qkv, positions, pages, cache, n_heads, rope=None, qn=None, kn=None, eps=1e-6, out=None):
+    """Appends a batch's new tokens to a paged cache (`paged_cache`): of the q|k|v rows `qkv` (S, T, (NH + 2 NKV) HD), fp32 or
+    fp16, at `positions` (S, T) int32 (-1: no token) RMSNorm of query and key heads by `qn` / `kn` (fp32 (HD,); None: no
+    norm), the rotation `rope` (`Rope`; None: none) of both, keys and values into `cache` (pages, 2, NKV, page, HD): position
+    n of sequence s is slot n % page of page pages[s, n // page] (int32 (S, most), -1: none). Returns q (S, T, NH, HD) in qkv's
+    dtype; n_heads 0 takes rows of k|v alone. A token without a position, a page or a row of the tables writes nothing, and its q is
+    zero. Of two tokens of one call at one slot either one's values may stay. `out`, if given, and the cache may
+    not overlap qkv or each other. (`CausalLM._qkv`, `_rope_np`, `kv_write`: `webtorch/llm.py:1498-1519, 1270-1304`,
+    `webtorch/_core.py:1504-1540`, one sequence into a contiguous cache.)"""
+    dev = _gpu_of("qkv", qkv)
+    _check_tensor("qkv", qkv, (torch.float32, torch.float16), 3, dev)
+    num, nkv, page, hd, positions, pages = _paged(cache, positions, pages, dev)
+    S, T, W = qkv.shape
+    if tuple(positions.shape) != (S, T):
+        raise ValueError("positions %s of qkv %s" % (tuple(positions.shape), tuple(qkv.shape)))
+    if n_heads < 0 or W != (n_heads + 2 * nkv) * hd:
+        raise ValueError("rows of %d values are not %d query, %d key and %d value heads of %d" % (W, n_heads, nkv, nkv, hd))
+    cp, sp, rows, rot, pairs = (None, None, 0, 0, 0) if rope is None else _rope_arg(rope, hd, dev)
+    for name, t in (("qn", qn), ("kn", kn)):
+        if t is not None:
+            _check_tensor(name, t, (torch.float32,), 1, dev)
+            if t.shape[0] != hd or not t.is_contiguous():
+                raise ValueError("%s has shape %s: (%d,) is expected" % (name, tuple(t.shape), hd))
+    # rows of one distance
+    ld = qkv.stride(1) if T > 1 else qkv.stride(0) if S > 1 else W
+    if qkv.stride(2) != 1 or ld < W or (S > 1 and T > 1 and qkv.stride(0) != T * ld):
+        qkv = qkv.contiguous()
+        ld = W
+    if out is None:
+        out = torch.empty(S, T, n_heads, hd, dtype=qkv.dtype, device=dev)
+    else:
+        _check_tensor("out", out, (qkv.dtype,), None, dev)
+        if out.numel() != S * T * n_heads * hd or not out.is_contiguous():
+            raise ValueError("out is a contiguous tensor of %d values: got %s" % (S * T * n_heads * hd, tuple(out.shape)))
+    qp, kp = (None if t is None else t.data_ptr() for t in (qn, kn))
+    _lib.call("miq_paged_append", qkv.data_ptr(), dtype_code(qkv), ld, qp, kp, float(eps), positions.data_ptr(), pages.data_ptr(), pages.shape[1],
+              cp, sp, rows, rot, pairs, out.data_ptr(), cache.data_ptr(), dtype_code(cache), num, page, S, T, n_heads, nkv, hd, _raw_stream(dev))
+    return out
+
+
+def paged_attention_workspace_bytes(S, T, NH, NKV, HD, page, max_pages, cache_dtype):
+    """Bytes of workspace `miq_paged_attention` needs (cached per shape)."""
+    return _bytes(("paged", S, T, NH, NKV, HD, page, max_pages, cache_dtype), "miq_paged_attention_workspace", S, T, NH, NKV, HD, page, max_pages,
+                  cache_dtype)
+
+
+def paged_attention(q, positions, pages, cache, scale=None, out=None):
+    """Grouped-query attention of q (S, T, NH, HD), fp32 or fp16, over a paged cache (`paged_append`): token t of sequence s
+    attends to the positions 0 .. positions[s, t] that have a page; scale is 1 / sqrt(HD) unless given. A token without a
+    position (-1), or with nothing to attend to, gets zeros. Made for the one or few new tokens (drafted ones) of many sequences; the
+    work is split by their lengths, on the device. `out`, if given, may not overlap q or the cache. Returns (S, T, NH, HD)
+    in q's dtype. (`KVCache.attn`, `gqa_attention`: `webtorch/_core.py:1543-1596, 1319-1340`.)"""
+    dev = _gpu_of("q", q)
+    _check_tensor("q", q, (torch.float32, torch.float16), 4, dev)
+    num, nkv, page, hd, positions, pages = _paged(cache, positions, pages, dev)
+    S, T, nh, qd = q.shape
+    if qd != hd or nh < 1 or nh % nkv or tuple(positions.shape) != (S, T):
+        raise ValueError("q %s does not go with a cache of %d heads of %d and positions %s" % (tuple(q.shape), nkv, hd, tuple(positions.shape)))
+    q = q.contiguous()
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _check_tensor("out", out, (q.dtype,), None, dev)
+        if out.numel() != q.numel() or not out.is_contiguous():
+            raise ValueError("out is a contiguous tensor of %d values: got %s" % (q.numel(), tuple(out.shape)))
+    code = dtype_code(cache)
+    wp, wn, _keep = _call_workspace(paged_attention_workspace_bytes(S, T, nh, nkv, hd, page, pages.shape[1], code), dev)
+    _lib.call("miq_paged_attention", q.data_ptr(), dtype_code(q), cache.data_ptr(), code, num, page, positions.data_ptr(), pages.data_ptr(),
+              pages.shape[1], out.data_ptr(), S, T, nh, nkv, hd, 1.0 / math.sqrt(hd) if scale is None else float(scale), wp, wn, _raw_stream(dev))
+    return out
+
+
+DraftVerdict = collections.namedtuple("DraftVerdict", "tokens accepted")
+
+
+def verify_drafts(logits, drafts, uniforms, draft_logits=None, temperature=1.0):
+    """Verifies drafted tokens against the target's probabilities and draws the token behind the accepted ones. `logits`
+    (S, D + 1, V), fp32 or fp16: the target's rows, row i judging draft i; `drafts` (S, D) int32, a sequence's end at the first
+    id below 0 (D may be 0: a draw alone); `uniforms` (S, D + 1) fp32 in [0, 1); `draft_logits` (S, D, V) of the same dtype,
+    the rows the drafts were drawn from, or None for drafts that were not drawn. With p and q the softmaxes over
+    `temperature` (a number, or fp32 (S,); 0: all at the largest logit) draft i is accepted while
+    uniforms[:, i] q_i(x_i) < p_i(x_i) (q = 1 without draft logits), and behind n accepted ones the token is drawn from max(p_n - q_n, 0),
+    or p_n where none was refused: the lowest index whose running sum passes uniforms[:, D] times the total, so that
+    tokens are distributed as the target's. Returns DraftVerdict of tokens (S, D + 1) int32 (accepted drafts, the token, then -1) and
+    accepted (S,) int32. -inf logits are tokens of probability 0; a target row with NaN or +inf, or of nothing above -inf, accepts
+    nothing and gives -1. D <= 32. (`_pick`: `webtorch/llm.py:1309-1336`, on the host.)"""
+    dev = _gpu_of("logits", logits)
+    _check_tensor("logits", logits, (torch.float32, torch.float16), 3, dev)
+    S, rows, V = logits.shape
+    D = rows - 1
+    if D < 0 or V < 1:
+        raise ValueError("logits (S, D + 1, V) have shape %s" % (tuple(logits.shape),))
+    drafts = _int32("drafts", drafts, (S, D), dev)
+    _check_tensor("uniforms", uniforms, (torch.float32,), 2, dev)
+    if tuple(uniforms.shape) != (S, D + 1):
+        raise ValueError("uniforms have shape %s: %s is expected" % (tuple(uniforms.shape), (S, D + 1)))
+    uniforms = uniforms.contiguous()
+    temps, temp = None, 0.0
+    if isinstance(temperature, torch.Tensor):
+        _check_tensor("temperature", temperature, (torch.float32,), 1, dev)
+        if temperature.shape[0] != S:
+            raise ValueError("temperature has shape %s: (%d,) is expected" % (tuple(temperature.shape), S))
+        temps = temperature.contiguous()
+    else:
+        temp = float(temperature)
+    rows_apart = lambda t: t.stride(2) == 1 and (t.shape[1] < 2 or t.stride(1) >= V) and (t.shape[0] < 2 or t.stride(0) >= 0)  # noqa: E731
+    ld = lambda t: (t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else V)  # noqa: E731
+    if not rows_apart(logits):
+        logits = logits.contiguous()
+    dp, dl = None, (0, V)
+    if draft_logits is not None:
+        _check_tensor("draft_logits", draft_logits, (logits.dtype,), 3, dev)
+        if tuple(draft_logits.shape) != (S, D, V):
+            raise ValueError("draft_logits have shape %s: %s is expected" % (tuple(draft_logits.shape), (S, D, V)))
+        if D:
+            if not rows_apart(draft_logits):
+                draft_logits = draft_logits.contiguous()
+            dp, dl = draft_logits.data_ptr(), ld(draft_logits)
+    tokens = torch.empty(S, D + 1, dtype=torch.int32, device=dev)
+    accepted = torch.empty(S, dtype=torch.int32, device=dev)
+    wp, wn, _keep = _call_workspace(_bytes(("verify", S, D, V), "miq_verify_drafts_workspace", S, D, V), dev)
+    _lib.call("miq_verify_drafts", logits.data_ptr(), dtype_code(logits), *ld(logits), drafts.data_ptr(), dp, *dl, uniforms.data_ptr(),
+              None if temps is None else temps.data_ptr(), temp, tokens.data_ptr(), accepted.data_ptr(), S, D, V, wp, wn, _raw_stream(dev))
+    return DraftVerdict(tokens, accepted)
