@@ -493,12 +493,12 @@ int miq_paged_attention(const void* q, int x_dtype, const void* cache, int cache
  * apart. drafts int32 [S][D]: a sequence's end at the first id below 0. With p, q the softmaxes of rows over the temperature
  * (temperatures fp32 [S], or null: `temperature`) draft i is accepted while uniforms[s][i] q_i(x_i) < p_i(x_i); behind
  * n accepted ones a token is drawn from max(p_n - q_n, 0), or from p_n if none was refused: the lowest index whose running sum of
- * weights passes uniforms[s][D] times their total. Temperature 0 (or below, or NaN): a draft is accepted if it is the largest logit's
+ * weights passes uniforms[s][D] times their total. Temperature 0 (or one that is no finite number above it): a draft is accepted if it is the largest logit's
  * index (the lowest of equal ones; NaN counts as -inf), which is the token too.
  * tokens int32 [S][D + 1]: the accepted drafts, the token, then -1; accepted int32 [S]: n. Logits of -inf are tokens of
  * probability 0. A target row without a distribution (NaN, +inf at a temperature above 0, nothing above -inf) accepts nothing and
  * its token is -1; without one a draft's row is refused and p drawn from; so is a draft from V on. Where max(p - q, 0) has no weight
- * the token is the draft. fp64 exponentials and sums (3e-13). D <= 32, S (2 D + 1) <= 65535. workspace as for
+ * the token is the draft. fp64 exponentials and sums (2e-13). D <= 32, S (2 D + 1) <= 65535. workspace as for
  * miq_paged_attention (always needed).
  * Replaces: the host's draw from logits read back, one token a pass (`_pick`: webtorch/llm.py:1309-1336). */
 int miq_verify_drafts_workspace(int S, int D, int V, size_t* bytes);

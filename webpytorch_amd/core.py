@@ -897,7 +897,7 @@ KV4_BLOCK = 32       # positions of one record of a 4-bit cache
 KV4_HEADS = (64, 128, 192, 256)
 MAX_TOP_LOGPROBS = 32
 # a captured call's own workspace: counters this many bytes long are cleared (the library's split
-# attention uses fewer than 256 of 128 bytes, its split logits rows fewer than 1024)
+# attention uses fewer than 256 of 128 bytes, its split logits rows fewer than 1024, its paged attention 4096 of 32)
 _CAPTURED_COUNTERS = 1 << 17
 
 
@@ -927,14 +927,14 @@ def _raw_stream(dev):
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _call_workspace(nbytes, dev):
+def _call_workspace(nbytes, dev, counters=_CAPTURED_COUNTERS):
     """(address, bytes) of the workspace of one call: the stream's, or, under graph capture, one of the graph's
-    own, so that two graphs replayed at a time never share one. The third item keeps it alive."""
+    own, its first `counters` bytes cleared, so that two graphs replayed at a time never share one. The third item keeps it alive."""
     if nbytes == 0:
         return None, 0, None
     if torch.cuda.is_current_stream_capturing():
         t = torch.empty(nbytes, dtype=torch.uint8, device=device())
-        t[:_CAPTURED_COUNTERS].zero_()
+        t[:counters].zero_()
     else:
         t = _WORKSPACE.get((dev, _raw_stream(dev)))
         if t is None or t.numel() < nbytes:
@@ -1362,7 +1362,7 @@ def verify_drafts(logits, drafts, uniforms, draft_logits=None, temperature=1.0):
             dp, dl = draft_logits.data_ptr(), ld(draft_logits)
     tokens = torch.empty(S, D + 1, dtype=torch.int32, device=dev)
     accepted = torch.empty(S, dtype=torch.int32, device=dev)
-    wp, wn, _keep = _call_workspace(_bytes(("verify", S, D, V), "miq_verify_drafts_workspace", S, D, V), dev)
+    wp, wn, _keep = _call_workspace(_bytes(("verify", S, D, V), "miq_verify_drafts_workspace", S, D, V), dev, 32 * S)
     _lib.call("miq_verify_drafts", logits.data_ptr(), dtype_code(logits), *ld(logits), drafts.data_ptr(), dp, *dl, uniforms.data_ptr(),
               None if temps is None else temps.data_ptr(), temp, tokens.data_ptr(), accepted.data_ptr(), S, D, V, wp, wn, _raw_stream(dev))
     return DraftVerdict(tokens, accepted)

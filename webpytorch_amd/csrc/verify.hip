@@ -5,12 +5,12 @@
 // passes u_D times their total. The reference draws on the host, from logits read back (`_pick`: webtorch/llm.py:1309-1336).
 //
 // Which side of a border between tokens a draw falls on must not depend on rounding: 150000 borders lie in [0, 1), so that
-// sums right to 1e-7 would give another token once in a hundred draws. Exponentials and sums are fp64 (to 3e-13; a draw is
+// sums right to 1e-7 would give another token once in a hundred draws. Exponentials and sums are fp64 (to 2e-13; a draw is
 // off once in 10^7).
 //
-// Two launches. Every row's maximum and sum of exponentials, in segments (a row's largest logit where the temperature is 0);
-// then a group of workgroups for each sequence, each of which accepts by itself, sums the weights of its chunks, and the last of
-// which to arrive finds the chunk, the thread and the index.
+// Two launches. Every row's maximum and sum of exponentials, in segments (a row's largest logit where the temperature is 0), where the
+// last segment of a sequence to arrive judges its drafts; then a group of workgroups for each sequence sums the weights of its
+// chunks, and the last of them to arrive finds the chunk, the thread and the index.
 #include <math.h>
 
 #include "attention_parts.h"
@@ -18,89 +18,122 @@
 namespace miq {
 
 constexpr int kVfThreads = 256;
-constexpr int kVfLane = 16;                        // consecutive logits a thread
-constexpr int kVfChunk = kVfThreads * kVfLane;     // logits of a chunk
+constexpr int kVfLane = 16, kVfLaneW = 8;          // logits of a chunk a thread: of a row's sums, and of the weights
+constexpr int kVfChunk = kVfThreads * kVfLane, kVfChunkW = kVfThreads * kVfLaneW;
 constexpr int kVfMaxDrafts = 32;
-constexpr int kVfMaxChunks = 1024;                 // sums of a row's chunks in LDS (a longer row's are of several rounds)
+constexpr int kVfMaxChunks = 1024;                 // sums of a row's weights (a longer row's are of several chunks each)
 constexpr int kVfSegments = 64;                    // segments of a row, at most: a lane each
-constexpr int kVfCtrStride = 8;                    // ints between arrival counters
+constexpr int kVfCtrStride = 8;                    // ints between the counters of sequences
 
-// 2^t, t <= 0: the whole part by ldexp, the rest by the series of 2^f = e^(f ln 2), |f| <= 1 / 2, to the tenth power (off by
-// 2.2e-13 at most). NaN stays NaN.
-__device__ __forceinline__ double exp2_d(double t) {
-  t = t < -1100. ? -1100. : t;
-  const double k = rint(t), f = t - k;
-  double p = 7.054911620801121e-09;  // (ln 2)^n / n!
-  p = fma(p, f, 1.0178086009239696e-07);
-  p = fma(p, f, 1.3215486790144305e-06);
-  p = fma(p, f, 1.5252733804059838e-05);
-  p = fma(p, f, 0.00015403530393381606);
-  p = fma(p, f, 0.0013333558146428441);
-  p = fma(p, f, 0.009618129107628477);
-  p = fma(p, f, 0.055504108664821576);
-  p = fma(p, f, 0.2402265069591007);
-  p = fma(p, f, 0.6931471805599453);
+// 2^(i / 256) in LDS
+constexpr int kVfPowers = 256;
+__device__ __forceinline__ void fill_powers(double* tab) {
+  tab[threadIdx.x] = exp2((double)threadIdx.x / kVfPowers);
+  __syncthreads();
+}
+// x is taken to be no further below m than 623 times the temperature (-inf among it): 2^-899, which no sum sees
+__device__ __forceinline__ float power_floor(float m, float drop) { return fmaxf(m - drop, -3.402823466e38f); }
+// c of a temperature, and the drop of its floor
+__device__ __forceinline__ double power_unit(float temperature, float& drop) {
+  drop = 623.f * temperature;
+  return kVfPowers * 1.4426950408889634 / (double)temperature;
+}
+// 2^((x - m) c / 256) added to `sum`, 1 for m itself: whole multiples of 1 / 256 by the table and the exponent, the rest, |f| <= 1 / 512, by the
+// series of e^(f ln 2) to the third power (1.4e-13). 10 fp64 instructions (a table of 32 takes 12, the series of |f| <= 1 / 2 alone 19),
+// which bound the kernel of the rows: 64 sequences of 4 drafts, fp16, 70 -> XX us.
+__device__ __forceinline__ double power_plus(float x, double m, double c, const double* tab, double sum) {
+  const double y = ((double)x - m) * c, magic = 6755399441055744.;  // 1.5 2^52: the whole part in the low word
+  const double up = y + magic, f = y - (up - magic);
+  const int k = __double2loint(up);
+  double p = 3.308302680541371e-09;  // (ln 2 / 256)^n / n!
+  p = fma(p, f, 3.665565596910106e-06);
+  p = fma(p, f, 0.0027076061740622863);
   p = fma(p, f, 1.0);
-  return ldexp(p, (int)k);
+  const double t = tab[k & (kVfPowers - 1)];
+  return fma(__hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t)), p, sum);
 }
-__device__ __forceinline__ double shfl_xor_d(double v, int d) {
-  return __hiloint2double(__shfl_xor(__double2hiint(v), d), __shfl_xor(__double2loint(v), d));
+template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ double dpp_double(double v) {  // 0 where no lane is the source
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, false),
+                          __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, false));
 }
-__device__ __forceinline__ double shfl_up_d(double v, int d) {
-  return __hiloint2double(__shfl_up(__double2hiint(v), d), __shfl_up(__double2loint(v), d));
+__device__ __forceinline__ double lane_double(double v, int l) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
+}
+// the sum over lanes 0 .. l, in a fixed order
+__device__ __forceinline__ double scan_double(double v) {
+  v += dpp_double<0x111>(v);  // row_shr 1, 2, 4, 8
+  v += dpp_double<0x112>(v);
+  v += dpp_double<0x114>(v);
+  v += dpp_double<0x118>(v);
+  v += dpp_double<0x142, 0xA>(v);  // a row's last lane to the next row: rows 1 and 3
+  return v + dpp_double<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
 }
 
 // What is known of a row, or of a part of it: its largest logit with the lowest index of it (-inf, -1: none above -inf) and the
-// sum of 2^((x - largest) c), NaN where a logit is NaN or +inf. At temperature 0 there is no sum.
+// sum of 2^((x - largest) c / 256), NaN where a logit is NaN or +inf. At temperature 0 there is no sum, otherwise no index.
 struct RowPart {
   float m;
   int at;
   double s;
 };
-__device__ __forceinline__ void row_merge(RowPart& a, float m, int at, double s, bool greedy, double c) {
+// of the parts that the lanes of a wave hold
+__device__ __forceinline__ RowPart row_of_lanes(RowPart r, bool greedy, double c, float drop, const double* tab) {
+  const float top = wave_max(r.m);
   if (greedy) {
-    if (m > a.m || (m == a.m && (uint32_t)at < (uint32_t)a.at)) a = RowPart{m, at, 0.};
-    return;
-  }
-  if (m == -INFINITY && s == 0.) return;
-  if (a.m == -INFINITY && a.s == 0.) {
-    a = RowPart{m, at, s};
-    return;
-  }
-  const float top = fmaxf(a.m, m);
-  const double fa = a.m == top ? 1. : exp2_d(((double)a.m - (double)top) * c), fb = m == top ? 1. : exp2_d(((double)m - (double)top) * c);
-  a.s = a.s * fa + s * fb;
-  a.m = top;
-}
-__device__ __forceinline__ void row_merge_wave(RowPart& r, bool greedy, double c) {
+    uint32_t at = r.m == top && r.m > -INFINITY ? (uint32_t)r.at : 0xFFFFFFFFu;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const float m = __shfl_xor(r.m, d);
-    const int at = __shfl_xor(r.at, d);
-    row_merge(r, m, at, shfl_xor_d(r.s, d), greedy, c);
+    for (int d = 1; d < 64; d *= 2) at = min(at, (uint32_t)__shfl_xor((int)at, d));
+    return RowPart{top, (int)at, 0.};
   }
+  const double s = r.m > -INFINITY ? r.s * power_plus(fmaxf(r.m, power_floor(top, drop)), top, c, tab, 0.) : r.s;  // 0 or NaN
+  return RowPart{top, -1, lane_double(scan_double(s), 63)};
 }
 
-// kVfLane consecutive logits from i on; -inf behind the row's end
-template <typename XT> __device__ __forceinline__ void load_logits(const XT* row, int i, int V, bool vec, float* v) {
-  constexpr int N = 16 / sizeof(XT);
-  if (vec && i + kVfLane <= V) {
+// A thread's N logits of a chunk of N kVfThreads from i0 on. In order: N consecutive ones; otherwise vectors (or values, where rows
+// are not aligned) of consecutive threads. -inf behind the row's end
+template <typename XT, int N> __device__ __forceinline__ int logit_at(int e, bool vec, bool in_order) {  // offset of value e in the chunk
+  constexpr int W = 16 / sizeof(XT);
+  const int tid = threadIdx.x;
+  return in_order ? N * tid + e : vec ? (e / W * kVfThreads + tid) * W + e % W : e * kVfThreads + tid;
+}
+// as they lie in memory, so that the next chunk's take few registers on their way
+template <typename XT, int N> struct Logits {
+  static constexpr int W = 16 / sizeof(XT);
+  uint32_t raw[N * sizeof(XT) / 4];
+  __device__ __forceinline__ void load(const XT* row, int64_t i0, int V, bool vec, bool in_order) {
+    if (vec && i0 + N * kVfThreads <= V) {
 #pragma unroll
-    for (int k = 0; k < kVfLane; k += N) {
-      const miq_u32x4 w = *reinterpret_cast<const miq_u32x4*>(row + i + k);
+      for (int k = 0; k < N; k += W)
+        *reinterpret_cast<miq_u32x4*>(&raw[k / W * 4]) = *reinterpret_cast<const miq_u32x4*>(row + i0 + logit_at<XT, N>(k, true, in_order));
+    } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if constexpr (N == 4)
-          v[k + e] = __uint_as_float(w[e]);
-        else
-          v[k + e] = __half2float(__ushort_as_half((unsigned short)(w[e >> 1] >> (16 * (e & 1)))));
+      for (int k = 0; k < N; ++k) {
+        const int64_t i = i0 + logit_at<XT, N>(k, vec, in_order);
+        if constexpr (W == 4) {
+          raw[k] = i < V ? __float_as_uint(row[i]) : 0xFF800000u;
+        } else {
+          const uint32_t h = i < V ? (uint32_t)__half_as_ushort(row[i]) : 0xFC00u;
+          raw[k / 2] = k & 1 ? raw[k / 2] | h << 16 : h;
+        }
       }
     }
-  } else {
-#pragma unroll
-    for (int k = 0; k < kVfLane; ++k) v[k] = i + k < V ? to_f32<XT>(row[i + k]) : -INFINITY;
   }
-}
+  __device__ __forceinline__ float operator[](int k) const {
+    if constexpr (W == 4)
+      return __uint_as_float(raw[k]);
+    else
+      return __half2float(__ushort_as_half((unsigned short)(raw[k >> 1] >> (16 * (k & 1)))));
+  }
+};
+
+// What a sequence's judgement leaves for its draw
+struct Verdict {
+  int n, token;                 // drafts accepted; the token, or kVfDraw
+  int refused, without;         // draft n was refused; the token that p lacks (-1: none)
+  float tmax, dmax;             // of the target's row n, and of the draft's
+  double ti, di;                // 1 / sums; di 0: nothing is taken off p
+};
+constexpr int kVfDraw = -2;
 
 struct VerifyArgs {
   const void* logits;      // [S][D + 1] rows
@@ -112,45 +145,66 @@ struct VerifyArgs {
   float temp;
   int32_t* tokens;         // [S][D + 1]
   int32_t* accepted;       // [S]
-  int S, D, V, segs, groups, rounds;  // segments of a row, workgroups of a sequence, rounds of 4096 logits a sum
+  int S, D, V, segs, groups, rounds;  // segments of a row, workgroups of a sequence, chunks a sum of weights
   int lvec, dvec;
   uint64_t* parts;         // [rows][segs][2]
   double* sums;            // [S][kVfMaxChunks]
-  int* counters;           // [S]
+  Verdict* verdicts;       // [S]
+  int* counters;           // [S][kVfCtrStride]: parts of rows, groups of weights
 };
-__device__ __forceinline__ float temperature(const VerifyArgs& a, int s) { return a.temps ? a.temps[s] : a.temp; }
-// drafts of sequence s: those ahead of the first id below 0 (a wave's 64 lanes call)
-__device__ __forceinline__ int drafts_of(const VerifyArgs& a, int s) {
-  const int lane = threadIdx.x & 63;
-  return __builtin_ctzll(__ballot(lane >= a.D || a.ids[(int64_t)s * a.D + lane] < 0));
+// 0 for what is no finite number above 0
+__device__ __forceinline__ float temperature(const VerifyArgs& a, int s) {
+  const float t = a.temps ? a.temps[s] : a.temp;
+  return t > 0.f && t < INFINITY ? t : 0.f;
+}
+__device__ __forceinline__ void answer(const VerifyArgs& a, int s, int n, int token) {  // by one thread
+  int32_t* o = a.tokens + (int64_t)s * (a.D + 1);
+  for (int i = 0; i <= a.D; ++i) o[i] = i < n ? a.ids[(int64_t)s * a.D + i] : i == n ? token : -1;
+  a.accepted[s] = n;
 }
 
-// Segment blockIdx.x of row blockIdx.y: the S (D + 1) target rows, then the S D draft rows.
+// Segment blockIdx.x of row blockIdx.y: the S (D + 1) target rows, then the S D draft rows. The last segment of a sequence's rows to
+// arrive judges its drafts.
 template <typename XT>
 __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
-  __shared__ RowPart waves[kVfThreads / 64];
-  const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, rows = a.S * (a.D + 1);
+  __shared__ RowPart waves[kVfThreads / 64], trow[kVfMaxDrafts + 1], drow[kVfMaxDrafts];
+  __shared__ double tab[kVfPowers];
+  __shared__ int last;
+  const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rows = a.S * (a.D + 1), D = a.D;
   const bool target = row < rows;
-  const int s = target ? row / (a.D + 1) : (row - rows) / a.D, i = target ? row % (a.D + 1) : (row - rows) % a.D;
+  const int s = target ? row / (D + 1) : (row - rows) / D, i = target ? row % (D + 1) : (row - rows) % D;
   const float temp = temperature(a, s);
-  const bool greedy = !(temp > 0.f);
+  const bool greedy = !(temp > 0.f), dist = a.drafted && !greedy;
   if (!target && greedy) return;
-  if (drafts_of(a, s) < (target ? i : i + 1)) return;  // behind the last draft: not looked at
-  const XT* x = target ? static_cast<const XT*>(a.logits) + s * a.ls + i * a.lr : static_cast<const XT*>(a.drafted) + s * a.ds + i * a.dr;
+  const XT* const tl = static_cast<const XT*>(a.logits) + s * a.ls;
+  const XT* const dl = static_cast<const XT*>(a.drafted) + s * a.ds;
+  const XT* x = target ? tl + i * a.lr : dl + i * a.dr;
   const bool vec = target ? a.lvec : a.dvec;
-  const double c = 1.4426950408889634 / (double)temp;
-  const int chunks = (a.V + kVfChunk - 1) / kVfChunk;
+  const int chunks = (int)(((int64_t)a.V + kVfChunk - 1) / kVfChunk);
+  Logits<XT, kVfLane> next;
+  next.load(x, (int64_t)seg * kVfChunk, a.V, vec, false);
+  // lane i has draft i, its logits and its random number: for the judgement, on the way from here on
+  const int id = lane < D ? a.ids[(int64_t)s * D + lane] : -1;
+  const int drafts = __builtin_ctzll(__ballot(id < 0));  // those ahead of the first id below 0
+  if (drafts < (target ? i : i + 1)) return;  // behind the last draft: not looked at
+  const bool inside = lane < drafts && id < a.V;
+  const float tx = inside ? to_f32<XT>(tl[lane * a.lr + id]) : 0.f, dx = inside && dist ? to_f32<XT>(dl[lane * a.dr + id]) : 0.f;
+  const float ux = lane < drafts ? a.uniforms[(int64_t)s * (D + 1) + lane] : 0.f;
+  float drop;
+  const double c = power_unit(temp, drop);
+  fill_powers(tab);
   RowPart r = {-INFINITY, -1, 0.};
+  double top = 0.;
+  float floor = 0.f;
   for (int ch = seg; ch < chunks; ch += a.segs) {
-    float v[kVfLane];
-    const int at = ch * kVfChunk + tid * kVfLane;
-    load_logits<XT>(x, at, a.V, vec, v);
+    const Logits<XT, kVfLane> v = next;
+    if (ch + a.segs < chunks) next.load(x, (int64_t)(ch + a.segs) * kVfChunk, a.V, vec, false);
     if (greedy) {
 #pragma unroll
       for (int k = 0; k < kVfLane; ++k)
         if (v[k] > r.m) {
           r.m = v[k];
-          r.at = at + k;
+          r.at = ch * kVfChunk + logit_at<XT, kVfLane>(k, vec, false);
         }
       continue;
     }
@@ -162,50 +216,85 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
       bad = bad || !(v[k] < INFINITY);
     }
     if (mx > r.m) {
-      r.s *= r.m == -INFINITY ? 0. : exp2_d(((double)r.m - (double)mx) * c);
+      r.s = r.m == -INFINITY ? r.s : r.s * power_plus(fmaxf(r.m, power_floor(mx, drop)), mx, c, tab, 0.);
       r.m = mx;
+      top = mx;
+      floor = power_floor(mx, drop);
     }
     if (bad) r.s = NAN;
     if (r.m > -INFINITY) {
 #pragma unroll
-      for (int k = 0; k < kVfLane; ++k) r.s += exp2_d(((double)v[k] - (double)r.m) * c);
+      for (int k = 0; k < kVfLane; ++k) r.s = power_plus(fmaxf(v[k], floor), top, c, tab, r.s);
     }
   }
-  row_merge_wave(r, greedy, c);
-  if ((tid & 63) == 0) waves[tid >> 6] = r;
+  r = row_of_lanes(r, greedy, c, drop, tab);
+  if (lane == 0) waves[wave] = r;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kVfThreads / 64; ++w) row_merge(r, waves[w].m, waves[w].at, waves[w].s, greedy, c);
-    uint64_t* o = a.parts + ((int64_t)row * a.segs + seg) * 2;
-    o[0] = (uint64_t)__float_as_uint(r.m) | ((uint64_t)(uint32_t)r.at << 32);
-    o[1] = (uint64_t)__double_as_longlong(r.s);
+  if (wave == 0) {
+    r = row_of_lanes(tid < kVfThreads / 64 ? waves[tid] : RowPart{-INFINITY, -1, 0.}, greedy, c, drop, tab);
+    if (tid == 0) {
+      uint64_t* o = a.parts + ((int64_t)row * a.segs + seg) * 2;
+      __hip_atomic_store(o, (uint64_t)__float_as_uint(r.m) | ((uint64_t)(uint32_t)r.at << 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(o + 1, (uint64_t)__double_as_longlong(r.s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
   }
-}
+  const int all = drafts + 1 + (dist ? drafts : 0);  // rows that are looked at
+  if (!last_slice(a.counters + s * kVfCtrStride, all * a.segs, &last)) return;
 
-// The whole row from its segments, by one wave
-__device__ __forceinline__ RowPart row_of(const uint64_t* parts, int segs, bool greedy, double c) {
-  const int lane = threadIdx.x & 63;
-  RowPart r = {-INFINITY, -1, 0.};
-  if (lane < segs) {
-    const uint64_t w = parts[2 * lane];
-    r = RowPart{__uint_as_float((uint32_t)w), (int)(w >> 32), __longlong_as_double((long long)parts[2 * lane + 1])};
+  // ---- the judgement: lane i of wave 0 has draft i ----
+  constexpr int U = 4;  // the target's rows, then the draft's: a wave U at a time, a lane a segment
+  for (int k0 = wave * U; k0 < all; k0 += kVfThreads / 64 * U) {
+    uint64_t w[U][2];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int k = min(k0 + j, all - 1);
+      const int64_t at = k <= drafts ? (int64_t)s * (D + 1) + k : rows + (int64_t)s * D + k - drafts - 1;
+      uint64_t* p = a.parts + (at * a.segs + min(lane, a.segs - 1)) * 2;
+      w[j][0] = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      w[j][1] = __hip_atomic_load(p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      RowPart one = {-INFINITY, -1, 0.};
+      if (lane < a.segs) one = RowPart{__uint_as_float((uint32_t)w[j][0]), (int)(w[j][0] >> 32), __longlong_as_double((long long)w[j][1])};
+      one = row_of_lanes(one, greedy, c, drop, tab);
+      const int k = k0 + j;
+      if (lane == 0 && k < all) (k <= drafts ? trow[k] : drow[k - drafts - 1]) = one;
+    }
   }
-  row_merge_wave(r, greedy, c);
-  return r;
+  __syncthreads();
+  if (wave != 0) return;
+  bool ok = false;
+  if (lane < drafts) {
+    if (greedy) {
+      ok = id == trow[lane].at;
+    } else if (inside && trow[lane].s > 0.) {  // a row without a distribution (NaN, or nothing above -inf) accepts nothing
+      // down to fp64's least numbers, where both sides are small
+      const double p = exp2(((double)tx - (double)trow[lane].m) * c / kVfPowers) / trow[lane].s;
+      double q = 1.;
+      if (dist) q = drow[lane].s > 0. ? exp2(((double)dx - (double)drow[lane].m) * c / kVfPowers) / drow[lane].s : (double)NAN;
+      ok = (double)ux * q < p;
+    }
+  }
+  const int n = __builtin_ctzll(__ballot(!ok));  // lanes from `drafts` on say no
+  const int refusal = __builtin_amdgcn_readlane(id, n);
+  if (lane != 0) return;
+  const bool refused = n < drafts, law = greedy ? trow[n].at >= 0 : trow[n].s > 0.;  // law: the row is a distribution
+  Verdict v = {n, greedy || !law ? (law ? trow[n].at : -1) : kVfDraw, refused, refused && !dist ? refusal : -1, trow[n].m, 0.f,
+               1. / trow[n].s, 0.};
+  if (refused && dist && drow[n].s > 0.) {  // max(p - q, 0)
+    v.dmax = drow[n].m;
+    v.di = 1. / drow[n].s;
+  }
+  a.verdicts[s] = v;
+  if (v.token != kVfDraw) answer(a, s, n, v.token);
 }
 
 // Exclusive sum of v over the workgroup's threads, in their order; all is the sum of them all
 __device__ __forceinline__ double sums_before(double v, double* waves, double& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const double o = shfl_up_d(x, d);
-    if (lane >= d) x += o;
-  }
-  if (lane == 63) waves[wave] = x;
-  double before = shfl_up_d(x, 1);
-  if (lane == 0) before = 0.;
+  const int wave = threadIdx.x >> 6;
+  const double x = scan_double(v);
+  if ((threadIdx.x & 63) == 63) waves[wave] = x;
   __syncthreads();
   double w = 0.;
   all = 0.;
@@ -215,191 +304,189 @@ __device__ __forceinline__ double sums_before(double v, double* waves, double& a
     all += waves[k];
   }
   __syncthreads();
-  return w + before;
+  return w + (x - v);
 }
 
 template <typename XT>
 __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) {
-  __shared__ float tm[kVfMaxDrafts + 1], dm[kVfMaxDrafts];
-  __shared__ double ts[kVfMaxDrafts + 1], dsum[kVfMaxDrafts], waves[kVfThreads / 64], list[kVfMaxChunks];
-  __shared__ int tat[kVfMaxDrafts + 1], verdict[2], last, found;
-  const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = a.D;
-  const float temp = temperature(a, s);
-  const bool greedy = !(temp > 0.f), dist = a.drafted && !greedy;
-  const double c = 1.4426950408889634 / (double)temp;
-  const int32_t* ids = a.ids + (int64_t)s * D;
-  const float* u = a.uniforms + (int64_t)s * (D + 1);
-  const int drafts = drafts_of(a, s);
-  for (int i = wave; i <= drafts; i += kVfThreads / 64) {
-    const RowPart r = row_of(a.parts + ((int64_t)s * (D + 1) + i) * a.segs * 2, a.segs, greedy, c);
-    if (lane == 0) {
-      tm[i] = r.m;
-      ts[i] = r.s;
-      tat[i] = r.at;
-    }
-  }
-  if (dist)
-    for (int i = wave; i < drafts; i += kVfThreads / 64) {
-      const RowPart r = row_of(a.parts + ((int64_t)a.S * (D + 1) + (int64_t)s * D + i) * a.segs * 2, a.segs, false, c);
-      if (lane == 0) {
-        dm[i] = r.m;
-        dsum[i] = r.s;
-      }
-    }
-  __syncthreads();
-  const XT* const tl = static_cast<const XT*>(a.logits) + s * a.ls;
-  const XT* const dl = dist ? static_cast<const XT*>(a.drafted) + s * a.ds : nullptr;
-  if (wave == 0) {  // lane i judges draft i
-    bool ok = false;
-    if (lane < drafts) {
-      const int x = ids[lane];
-      if (greedy) {
-        ok = x == tat[lane];
-      } else if (x < a.V && ts[lane] > 0.) {  // a row without a distribution (NaN, or nothing above -inf) accepts nothing
-        const double p = exp2_d(((double)to_f32<XT>(tl[lane * a.lr + x]) - (double)tm[lane]) * c) / ts[lane];
-        double q = 1.;
-        if (dist) q = dsum[lane] > 0. ? exp2_d(((double)to_f32<XT>(dl[lane * a.dr + x]) - (double)dm[lane]) * c) / dsum[lane] : NAN;
-        ok = (double)u[lane] * q < p;
-      }
-    }
-    const uint64_t no = __ballot(!ok);  // lanes from `drafts` on among them
-    if (lane == 0) verdict[0] = __builtin_ctzll(no);
-  }
-  __syncthreads();
-  const int n = verdict[0];
-  const bool refused = n < drafts;
-  const bool law = greedy ? tat[n] >= 0 : ts[n] > 0.;  // the row is a distribution
-  auto answer = [&](int token) {  // by one thread
-    int32_t* o = a.tokens + (int64_t)s * (D + 1);
-    for (int i = 0; i <= D; ++i) o[i] = i < n ? ids[i] : i == n ? token : -1;
-    a.accepted[s] = n;
+  __shared__ double waves[kVfThreads / 64], tab[kVfPowers], found_before;
+  __shared__ int verdict[2], last;
+  const int s = blockIdx.y, tid = threadIdx.x, D = a.D;
+  const Verdict j = a.verdicts[s];
+  float drop;
+  const double c = power_unit(temperature(a, s), drop), ulast = a.uniforms[(int64_t)s * (D + 1) + D];
+  fill_powers(tab);
+  if (j.token != kVfDraw) return;
+  const bool minus = j.di > 0.;
+  const XT* const trow = static_cast<const XT*>(a.logits) + s * a.ls + j.n * a.lr;
+  const XT* const drow = minus ? static_cast<const XT*>(a.drafted) + s * a.ds + j.n * a.dr : nullptr;
+  const bool vec = a.lvec && (!minus || a.dvec);  // both rows in one order
+  const double tmax = j.tmax, dmax = j.dmax;
+  const float tfloor = power_floor(j.tmax, drop), dfloor = power_floor(j.dmax, drop);
+  struct Chunk {
+    Logits<XT, kVfLaneW> t, d;
   };
-  if (greedy || !law) {
-    if (blockIdx.x == 0 && tid == 0) answer(law ? tat[n] : -1);
-    return;
-  }
-  // ---- weights ----
-  const XT* const trow = tl + n * a.lr;
-  const bool minus = refused && dist && dsum[n] > 0.;   // max(p - q, 0)
-  const int without = refused && !dist ? ids[n] : -1;   // p but for the draft
-  const XT* const drow = minus ? dl + n * a.dr : nullptr;
-  const double tmax = tm[n], ti = 1. / ts[n], dmax = minus ? dm[n] : 0., di = minus ? 1. / dsum[n] : 0.;
-  auto weights = [&](int at, double* w) __attribute__((always_inline)) {
-    float v[kVfLane];
-    load_logits<XT>(trow, at, a.V, a.lvec, v);
+  auto load = [&](Chunk& x, int64_t i0, bool in_order) __attribute__((always_inline)) {
+    x.t.load(trow, i0, a.V, vec, in_order);
+    if (minus) x.d.load(drow, i0, a.V, vec, in_order);
+  };
+  auto weights = [&](const Chunk& x, int64_t i0, bool in_order, double* w) __attribute__((always_inline)) {
+    const Logits<XT, kVfLaneW>&v = x.t, &q = x.d;
 #pragma unroll
-    for (int k = 0; k < kVfLane; ++k) w[k] = exp2_d(((double)v[k] - tmax) * c) * ti;
+    for (int k = 0; k < kVfLaneW; ++k) w[k] = v[k] == -INFINITY ? 0. : power_plus(fmaxf(v[k], tfloor), tmax, c, tab, 0.) * j.ti;
     if (minus) {
-      load_logits<XT>(drow, at, a.V, a.dvec, v);
 #pragma unroll
-      for (int k = 0; k < kVfLane; ++k) {
-        const double d = w[k] - exp2_d(((double)v[k] - dmax) * c) * di;
-        w[k] = d > 0. ? d : 0.;
-      }
+      for (int k = 0; k < kVfLaneW; ++k)
+        w[k] = fmax(q[k] == -INFINITY ? w[k] : w[k] - power_plus(fmaxf(q[k], dfloor), dmax, c, tab, 0.) * j.di, 0.);
     }
-    if (without >= at && without < at + kVfLane)
+    if (j.without >= i0 && j.without < i0 + kVfChunkW)
 #pragma unroll
-      for (int k = 0; k < kVfLane; ++k)
-        if (at + k == without) w[k] = 0.;
+      for (int k = 0; k < kVfLaneW; ++k)
+        if (i0 + logit_at<XT, kVfLaneW>(k, vec, in_order) == j.without) w[k] = 0.;
     double sum = 0.;
 #pragma unroll
-    for (int k = 0; k < kVfLane; ++k) sum += w[k];
+    for (int k = 0; k < kVfLaneW; ++k) sum += w[k];
     return sum;
   };
-  const int span = a.rounds * kVfChunk, chunks = (int)(((int64_t)a.V + span - 1) / span);
+  const int span = a.rounds * kVfChunkW, chunks = (int)(((int64_t)a.V + span - 1) / span);
   double* const sums = a.sums + (int64_t)s * kVfMaxChunks;
+  // this workgroup's chunks, span after span of them: the next one is loaded while one is added up
+  auto start = [&](int ch, int k) __attribute__((always_inline)) { return (int64_t)ch * span + k * kVfChunkW; };
+  Chunk next;
+  load(next, start(blockIdx.x, 0), false);
   for (int ch = blockIdx.x; ch < chunks; ch += a.groups) {
-    double total = 0.;
+    double mine = 0., all;
     for (int k = 0; k < a.rounds; ++k) {
-      const int64_t at = (int64_t)ch * span + k * kVfChunk + tid * kVfLane;
-      double w[kVfLane], all;
-      const double mine = at < a.V ? weights((int)at, w) : 0.;
-      sums_before(mine, waves, all);
-      total += all;
+      const Chunk x = next;
+      if (k + 1 < a.rounds)
+        load(next, start(ch, k + 1), false);
+      else if (ch + a.groups < chunks)
+        load(next, start(ch + a.groups, 0), false);
+      double w[kVfLaneW];
+      mine += weights(x, start(ch, k), false, w);
     }
+    sums_before(mine, waves, all);
     if (tid == 0)
-      __hip_atomic_store(reinterpret_cast<uint64_t*>(sums + ch), (uint64_t)__double_as_longlong(total), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(reinterpret_cast<uint64_t*>(sums + ch), (uint64_t)__double_as_longlong(all), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (a.groups > 1) {
-    if (!last_slice(a.counters + s * kVfCtrStride, a.groups, &last)) return;
+    if (!last_slice(a.counters + s * kVfCtrStride + 1, a.groups, &last)) return;
   } else {
     parts_stored();
     __syncthreads();
   }
   // ---- the last to arrive: the first index whose running sum passes u times the total ----
-  for (int ch = tid; ch < chunks; ch += kVfThreads)
-    list[ch] = __longlong_as_double((long long)__hip_atomic_load(reinterpret_cast<uint64_t*>(sums + ch), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-  if (tid == 0) found = -1;
-  __syncthreads();
-  double total = 0.;
-  int heavy = -1;  // the last chunk with any weight
-  for (int ch = 0; ch < chunks; ++ch) {
-    total += list[ch];
-    if (list[ch] > 0.) heavy = ch;
-  }
-  if (heavy < 0) {  // the target leaves nothing beside the draft, or the two are the same
-    if (tid == 0) answer(refused && ids[n] < a.V ? ids[n] : -1);
-    return;
-  }
-  const double want = (double)u[D] * total;
-  double before = 0.;
-  int ch = 0;
-  for (; ch < heavy; ++ch) {
-    if (before + list[ch] > want) break;
-    before += list[ch];
-  }
-  for (int k = 0; k < a.rounds; ++k) {
-    const int64_t at = (int64_t)ch * span + k * kVfChunk + tid * kVfLane;
-    double w[kVfLane], all;
-    const double mine = at < a.V ? weights((int)at, w) : 0.;
-    double run = before + sums_before(mine, waves, all);
-    int hit = -1, any = -1;
-    if (mine > 0.) {
+  // the chunk: each thread has some of them, in order
+  constexpr int kEach = kVfMaxChunks / kVfThreads;
+  double part[kEach], mine = 0., total;
 #pragma unroll
-      for (int i = 0; i < kVfLane; ++i) {
-        run += w[i];
-        if (w[i] > 0.) any = (int)at + i;
-        if (w[i] > 0. && run > want && hit < 0) hit = (int)at + i;
+  for (int k = 0; k < kEach; ++k) {
+    const int ch = tid * kEach + k;
+    part[k] = ch < chunks ? __longlong_as_double((long long)__hip_atomic_load(reinterpret_cast<uint64_t*>(sums + ch), __ATOMIC_RELAXED,
+                                                                              __HIP_MEMORY_SCOPE_AGENT))
+                          : 0.;
+    mine += part[k];
+  }
+  if (tid == 0) {
+    verdict[0] = 0x7FFFFFFF;
+    verdict[1] = -1;
+  }
+  double run = sums_before(mine, waves, total);  // its barriers lie between the marks and what follows
+  const double want = ulast * total;
+  int hit = -1, heavy = -1;  // the first chunk past it; the last with any weight
+  double at_hit = 0., at_heavy = 0.;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    if (part[k] > 0.) {
+      heavy = tid * kEach + k;
+      at_heavy = run;
+      if (hit < 0 && run + part[k] > want) {
+        hit = heavy;
+        at_hit = run;
       }
     }
-    // the first hit; where rounding leaves none, the last index of the chunk with any weight
+    run += part[k];
+  }
+  if (hit >= 0) atomicMin(&verdict[0], hit);
+  if (heavy >= 0) atomicMax(&verdict[1], heavy);
+  __syncthreads();
+  const int ch = verdict[0] != 0x7FFFFFFF ? verdict[0] : verdict[1];
+  if (ch < 0) {  // the target leaves nothing beside the draft, or the two are the same
+    if (tid == 0) {
+      const int id = j.refused ? a.ids[(int64_t)s * D + j.n] : -1;
+      answer(a, s, j.n, id < a.V ? id : -1);
+    }
+    return;
+  }
+  if (hit == ch)
+    found_before = at_hit;
+  else if (heavy == ch && verdict[0] == 0x7FFFFFFF)
+    found_before = at_heavy;
+  __syncthreads();
+  double before = found_before;
+  int fallback = -1;
+  for (int k = 0; k < a.rounds; ++k) {
+    const int64_t i0 = (int64_t)ch * span + k * kVfChunkW;
+    double w[kVfLaneW], all;
     if (tid == 0) {
       verdict[0] = 0x7FFFFFFF;
       verdict[1] = -1;
     }
-    __syncthreads();
+    Chunk x;
+    load(x, i0, true);
+    const double mine = weights(x, i0, true, w);
+    double run = before + sums_before(mine, waves, all);
+    int hit = -1, any = -1;
+#pragma unroll
+    for (int i = 0; i < kVfLaneW; ++i) {
+      run += w[i];
+      if (w[i] > 0.) {
+        any = (int)i0 + kVfLaneW * tid + i;
+        if (run > want && hit < 0) hit = any;
+      }
+    }
+    // the first hit; where rounding leaves none, the last index of the chunk with any weight
     if (hit >= 0) atomicMin(&verdict[0], hit);
     if (any >= 0) atomicMax(&verdict[1], any);
     __syncthreads();
     const int first = verdict[0];
-    if (first != 0x7FFFFFFF) {
-      if (tid == 0) answer(first);
+    if (verdict[1] >= 0) fallback = verdict[1];
+    if (first != 0x7FFFFFFF || k == a.rounds - 1) {
+      if (tid == 0) answer(a, s, j.n, first != 0x7FFFFFFF ? first : fallback);
       return;
     }
-    if (tid == 0 && verdict[1] >= 0) found = verdict[1];
     before += all;
     __syncthreads();
   }
-  if (tid == 0) answer(found);
 }
 
 struct VerifyPlan {
   int segs, groups, rounds;
-  size_t parts, sums;
+  size_t parts, sums, verdicts;
 };
-// Segments of a row that give every CU several workgroups; workgroups of a sequence likewise.
-static VerifyPlan verify_plan(int S, int D, int V) {
+// Segments of a row: four workgroups a CU run at once, one after another takes as long as its chunks and some 4 more (start and sums).
+// (24 sequences of 6 drafts, fp16, V 32003: 7 segments, 1176 workgroups, 20.4 us; 6, which fit at once, XX.) Workgroups of a sequence's
+// weights: likewise at once.
+static VerifyPlan verify_plan(int S, int D, int V, bool dist) {
   VerifyPlan p;
-  const int chunks = (int)(((int64_t)V + kVfChunk - 1) / kVfChunk);
-  const int64_t rows = (int64_t)S * (2 * D + 1);
-  int64_t segs = (8 * kCUs + rows - 1) / rows, groups = (4 * kCUs + S - 1) / S;
-  p.rounds = (chunks + kVfMaxChunks - 1) / kVfMaxChunks;
-  const int spans = (chunks + p.rounds - 1) / p.rounds;
-  if (segs > chunks) segs = chunks;
-  p.segs = (int)(segs > kVfSegments ? kVfSegments : segs);
-  p.groups = (int)(groups > spans ? spans : groups);
+  const int chunks = (int)(((int64_t)V + kVfChunk - 1) / kVfChunk), most = chunks < kVfSegments ? chunks : kVfSegments;
+  const int64_t rows = (int64_t)S * (dist ? 2 * D + 1 : D + 1);
+  p.segs = 1;
+  int64_t best = INT64_MAX;
+  for (int s = 1; s <= most; ++s) {
+    const int64_t cost = (rows * s + 4 * kCUs - 1) / (4 * kCUs) * ((chunks + s - 1) / s + 4);
+    if (cost < best) {
+      best = cost;
+      p.segs = s;
+    }
+  }
+  const int wchunks = (int)(((int64_t)V + kVfChunkW - 1) / kVfChunkW);
+  p.rounds = (wchunks + kVfMaxChunks - 1) / kVfMaxChunks;
+  const int spans = (wchunks + p.rounds - 1) / p.rounds, groups = (4 * kCUs + S - 1) / S;
+  p.groups = groups > spans ? spans : groups;
   p.parts = (size_t)rows * p.segs * 16;
   p.sums = (size_t)S * kVfMaxChunks * 8;
+  p.verdicts = (size_t)S * sizeof(Verdict);
   return p;
 }
 
@@ -419,8 +506,8 @@ extern "C" int miq_verify_drafts_workspace(int S, int D, int V, size_t* bytes) {
   if (int rc = check_verify("verify_drafts_workspace", S, D, V)) return rc;
   *bytes = 0;
   if (S == 0) return MIQ_OK;
-  const VerifyPlan p = verify_plan(S, D, V);
-  *bytes = kCounterBytes + p.parts + p.sums;
+  const VerifyPlan p = verify_plan(S, D, V, true), q = verify_plan(S, D, V, false);  // with and without draft rows
+  *bytes = kCounterBytes + (p.parts > q.parts ? p.parts : q.parts) + p.sums + p.verdicts;
   return MIQ_OK;
 }
 
@@ -438,8 +525,8 @@ extern "C" int miq_verify_drafts(const void* logits, int x_dtype, int64_t ld_seq
   MIQ_REQUIRE(logits && (drafts || D == 0) && uniforms && tokens && accepted, MIQ_ERR_INVALID, "verify_drafts: null pointer");
   const int size = x_dtype == MIQ_F32 ? 4 : 2;
   MIQ_REQUIRE(aligned(logits, size) && (!dist || aligned(draft_logits, size)), MIQ_ERR_ALIGN, "verify_drafts: logits must be aligned to their type");
-  const VerifyPlan p = verify_plan(S, D, V);
-  const size_t need = kCounterBytes + p.parts + p.sums;
+  const VerifyPlan p = verify_plan(S, D, V, dist);
+  const size_t need = kCounterBytes + p.parts + p.sums + p.verdicts;
   MIQ_REQUIRE(workspace && ws_bytes >= need, MIQ_ERR_INVALID, "verify_drafts: workspace of %zu bytes, %zu needed", workspace ? ws_bytes : (size_t)0,
               need);
   MIQ_REQUIRE(aligned(workspace, 256), MIQ_ERR_ALIGN, "verify_drafts: the workspace must be 256-byte aligned");
@@ -467,6 +554,7 @@ extern "C" int miq_verify_drafts(const void* logits, int x_dtype, int64_t ld_seq
   a.counters = static_cast<int*>(workspace);
   a.parts = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + kCounterBytes);
   a.sums = reinterpret_cast<double*>(static_cast<char*>(workspace) + kCounterBytes + p.parts);
+  a.verdicts = reinterpret_cast<Verdict*>(static_cast<char*>(workspace) + kCounterBytes + p.parts + p.sums);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   // the second launch reads what the first left in the workspace: another thread's call on the stream waits
   std::unique_lock<std::mutex> whole(stream_lock(st));
