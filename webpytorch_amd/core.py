@@ -906,7 +906,7 @@ def _gpu_of(name, t):
     d = t.get_device() if isinstance(t, torch.Tensor) else -1
     if d < 0:
         raise ValueError("%s must be a torch tensor on the GPU" % name)
-    if d != torch.cuda.current_device():
+    if d != torch._C._cuda_getDevice():  # without torch.cuda's check that it is initialised, which a tensor on a GPU shows
         raise ValueError("%s is on cuda:%d, the current device is cuda:%d" % (name, d, torch.cuda.current_device()))
     return d
 
@@ -1172,16 +1172,18 @@ def _rope_arg(rope, hd, dev):
     cos, sin, pairs = rope
     for name, t in (("cos", cos), ("sin", sin)):
         _check_tensor(name, t, (torch.float32,), 2, dev)
-        if t.shape != cos.shape or not 2 <= 2 * t.shape[1] <= hd or t.shape[0] < 1 or not t.is_contiguous():
-            raise ValueError("cos and sin are two contiguous (positions, rot / 2) tables, rot at most %d: got %s and %s"
-                             % (hd, tuple(cos.shape), tuple(sin.shape)))
-    return cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], int(bool(pairs))
+    shape = cos.shape
+    rows, half = shape
+    if sin.shape != shape or not 1 <= half <= hd // 2 or rows < 1 or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("cos and sin are two contiguous (positions, rot / 2) tables, rot at most %d: got %s and %s"
+                         % (hd, tuple(shape), tuple(sin.shape)))
+    return cos.data_ptr(), sin.data_ptr(), rows, 2 * half, 1 if pairs else 0
 
 
 def _int32(name, t, shape, dev):
     """A contiguous int32 tensor of this shape."""
     _check_tensor(name, t, (torch.int32,), len(shape), dev)
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError("%s has shape %s: %s is expected" % (name, tuple(t.shape), tuple(shape)))
     return t if t.is_contiguous() else t.contiguous()
 
@@ -1200,18 +1202,23 @@ def rope(x, positions, rope, transpose=False, out=None):
     cp, sp, rows, rot, pairs = _rope_arg(rope, hd, dev)
     positions = _int32("positions", positions, (T,), dev)
     same = out is x
-    if x.stride(2) != 1 or (H > 1 and x.stride(1) < hd) or (T > 1 and x.stride(0) < hd):
+    lt, lh, one = x.stride()
+    if one != 1 or (H > 1 and lh < hd) or (T > 1 and lt < hd):
         if same:
             raise ValueError("x is rotated in place where its heads are contiguous and apart: strides %s" % (x.stride(),))
         x = x.contiguous()
+        lt, lh, one = x.stride()
     if out is None:
-        out = torch.empty(T, H, hd, dtype=x.dtype, device=dev)
-    elif not same:
-        _check_tensor("out", out, (x.dtype,), 3, dev)
-        if out.shape != x.shape or (out.numel() and out.stride(2) != 1):
-            raise ValueError("out has shape %s, strides %s: %s with contiguous heads is expected" % (tuple(out.shape), out.stride(), tuple(x.shape)))
-    _lib.call("miq_rope", x.data_ptr(), dtype_code(x), x.stride(0), x.stride(1), positions.data_ptr(), cp, sp, rows, rot, pairs,
-              int(bool(transpose)), out.data_ptr(), out.stride(0), out.stride(1), T, H, hd, _raw_stream(dev))
+        out = x.new_empty((T, H, hd))
+        ot, oh = H * hd, hd
+    else:
+        if not same:
+            _check_tensor("out", out, (x.dtype,), 3, dev)
+            if out.shape != x.shape or (out.numel() and out.stride(2) != 1):
+                raise ValueError("out has shape %s, strides %s: %s with contiguous heads is expected" % (tuple(out.shape), out.stride(), tuple(x.shape)))
+        ot, oh = out.stride(0), out.stride(1)
+    _lib.call("miq_rope", x.data_ptr(), dtype_code(x), lt, lh, positions.data_ptr(), cp, sp, rows, rot, pairs, 1 if transpose else 0,
+              out.data_ptr(), ot, oh, T, H, hd, _raw_stream(dev))
     return out
 
 
@@ -1255,7 +1262,7 @@ def paged_append(qkv, positions, pages, cache, n_heads, rope=None, qn=None, kn=N
     _check_tensor("qkv", qkv, (torch.float32, torch.float16), 3, dev)
     num, nkv, page, hd, positions, pages = _paged(cache, positions, pages, dev)
     S, T, W = qkv.shape
-    if tuple(positions.shape) != (S, T):
+    if positions.shape != (S, T):
         raise ValueError("positions %s of qkv %s" % (tuple(positions.shape), tuple(qkv.shape)))
     if n_heads < 0 or W != (n_heads + 2 * nkv) * hd:
         raise ValueError("rows of %d values are not %d query, %d key and %d value heads of %d" % (W, n_heads, nkv, nkv, hd))
@@ -1266,17 +1273,20 @@ def paged_append(qkv, positions, pages, cache, n_heads, rope=None, qn=None, kn=N
             if t.shape[0] != hd or not t.is_contiguous():
                 raise ValueError("%s has shape %s: (%d,) is expected" % (name, tuple(t.shape), hd))
     # rows of one distance
-    ld = qkv.stride(1) if T > 1 else qkv.stride(0) if S > 1 else W
-    if qkv.stride(2) != 1 or ld < W or (S > 1 and T > 1 and qkv.stride(0) != T * ld):
-        qkv = qkv.contiguous()
+    if qkv.is_contiguous():
         ld = W
+    else:
+        ld = qkv.stride(1) if T > 1 else qkv.stride(0) if S > 1 else W
+        if qkv.stride(2) != 1 or ld < W or (S > 1 and T > 1 and qkv.stride(0) != T * ld):
+            qkv = qkv.contiguous()
+            ld = W
     if out is None:
-        out = torch.empty(S, T, n_heads, hd, dtype=qkv.dtype, device=dev)
+        out = qkv.new_empty((S, T, n_heads, hd))
     else:
         _check_tensor("out", out, (qkv.dtype,), None, dev)
         if out.numel() != S * T * n_heads * hd or not out.is_contiguous():
             raise ValueError("out is a contiguous tensor of %d values: got %s" % (S * T * n_heads * hd, tuple(out.shape)))
-    qp, kp = (None if t is None else t.data_ptr() for t in (qn, kn))
+    qp, kp = None if qn is None else qn.data_ptr(), None if kn is None else kn.data_ptr()
     _lib.call("miq_paged_append", qkv.data_ptr(), dtype_code(qkv), ld, qp, kp, float(eps), positions.data_ptr(), pages.data_ptr(), pages.shape[1],
               cp, sp, rows, rot, pairs, out.data_ptr(), cache.data_ptr(), dtype_code(cache), num, page, S, T, n_heads, nkv, hd, _raw_stream(dev))
     return out
@@ -1298,7 +1308,7 @@ def paged_attention(q, positions, pages, cache, scale=None, out=None):
     _check_tensor("q", q, (torch.float32, torch.float16), 4, dev)
     num, nkv, page, hd, positions, pages = _paged(cache, positions, pages, dev)
     S, T, nh, qd = q.shape
-    if qd != hd or nh < 1 or nh % nkv or tuple(positions.shape) != (S, T):
+    if qd != hd or nh < 1 or nh % nkv or positions.shape != (S, T):
         raise ValueError("q %s does not go with a cache of %d heads of %d and positions %s" % (tuple(q.shape), nkv, hd, tuple(positions.shape)))
     q = q.contiguous()
     if out is None:

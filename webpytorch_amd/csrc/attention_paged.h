@@ -323,9 +323,9 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
 #pragma unroll
       for (int a = 0; a < NT; ++a) sc[n][a] = (float4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
+      for (int n = 0; n < NR; ++n) {
         if constexpr (C16) {
 #pragma unroll
           for (int p = QP - 1; p >= 0; --p) {
