@@ -448,7 +448,6 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
   }
 
   // ---- the waves' sums, rescaled to their common reference, a tile at a time ----
-  const int nw = max(1, min(NW, b1 - b0));  // waves that had keys (wave 0 always takes part)
   const int rows = min(16 * NR, R - r0);
   float* const os = reinterpret_cast<float*>(lds);  // [wave][row][HD + 4]
   // a part: [row][HD + 4], the sums, the reference and the sum of probabilities
@@ -461,38 +460,42 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
     const int nr = min(16, rows - 16 * n);
     if (nr <= 0) break;
     __syncthreads();
-    if (wave < nw) {
-      float sum = l[n][0];
-      if constexpr (!C16) {
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-      }
-      if (g == 0) {
-        ms[wave][c] = ref_log2(ref[n], back[n]);
-        ls[wave][c] = sum;
-      }
-      if (c < nr)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int d = 0; d < DL; d += 4)
-            *reinterpret_cast<float4v*>(&os[((size_t)wave * 16 + c) * (HD + 4) + DL * (4 * g + r) + d]) =
-                (float4v){o[n][d][r], o[n][d + 1][r], o[n][d + 2][r], o[n][d + 3][r]};
+    float sum = l[n][0];  // a wave that had no keys leaves zeros
+    if constexpr (!C16) {
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
     }
+    if (g == 0) {
+      ms[wave][c] = ref_log2(ref[n], back[n]);
+      ls[wave][c] = sum;
+    }
+    if (c < nr)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int d = 0; d < DL; d += 4)
+          *reinterpret_cast<float4v*>(&os[((size_t)wave * 16 + c) * (HD + 4) + DL * (4 * g + r) + d]) =
+              (float4v){o[n][d][r], o[n][d + 1][r], o[n][d + 2][r], o[n][d + 3][r]};
     __syncthreads();
     for (int x = tid; x < nr * (HD / 4); x += 64 * NW) {
       const int row = x / (HD / 4), d = 4 * (x % (HD / 4));
-      float mx = ms[0][row];
-      for (int w = 1; w < nw; ++w) mx = fmaxf(mx, ms[w][row]);
-      const float rf = mx == -INFINITY ? 0.f : mx;
-      float4v a = (float4v){0.f, 0.f, 0.f, 0.f};
-      float sum = 0.f;
-      for (int w = 0; w < nw; ++w) {
-        const float f = __builtin_amdgcn_exp2f(ms[w][row] - rf);
-        sum = fmaf(f, ls[w][row], sum);
-        const float4v v = *reinterpret_cast<const float4v*>(&os[((size_t)w * 16 + row) * (HD + 4) + d]);
+      float m[NW], sums[NW], mx = -INFINITY, sum = 0.f;
+      float4v v[NW], a = (float4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = fmaf(f, v[e], a[e]);
+      for (int w = 0; w < NW; ++w) {
+        m[w] = ms[w][row];
+        sums[w] = ls[w][row];
+        v[w] = *reinterpret_cast<const float4v*>(&os[((size_t)w * 16 + row) * (HD + 4) + d]);
+      }
+#pragma unroll
+      for (int w = 0; w < NW; ++w) mx = fmaxf(mx, m[w]);
+      const float rf = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = __builtin_amdgcn_exp2f(m[w] - rf);
+        sum = fmaf(f, sums[w], sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = fmaf(f, v[w][e], a[e]);
       }
       const int r = 16 * n + row;
       const uint32_t nan = nans[r][d >> 5] >> (d & 31);
