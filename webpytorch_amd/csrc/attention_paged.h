@@ -528,9 +528,13 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
       float4v st[U], v[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        const __amdgpu_buffer_rsrc_t pr = part_at(p0 + (int64_t)min(k0 + i, nparts - 1) * units);
-        st[i] = get4(pr, stat);
-        v[i] = get4(pr, at);
+        st[i] = (float4v){-INFINITY, 0.f, 0.f, 0.f};
+        v[i] = (float4v){0.f, 0.f, 0.f, 0.f};
+        if (k0 + i < nparts) {
+          const __amdgpu_buffer_rsrc_t pr = part_at(p0 + (int64_t)(k0 + i) * units);
+          st[i] = get4(pr, stat);
+          v[i] = get4(pr, at);
+        }
       }
       float mn = mx;
 #pragma unroll
@@ -540,13 +544,12 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
       a *= al;
       mx = mn;
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (k0 + i < nparts) {
-          const float f = __builtin_amdgcn_exp2f(st[i][0] - rf);
-          sum = fmaf(f, st[i][1], sum);
+      for (int i = 0; i < U; ++i) {
+        const float f = __builtin_amdgcn_exp2f(st[i][0] - rf);
+        sum = fmaf(f, st[i][1], sum);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a[e] = fmaf(f, v[i][e], a[e]);
-        }
+        for (int e = 0; e < 4; ++e) a[e] = fmaf(f, v[i][e], a[e]);
+      }
     }
     const int t = token(r0 + r);
     XT* orow = out + (((int64_t)s * T + t) * NH + h * rep + r0 + r - t * rep) * HD + d;
