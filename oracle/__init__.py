@@ -11,4 +11,6 @@ Modules and what pins each function (anything not listed as pinned says so in it
   q4k.py     -- Q4_K super-block dequant (`webtorch/ggufload.py:116-130, 188-202`)
   moe.py     -- sparse MoE MLP (`webtorch/lm_engine.py:294-333`)
   decode.py  -- growing-cache CPU decode of a Qwen2-shaped model (`webtorch/llm.py:1619-1636`)
+  kv4.py     -- the 4-bit cache and what goes with it; paged.py -- rotation, paged cache, attention, drafted tokens (float64,
+                from the definitions in include/miq.h; the reference has no counterpart)
 """

@@ -15,6 +15,11 @@
 // The work is split by the lengths, which are the device's: every workgroup adds them up and takes its part of a sequence, the
 // parts as long as give the chip the workgroups that it holds, so that long sequences beside short ones fill it too. The last
 // part of a sequence and head to arrive adds the parts, in their order.
+//
+// Bound and measured (us a replay over three states; a large copy moves 5.1 TB/s): memory for long caches, 64 sequences of 50 to 8000 positions,
+// 32 / 8 heads of 128, fp16 199 (1.06 GB), one token behind 131000 positions 111 (537 MB); the chain of positions, pages, blocks and joins, and
+// code fetched cold, for short ones, one token behind 700 positions of 14 / 2 heads of 64 8.8, behind 120 7.4; the fp32 matrix cores
+// where an fp32 cache meets several tiles, 16 sequences of up to 5000, 5 tokens of 28 / 4 heads 72 (174 MB, a block of 16 keys and 48 rows 2.6 us a wave).
 #pragma once
 #include <math.h>
 
