@@ -5,7 +5,7 @@
 // webtorch/llm.py:1270-1304; `rope_decode`: webtorch/_core.py:2302-2330) and writes to one contiguous cache (`kv_write`:
 // webtorch/_core.py:1504-1540).
 //
-// A thread takes 4 pairs of a head: two 16-byte loads of fp32 (8-byte ones of fp16 halves), both partners in one
+// A thread takes 4 pairs of a head: two 16-byte loads of fp32 (8-byte ones of fp16), both partners in one
 // thread, so that nothing passes between lanes but the sum of a norm, and a tensor may be rotated in place.
 //
 // Bound: memory for prompts (us a replay: 7001 tokens of 32 heads of 128 fp16, half of each rotated, 116 MB in 23.0, 5.0 TB/s; four prompts of 300 to
@@ -34,44 +34,41 @@ template <bool PAIRS> __device__ __forceinline__ void pair_at(int p, int half, i
   }
 }
 
-template <typename XT> __device__ __forceinline__ void load4(const XT* p, float* v);
-template <> __device__ __forceinline__ void load4<float>(const float* p, float* v) {
-  const float4v t = *reinterpret_cast<const float4v*>(p);
+// Vectors at any address that their elements may have: this target's loads and stores take them, at some cost where they cross lines
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 half4u __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void load4(const float* p, float* v) {
+  const float4u t = *reinterpret_cast<const float4u*>(p);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = t[i];
 }
-template <> __device__ __forceinline__ void load4<__half>(const __half* p, float* v) {
-  typedef _Float16 half4v __attribute__((ext_vector_type(4)));
-  const half4v t = *reinterpret_cast<const half4v*>(p);
+__device__ __forceinline__ void load4(const __half* p, float* v) {
+  const half4u t = *reinterpret_cast<const half4u*>(p);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = (float)t[i];
 }
-template <typename XT> __device__ __forceinline__ void store4(XT* p, const float* v);
-template <> __device__ __forceinline__ void store4<float>(float* p, const float* v) {
-  *reinterpret_cast<float4v*>(p) = (float4v){v[0], v[1], v[2], v[3]};
-}
-template <> __device__ __forceinline__ void store4<__half>(__half* p, const float* v) {
-  typedef _Float16 half4v __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<half4v*>(p) = (half4v){(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+__device__ __forceinline__ void store4(float* p, const float* v) { *reinterpret_cast<float4u*>(p) = (float4u){v[0], v[1], v[2], v[3]}; }
+__device__ __forceinline__ void store4(__half* p, const float* v) {
+  *reinterpret_cast<half4u*>(p) = (half4u){(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
 }
 
-// The 4 pairs p0 .. p0 + 3 of a head: a[i], b[i]. FAST: rot and HD are multiples of 8 and the addresses of 16 bytes, so that
-// the 4 are all rotated or all not, and lie in two vectors.
+// The 4 pairs p0 .. p0 + 3 of a head: a[i], b[i]. FAST: rot and HD are multiples of 8, so that the 4 are all rotated or all
+// not, and lie in two vectors.
 template <typename XT, bool FAST, bool PAIRS>
 __device__ __forceinline__ void load_pairs(const XT* x, int p0, int half, int HD, float* a, float* b) {
   if constexpr (FAST) {
     if (PAIRS || p0 >= half) {
       float v[8];
-      load4<XT>(x + 2 * p0, v);
-      load4<XT>(x + 2 * p0 + 4, v + 4);
+      load4(x + 2 * p0, v);
+      load4(x + 2 * p0 + 4, v + 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         a[i] = v[2 * i];
         b[i] = v[2 * i + 1];
       }
     } else {
-      load4<XT>(x + p0, a);
-      load4<XT>(x + p0 + half, b);
+      load4(x + p0, a);
+      load4(x + p0 + half, b);
     }
   } else {
 #pragma unroll
@@ -89,11 +86,11 @@ __device__ __forceinline__ void store_pairs(XT* x, int p0, int half, int HD, con
   if constexpr (FAST) {
     if (PAIRS || p0 >= half) {
       const float v[8] = {a[0], b[0], a[1], b[1], a[2], b[2], a[3], b[3]};
-      store4<XT>(x + 2 * p0, v);
-      store4<XT>(x + 2 * p0 + 4, v + 4);
+      store4(x + 2 * p0, v);
+      store4(x + 2 * p0 + 4, v + 4);
     } else {
-      store4<XT>(x + p0, a);
-      store4<XT>(x + p0 + half, b);
+      store4(x + p0, a);
+      store4(x + p0 + half, b);
     }
   } else {
 #pragma unroll
@@ -110,8 +107,8 @@ __device__ __forceinline__ void store_pairs(XT* x, int p0, int half, int HD, con
 template <bool FAST> __device__ __forceinline__ void load_angles(const float* cos_t, const float* sin_t, size_t row, int p0, int half, float* c, float* s) {
   if constexpr (FAST) {
     if (p0 < half) {
-      load4<float>(cos_t + row * half + p0, c);
-      load4<float>(sin_t + row * half + p0, s);
+      load4(cos_t + row * half + p0, c);
+      load4(sin_t + row * half + p0, s);
       return;
     }
   }
@@ -282,8 +279,7 @@ extern "C" int miq_rope(const void* x, int x_dtype, int64_t ld, int64_t lh, cons
   const int U = rope_many(T, H) ? kRopeHeads : 1;
   const int64_t threads = (int64_t)T * ((H + U - 1) / U) * ((HD + 7) / 8);
   MIQ_REQUIRE(threads < (1ll << 32) - kRopeThreads, MIQ_ERR_UNSUPPORTED, "rope: T=%d is past the grid", T);
-  const bool fast = rot % 8 == 0 && HD % 8 == 0 && aligned(x, 16) && aligned(out, 16) && aligned(cos_tab, 16) && aligned(sin_tab, 16) &&
-                    (T == 1 || (ld * size % 16 == 0 && out_ld * size % 16 == 0)) && (H == 1 || (lh * size % 16 == 0 && out_lh * size % 16 == 0));
+  const bool fast = rot % 8 == 0 && HD % 8 == 0;
   const dim3 grid((unsigned)((threads + kRopeThreads - 1) / kRopeThreads)), block(kRopeThreads);
   const hipStream_t st = static_cast<hipStream_t>(stream);
 #define MIQ_RP(XT, FV, PV, UV)                                                                                                     \
@@ -327,8 +323,7 @@ extern "C" int miq_paged_append(const void* qkv, int x_dtype, int64_t ld, const 
   const size_t nx = (size_t)((tokens - 1) * ld + W) * size, nq = (size_t)tokens * NH * HD * size, nc = (size_t)num_pages * 2 * NKV * page * HD * csize;
   MIQ_REQUIRE((!nq || !share_bytes(q_out, nq, qkv, nx)) && !share_bytes(cache, nc, qkv, nx) && (!nq || !share_bytes(cache, nc, q_out, nq)),
               MIQ_ERR_INVALID, "paged_append: qkv, q_out and the cache must lie apart");
-  const bool fast = rot % 8 == 0 && aligned(qkv, 16) && (tokens == 1 || ld * size % 16 == 0) && (NH == 0 || aligned(q_out, 16)) &&
-                    (rot == 0 || (aligned(cos_tab, 16) && aligned(sin_tab, 16)));
+  const bool fast = rot % 8 == 0;
   const dim3 grid((unsigned)((threads + kRopeThreads - 1) / kRopeThreads)), block(kRopeThreads);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int pshift = __builtin_ctz((unsigned)page);

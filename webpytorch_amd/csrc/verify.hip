@@ -92,26 +92,30 @@ __device__ __forceinline__ RowPart row_of_lanes(RowPart r, bool greedy, double c
   return RowPart{top, -1, lane_double(scan_double(s), 63)};
 }
 
-// A thread's N logits of a chunk of N kVfThreads from i0 on. In order: N consecutive ones; otherwise vectors (or values, where rows
-// are not aligned) of consecutive threads. -inf behind the row's end
-template <typename XT, int N> __device__ __forceinline__ int logit_at(int e, bool vec, bool in_order) {  // offset of value e in the chunk
+// A thread's N logits of a chunk of N kVfThreads from i0 on. In order: N consecutive ones; otherwise vectors of consecutive threads. Rows
+// may start at any value: this target's 16-byte loads do. -inf behind the row's end
+template <typename XT, int N> __device__ __forceinline__ int logit_at(int e, bool in_order) {  // offset of value e in the chunk
   constexpr int W = 16 / sizeof(XT);
   const int tid = threadIdx.x;
-  return in_order ? N * tid + e : vec ? (e / W * kVfThreads + tid) * W + e % W : e * kVfThreads + tid;
+  return in_order ? N * tid + e : (e / W * kVfThreads + tid) * W + e % W;
 }
 // as they lie in memory, so that the next chunk's take few registers on their way
+typedef uint32_t UnalignedVector __attribute__((ext_vector_type(4), aligned(2)));
 template <typename XT, int N> struct Logits {
   static constexpr int W = 16 / sizeof(XT);
   uint32_t raw[N * sizeof(XT) / 4];
-  __device__ __forceinline__ void load(const XT* row, int64_t i0, int V, bool vec, bool in_order) {
-    if (vec && i0 + N * kVfThreads <= V) {
+  __device__ __forceinline__ void load(const XT* row, int64_t i0, int V, bool in_order) {
+    if (i0 + N * kVfThreads <= V) {
 #pragma unroll
-      for (int k = 0; k < N; k += W)
-        *reinterpret_cast<miq_u32x4*>(&raw[k / W * 4]) = *reinterpret_cast<const miq_u32x4*>(row + i0 + logit_at<XT, N>(k, true, in_order));
+      for (int k = 0; k < N; k += W) {
+        const UnalignedVector w = *reinterpret_cast<const UnalignedVector*>(row + i0 + logit_at<XT, N>(k, in_order));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[k / W * 4 + e] = w[e];
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const int64_t i = i0 + logit_at<XT, N>(k, vec, in_order);
+        const int64_t i = i0 + logit_at<XT, N>(k, in_order);
         if constexpr (W == 4) {
           raw[k] = i < V ? __float_as_uint(row[i]) : 0xFF800000u;
         } else {
@@ -149,7 +153,6 @@ struct VerifyArgs {
   int32_t* tokens;         // [S][D + 1]
   int32_t* accepted;       // [S]
   int S, D, V, segs, groups, rounds;  // segments of a row, workgroups of a sequence, chunks a sum of weights
-  int lvec, dvec;
   uint64_t* parts;         // [rows][segs][2]
   double* sums;            // [S][kVfMaxChunks]
   Verdict* verdicts;       // [S]
@@ -182,10 +185,9 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
   const XT* const tl = static_cast<const XT*>(a.logits) + s * a.ls;
   const XT* const dl = static_cast<const XT*>(a.drafted) + s * a.ds;
   const XT* x = target ? tl + i * a.lr : dl + i * a.dr;
-  const bool vec = target ? a.lvec : a.dvec;
   const int chunks = (int)(((int64_t)a.V + kVfChunk - 1) / kVfChunk);
   Logits<XT, kVfLane> next;
-  next.load(x, (int64_t)seg * kVfChunk, a.V, vec, false);
+  next.load(x, (int64_t)seg * kVfChunk, a.V, false);
   // lane i has draft i, its logits and its random number: for the judgement, on the way from here on
   const int id = lane < D ? a.ids[(int64_t)s * D + lane] : -1;
   const int drafts = __builtin_ctzll(__ballot(id < 0));  // those ahead of the first id below 0
@@ -201,13 +203,13 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
   float floor = 0.f;
   for (int ch = seg; ch < chunks; ch += a.segs) {
     const Logits<XT, kVfLane> v = next;
-    if (ch + a.segs < chunks) next.load(x, (int64_t)(ch + a.segs) * kVfChunk, a.V, vec, false);
+    if (ch + a.segs < chunks) next.load(x, (int64_t)(ch + a.segs) * kVfChunk, a.V, false);
     if (greedy) {
 #pragma unroll
       for (int k = 0; k < kVfLane; ++k)
         if (v[k] > r.m) {
           r.m = v[k];
-          r.at = ch * kVfChunk + logit_at<XT, kVfLane>(k, vec, false);
+          r.at = ch * kVfChunk + logit_at<XT, kVfLane>(k, false);
         }
       continue;
     }
@@ -323,15 +325,14 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
   const bool minus = j.di > 0.;
   const XT* const trow = static_cast<const XT*>(a.logits) + s * a.ls + j.n * a.lr;
   const XT* const drow = minus ? static_cast<const XT*>(a.drafted) + s * a.ds + j.n * a.dr : nullptr;
-  const bool vec = a.lvec && (!minus || a.dvec);  // both rows in one order
   const double tmax = j.tmax, dmax = j.dmax;
   const float tfloor = power_floor(j.tmax, drop), dfloor = power_floor(j.dmax, drop);
   struct Chunk {
     Logits<XT, kVfLaneW> t, d;
   };
   auto load = [&](Chunk& x, int64_t i0, bool in_order) __attribute__((always_inline)) {
-    x.t.load(trow, i0, a.V, vec, in_order);
-    if (minus) x.d.load(drow, i0, a.V, vec, in_order);
+    x.t.load(trow, i0, a.V, in_order);
+    if (minus) x.d.load(drow, i0, a.V, in_order);
   };
   auto weights = [&](const Chunk& x, int64_t i0, bool in_order, double* w) __attribute__((always_inline)) {
     const Logits<XT, kVfLaneW>&v = x.t, &q = x.d;
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
     if (j.without >= i0 && j.without < i0 + kVfChunkW)
 #pragma unroll
       for (int k = 0; k < kVfLaneW; ++k)
-        if (i0 + logit_at<XT, kVfLaneW>(k, vec, in_order) == j.without) w[k] = 0.;
+        if (i0 + logit_at<XT, kVfLaneW>(k, in_order) == j.without) w[k] = 0.;
     double sum = 0.;
 #pragma unroll
     for (int k = 0; k < kVfLaneW; ++k) sum += w[k];
@@ -552,8 +553,6 @@ extern "C" int miq_verify_drafts(const void* logits, int x_dtype, int64_t ld_seq
   a.segs = p.segs;
   a.groups = p.groups;
   a.rounds = p.rounds;
-  a.lvec = aligned(logits, 16) && ld_seq * size % 16 == 0 && ld_row * size % 16 == 0;
-  a.dvec = dist && aligned(draft_logits, 16) && draft_ld_seq * size % 16 == 0 && draft_ld_row * size % 16 == 0;
   a.counters = static_cast<int*>(workspace);
   a.parts = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + kCounterBytes);
   a.sums = reinterpret_cast<double*>(static_cast<char*>(workspace) + kCounterBytes + p.parts);
