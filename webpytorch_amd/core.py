@@ -1129,7 +1129,7 @@ def rope_tables(n, rot, theta=10000.0, scaling=None, interleaved=False):
       "dynamic": theta grows by (factor n / original - factor + 1)^(rot / (rot - 2)) where n is past `original`;
       "yarn": f_i where a pair turns more than beta_fast (32) times in `original` positions, f_i / factor where fewer than
         beta_slow (1), a linear ramp over i between; cos and sin times attention_factor (0.1 ln factor + 1);
-      "wavelength": f_i where 2 pi / f_i < original / high_freq_factor (4), f_i / factor where it is above original /
+      "wavelength" (also "llama3"): f_i where 2 pi / f_i < original / high_freq_factor (4), f_i / factor where it is above original /
         low_freq_factor (1), and between them the two mixed linearly in original f_i / 2 pi;
     with "factor" and (but for linear) "original_max_position_embeddings"."""
     n, rot = int(n), int(rot)
@@ -1140,9 +1140,10 @@ def rope_tables(n, rot, theta=10000.0, scaling=None, interleaved=False):
     kind = sc.get("rope_type", sc.get("type", "default"))
     factor, mul = float(sc.get("factor", 1.0)), 1.0
     original = float(sc.get("original_max_position_embeddings", 0) or 0)
+    kind = {"llama3": "wavelength", None: "default"}.get(kind, kind)
     if kind not in ("default", "linear", "dynamic", "yarn", "wavelength"):
         raise NotImplementedError("rope_type %r (linear, dynamic, yarn or wavelength)" % (kind,))
-    if not factor > 0 or not theta > 0 or (kind in ("dynamic", "yarn", "wavelength") and not original > 0):
+    if not factor > 0 or not theta > 0 or (kind in ("dynamic", "yarn", "wavelength") and not original > 0) or (kind == "yarn" and theta <= 1):
         raise ValueError("rope_tables: theta=%g factor=%g original_max_position_embeddings=%g" % (theta, factor, original))
     if kind == "dynamic" and n > original and rot > 2:
         theta = theta * (factor * n / original - factor + 1.0) ** (rot / (rot - 2.0))
