@@ -232,6 +232,23 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
     return b;
   };
 
+  // ---- q, LG lanes a row: on its way ahead of the first block, which would hold it up (16 sequences of 5 tokens 72 -> 70 us) ----
+  constexpr int LG = HD == 64 ? 8 : HD == 128 ? 16 : 32, QI = (16 * NR * LG + 64 * NW - 1) / (64 * NW);
+  const int ch = tid % LG;
+  float qv[QI][8];
+#pragma unroll
+  for (int i = 0; i < QI; ++i) {
+    const int row = tid / LG + i * (64 * NW / LG), r = r0 + row;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) qv[i][e] = 0.f;
+    if (row < 16 * NR && r < R && ch < HD / 8) {
+      const int t = token(r);
+      const XT* p = q + (((int64_t)s * T + t) * NH + h * rep + r - t * rep) * HD + 8 * ch;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qv[i][e] = to_f32<XT>(p[e]);
+    }
+  }
+
   int blk = b0 + wave;
   const bool work = blk < b1;  // wave-uniform
   Block cur;
@@ -242,26 +259,16 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
     load_values(blk, cur);
   }
 
-  // ---- q as operands in LDS, LG lanes a row ----
+  // ---- q as operands in LDS ----
   {
-    constexpr int LG = HD == 64 ? 8 : HD == 128 ? 16 : 32;
     const float sign = scale < 0.f ? -1.f : scale == 0.f ? 0.f : 1.f;
-    const int ch = tid % LG;
-    for (int row = tid / LG; row < 16 * NR; row += 64 * NW / LG) {
-      const int r = r0 + row;
-      const bool in = r < R && ch < HD / 8;
-      float v[8], mx = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      if (in) {
-        const int t = token(r);
-        const XT* p = q + (((int64_t)s * T + t) * NH + h * rep + r - t * rep) * HD + 8 * ch;
+    for (int i = 0; i < QI; ++i) {
+      const int row = tid / LG + i * (64 * NW / LG), r = r0 + row;
+      if (row >= 16 * NR) break;
+      float mx = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = to_f32<XT>(p[e]);
-          mx = fmaxf(mx, fabsf(v[e]));
-        }
-      }
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(qv[i][e]));
       int n = 0;
       if constexpr (QP == 2) {
 #pragma unroll
@@ -269,14 +276,16 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
         n = row_shift(mx);
       }
       if (ch < HD / 32) nans[row][ch] = 0;
-      if (ch == 0) lims[row] = r >= R ? -1 : T == 1 ? len - 1 : min(pos[token(r)], cap - 1);
-      if (ch == 0) backs[row] = scale == 0.f ? 1.f : fmaxf(ldexpf(fabsf(scale) * 1.44269504088896340736f, -n), 0x1p-126f);
+      if (ch == 0) {
+        lims[row] = r >= R ? -1 : T == 1 ? len - 1 : min(pos[token(r)], cap - 1);
+        backs[row] = scale == 0.f ? 1.f : fmaxf(ldexpf(fabsf(scale) * 1.44269504088896340736f, -n), 0x1p-126f);
+      }
       if (ch < HD / 8) {
         if constexpr (C16) {  // [tile][plane][32 dimensions][g][row][8 dimensions]
           half8v hi, lo;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float x = sign * (QP == 2 ? ldexpf(v[e], n) : v[e]);
+            const float x = sign * (QP == 2 ? ldexpf(qv[i][e], n) : qv[i][e]);
             hi[e] = (_Float16)x;
             lo[e] = (_Float16)(x - (float)hi[e]);
           }
@@ -285,9 +294,9 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
           if constexpr (QP == 2) o[NJ * 64] = lo;
         } else {  // [tile][16 dimensions][g][row][4 dimensions]
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            *(reinterpret_cast<float4v*>(lds) + ((row >> 4) * NJ + (2 * ch + i) / 4) * 64 + ((2 * ch + i) & 3) * 16 + (row & 15)) =
-                (float4v){sign * v[4 * i], sign * v[4 * i + 1], sign * v[4 * i + 2], sign * v[4 * i + 3]};
+          for (int k = 0; k < 2; ++k)
+            *(reinterpret_cast<float4v*>(lds) + ((row >> 4) * NJ + (2 * ch + k) / 4) * 64 + ((2 * ch + k) & 3) * 16 + (row & 15)) =
+                (float4v){sign * qv[i][4 * k], sign * qv[i][4 * k + 1], sign * qv[i][4 * k + 2], sign * qv[i][4 * k + 3]};
         }
       }
     }
