@@ -113,7 +113,7 @@ def lib():
 
 def call(name, *args):
     """Invoke an entry point and turn a negative return code into a Python exception."""
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != 0:
         msg = lib().miq_last_error().decode(errors="replace")
         raise ERRORS.get(rc, MiqError)("%s failed (%d): %s" % (name, rc, msg))

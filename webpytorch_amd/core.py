@@ -901,9 +901,12 @@ MAX_TOP_LOGPROBS = 32
 _CAPTURED_COUNTERS = 1 << 17
 
 
+_Tensor = torch.Tensor
+
+
 def _gpu_of(name, t):
     """The device index of a torch tensor, which has to be the current GPU's."""
-    d = t.get_device() if isinstance(t, torch.Tensor) else -1
+    d = t.get_device() if isinstance(t, _Tensor) else -1
     if d < 0:
         raise ValueError("%s must be a torch tensor on the GPU" % name)
     if d != torch._C._cuda_getDevice():  # without torch.cuda's check that it is initialised, which a tensor on a GPU shows
@@ -913,7 +916,7 @@ def _gpu_of(name, t):
 
 def _check_tensor(name, t, dtypes, dim, dev):
     """Refuse what a kernel would read wrongly: no tensor on GPU `dev`, another dtype or rank (dim None: any)."""
-    if isinstance(t, torch.Tensor) and t.dtype in dtypes and (dim is None or t.dim() == dim) and t.get_device() == dev:
+    if isinstance(t, _Tensor) and t.dtype in dtypes and (dim is None or t.dim() == dim) and t.get_device() == dev:
         return
     if _gpu_of(name, t) != dev:
         raise ValueError("%s is on another GPU than the other tensors" % name)
@@ -1118,6 +1121,7 @@ def token_logprobs(logits, ids, top_k=0):
 PAGE_SIZES = (16, 4096)  # least and most positions of a page, a power of two
 MAX_DRAFTS = 32
 Rope = collections.namedtuple("Rope", "cos sin interleaved")
+_FLOATS, _F32, _I32 = (torch.float32, torch.float16), (torch.float32,), (torch.int32,)
 
 
 def rope_tables(n, rot, theta=10000.0, scaling=None, interleaved=False):
@@ -1172,7 +1176,7 @@ def _rope_arg(rope, hd, dev):
     """(cos address, sin address, rows, rot, pairs) of a `Rope` for heads of hd."""
     cos, sin, pairs = rope
     for name, t in (("cos", cos), ("sin", sin)):
-        _check_tensor(name, t, (torch.float32,), 2, dev)
+        _check_tensor(name, t, _F32, 2, dev)
     shape = cos.shape
     rows, half = shape
     if sin.shape != shape or not 1 <= half <= hd // 2 or rows < 1 or not (cos.is_contiguous() and sin.is_contiguous()):
@@ -1183,7 +1187,7 @@ def _rope_arg(rope, hd, dev):
 
 def _int32(name, t, shape, dev):
     """A contiguous int32 tensor of this shape."""
-    _check_tensor(name, t, (torch.int32,), len(shape), dev)
+    _check_tensor(name, t, _I32, len(shape), dev)
     if t.shape != shape:
         raise ValueError("%s has shape %s: %s is expected" % (name, tuple(t.shape), tuple(shape)))
     return t if t.is_contiguous() else t.contiguous()
@@ -1196,7 +1200,7 @@ def rope(x, positions, rope, transpose=False, out=None):
     position outside the tables makes zeros. `out`, if given, is of x's type and shape; it may be x itself, but not overlap it
     otherwise. (`_rope_np`, `_rot`: `webtorch/llm.py:1270-1304`.)"""
     dev = _gpu_of("x", x)
-    _check_tensor("x", x, (torch.float32, torch.float16), 3, dev)
+    _check_tensor("x", x, _FLOATS, 3, dev)
     T, H, hd = x.shape
     if hd % 2 or not 2 <= hd <= 1024:
         raise ValueError("heads of %d dimensions (even, 2 .. 1024)" % hd)
@@ -1237,14 +1241,14 @@ def paged_cache(num_pages, nkv, page, hd, dtype=torch.float16):
 
 def _paged(cache, positions, pages, dev):
     """Checks a paged cache with a batch's positions (S, T) and pages (S, most): (num_pages, nkv, page, hd, positions, pages)."""
-    _check_tensor("the cache", cache, (torch.float16, torch.float32), 5, dev)
+    _check_tensor("the cache", cache, _FLOATS, 5, dev)
     num, two, nkv, page, hd = cache.shape
     if two != 2 or hd not in KV4_HEADS or num < 1 or nkv < 1 or not PAGE_SIZES[0] <= page <= PAGE_SIZES[1] or page & (page - 1) \
             or not cache.is_contiguous():
         raise ValueError("a paged cache is a contiguous (pages, 2, NKV, page, HD) tensor, page a power of two from %d to %d, HD 64, 128, 192 or "
                          "256: got %s" % (PAGE_SIZES + (tuple(cache.shape),)))
-    _check_tensor("positions", positions, (torch.int32,), 2, dev)
-    _check_tensor("pages", pages, (torch.int32,), 2, dev)
+    _check_tensor("positions", positions, _I32, 2, dev)
+    _check_tensor("pages", pages, _I32, 2, dev)
     if pages.shape[0] != positions.shape[0]:
         raise ValueError("pages of %d sequences, positions of %d" % (pages.shape[0], positions.shape[0]))
     return num, nkv, page, hd, positions if positions.is_contiguous() else positions.contiguous(), pages if pages.is_contiguous() else pages.contiguous()
@@ -1260,7 +1264,7 @@ def paged_append(qkv, positions, pages, cache, n_heads, rope=None, qn=None, kn=N
     not overlap qkv or each other. (`CausalLM._qkv`, `_rope_np`, `kv_write`: `webtorch/llm.py:1498-1519, 1270-1304`,
     `webtorch/_core.py:1504-1540`, one sequence into a contiguous cache.)"""
     dev = _gpu_of("qkv", qkv)
-    _check_tensor("qkv", qkv, (torch.float32, torch.float16), 3, dev)
+    _check_tensor("qkv", qkv, _FLOATS, 3, dev)
     num, nkv, page, hd, positions, pages = _paged(cache, positions, pages, dev)
     S, T, W = qkv.shape
     if positions.shape != (S, T):
@@ -1270,7 +1274,7 @@ def paged_append(qkv, positions, pages, cache, n_heads, rope=None, qn=None, kn=N
     cp, sp, rows, rot, pairs = (None, None, 0, 0, 0) if rope is None else _rope_arg(rope, hd, dev)
     for name, t in (("qn", qn), ("kn", kn)):
         if t is not None:
-            _check_tensor(name, t, (torch.float32,), 1, dev)
+            _check_tensor(name, t, _F32, 1, dev)
             if t.shape[0] != hd or not t.is_contiguous():
                 raise ValueError("%s has shape %s: (%d,) is expected" % (name, tuple(t.shape), hd))
     # rows of one distance
@@ -1306,7 +1310,7 @@ def paged_attention(q, positions, pages, cache, scale=None, out=None):
     work is split by their lengths, on the device. `out`, if given, may not overlap q or the cache. Returns (S, T, NH, HD)
     in q's dtype. (`KVCache.attn`, `gqa_attention`: `webtorch/_core.py:1543-1596, 1319-1340`.)"""
     dev = _gpu_of("q", q)
-    _check_tensor("q", q, (torch.float32, torch.float16), 4, dev)
+    _check_tensor("q", q, _FLOATS, 4, dev)
     num, nkv, page, hd, positions, pages = _paged(cache, positions, pages, dev)
     S, T, nh, qd = q.shape
     if qd != hd or nh < 1 or nh % nkv or positions.shape != (S, T):
@@ -1340,19 +1344,19 @@ def verify_drafts(logits, drafts, uniforms, draft_logits=None, temperature=1.0):
     accepted (S,) int32. -inf logits are tokens of probability 0; a target row with NaN or +inf, or of nothing above -inf, accepts
     nothing and gives -1. D <= 32. (`_pick`: `webtorch/llm.py:1309-1336`, on the host.)"""
     dev = _gpu_of("logits", logits)
-    _check_tensor("logits", logits, (torch.float32, torch.float16), 3, dev)
+    _check_tensor("logits", logits, _FLOATS, 3, dev)
     S, rows, V = logits.shape
     D = rows - 1
     if D < 0 or V < 1:
         raise ValueError("logits (S, D + 1, V) have shape %s" % (tuple(logits.shape),))
     drafts = _int32("drafts", drafts, (S, D), dev)
-    _check_tensor("uniforms", uniforms, (torch.float32,), 2, dev)
+    _check_tensor("uniforms", uniforms, _F32, 2, dev)
     if tuple(uniforms.shape) != (S, D + 1):
         raise ValueError("uniforms have shape %s: %s is expected" % (tuple(uniforms.shape), (S, D + 1)))
     uniforms = uniforms.contiguous()
     temps, temp = None, 0.0
     if isinstance(temperature, torch.Tensor):
-        _check_tensor("temperature", temperature, (torch.float32,), 1, dev)
+        _check_tensor("temperature", temperature, _F32, 1, dev)
         if temperature.shape[0] != S:
             raise ValueError("temperature has shape %s: (%d,) is expected" % (tuple(temperature.shape), S))
         temps = temperature.contiguous()
