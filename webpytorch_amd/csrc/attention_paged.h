@@ -18,8 +18,8 @@
 //
 // Bound and measured (us a replay over three states; a large copy moves 5.1 TB/s): memory for long caches, 64 sequences of 50 to 8000 positions,
 // 32 / 8 heads of 128, fp16 199 (1.06 GB), one token behind 131000 positions 111 (537 MB); the chain of positions, pages, blocks and joins, and
-// code fetched cold, for short ones, one token behind 700 positions of 14 / 2 heads of 64 8.8, behind 120 7.4; the fp32 matrix cores
-// where an fp32 cache meets several tiles, 16 sequences of up to 5000, 5 tokens of 28 / 4 heads 72 (174 MB, a block of 16 keys and 48 rows 2.6 us a wave).
+// code fetched cold, for short ones, one token behind 700 positions of 14 / 2 heads of 64 9.0, behind 120 of 32 / 8 of 128 7.6; the fp32 matrix cores
+// where an fp32 cache meets several tiles, 16 sequences of up to 5000, 5 tokens of 28 / 4 heads 70 (174 MB, a block of 16 keys and 48 rows 2.6 us a wave).
 #pragma once
 #include <math.h>
 

@@ -12,7 +12,7 @@
 // last segment of a sequence to arrive judges its drafts; then a group of workgroups for each sequence sums the weights of its
 // chunks, and the last of them to arrive finds the chunk, the thread and the index.
 //
-// Bound and measured (us a replay): 64 sequences of 4 drafts, V 128256, fp32 97: the rows 64 (295 MB, 4.6 TB/s) and the draw 33 (66 MB of them
+// Bound and measured (us a replay): 64 sequences of 4 drafts, V 128256, fp32 100: the rows 65 (295 MB, 4.5 TB/s) and the draw 32 (66 MB of them
 // again, fp64 issue); one sequence, V 151936, 26: the chain logits, part, counter, judgement and then weights, sum, counter, chunk.
 #include <math.h>
 
@@ -42,7 +42,7 @@ __device__ __forceinline__ double power_unit(float temperature, float& drop) {
   return kVfPowers * 1.4426950408889634 / (double)temperature;
 }
 // 2^((x - m) c / 256) added to `sum`, 1 for m itself: whole multiples of 1 / 256 by the table and the exponent, the rest, |f| <= 1 / 512, by the
-// series of e^(f ln 2) to the third power (1.4e-13). 10 fp64 instructions (a table of 32 takes 12, the series of |f| <= 1 / 2 alone 19),
+// series of e^(f ln 2) to the third power (1.4e-13). 10 fp64 operations (a table of 32 takes 12, the series of |f| <= 1 / 2 alone 19),
 // which with the loads' latency bound the kernel of the rows (64 sequences of 4 drafts, V 128256: fp16 61 us, fp32 64, where its bytes take 62).
 __device__ __forceinline__ double power_plus(float x, double m, double c, const double* tab, double sum) {
   const double y = ((double)x - m) * c, magic = 6755399441055744.;  // 1.5 2^52: the whole part in the low word
@@ -469,7 +469,8 @@ struct VerifyPlan {
   size_t parts, sums, verdicts;
 };
 // Segments of a row: four workgroups a CU run at once, one after another takes as long as its chunks and some 4 more (start and sums).
-// (24 sequences of 6 looked-up drafts, fp16, V 32003: 7 segments, 1176 workgroups, 20.4 us; 4, which fit at once, 17.8.) Workgroups of a sequence's
+// (24 sequences of 6 looked-up drafts, fp16, V 32003: 7 segments, 1176 workgroups, 20.4 us; 4, which fit at once, 17.8, and 14.8 since rows
+// of odd length are read by vectors.) Workgroups of a sequence's
 // weights: likewise at once.
 static VerifyPlan verify_plan(int S, int D, int V, bool dist) {
   VerifyPlan p;
