@@ -12,8 +12,8 @@
 // last segment of a sequence to arrive judges its drafts; then a group of workgroups for each sequence sums the weights of its
 // chunks, and the last of them to arrive finds the chunk, the thread and the index.
 //
-// Bound and measured (us a replay): 64 sequences of 4 drafts, V 128256, fp32 100: the rows 65 (295 MB, 4.5 TB/s) and the draw 32 (66 MB of them
-// again, fp64 issue); one sequence, V 151936, 26: the chain logits, part, counter, judgement and then weights, sum, counter, chunk.
+// Bound and measured (us a replay): 64 sequences of 4 drafts, V 128256, fp32 95: the rows 65 (295 MB, 4.5 TB/s) and the draw 27 (66 MB of them
+// again, fp64 issue); one sequence, V 151936, 21: the chain logits, part, counter, judgement and then weights, sum, counter, chunk.
 #include <math.h>
 
 #include "attention_parts.h"
@@ -163,10 +163,12 @@ __device__ __forceinline__ float temperature(const VerifyArgs& a, int s) {
   const float t = a.temps ? a.temps[s] : a.temp;
   return t > 0.f && t < INFINITY ? t : 0.f;
 }
-__device__ __forceinline__ void answer(const VerifyArgs& a, int s, int n, int token) {  // by one thread
-  int32_t* o = a.tokens + (int64_t)s * (a.D + 1);
-  for (int i = 0; i <= a.D; ++i) o[i] = i < n ? a.ids[(int64_t)s * a.D + i] : i == n ? token : -1;
-  a.accepted[s] = n;
+// by a wave, whose lane i has draft i: one store (with the marks by ballots, where LDS atomics and one thread in a loop were, the draw behind 4 drafts
+// 12.6 -> 7.8 us)
+__device__ __forceinline__ void answer(const VerifyArgs& a, int s, int n, int token, int id) {
+  const int lane = threadIdx.x & 63;
+  if (lane <= a.D) a.tokens[(int64_t)s * (a.D + 1) + lane] = lane < n ? id : lane == n ? token : -1;
+  if (lane == 0) a.accepted[s] = n;
 }
 
 // Segment blockIdx.x of row blockIdx.y: the S (D + 1) target rows, then the S D draft rows. The last segment of a sequence's rows to
@@ -283,7 +285,6 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
   }
   const int n = __builtin_ctzll(__ballot(!ok));  // lanes from `drafts` on say no
   const int refusal = __builtin_amdgcn_readlane(id, n);
-  if (lane != 0) return;
   const bool refused = n < drafts, law = greedy ? trow[n].at >= 0 : trow[n].s > 0.;  // law: the row is a distribution
   Verdict v = {n, greedy || !law ? (law ? trow[n].at : -1) : kVfDraw, refused, refused && !dist ? refusal : -1, trow[n].m, 0.f,
                1. / trow[n].s, 0.};
@@ -291,8 +292,8 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     v.dmax = drow[n].m;
     v.di = 1. / drow[n].s;
   }
-  a.verdicts[s] = v;
-  if (v.token != kVfDraw) answer(a, s, n, v.token);
+  if (lane == 0) a.verdicts[s] = v;
+  if (v.token != kVfDraw) answer(a, s, n, v.token, id);
 }
 
 // Exclusive sum of v over the workgroup's threads, in their order; all is the sum of them all
@@ -312,12 +313,31 @@ __device__ __forceinline__ double sums_before(double v, double* waves, double& a
   return w + (x - v);
 }
 
+// The first of the threads' `hit` and the last of their `any` that are not -1 (they ascend with the threads); -1 where there is none
+__device__ __forceinline__ void first_and_last(int hit, int any, int (*marks)[kVfThreads / 64], int& first, int& last) {
+  const uint64_t h = __ballot(hit >= 0), y = __ballot(any >= 0);
+  first = h ? __builtin_amdgcn_readlane(hit, __builtin_ctzll(h)) : -1;
+  last = y ? __builtin_amdgcn_readlane(any, 63 - __builtin_clzll(y)) : -1;
+  if ((threadIdx.x & 63) == 0) {
+    marks[0][threadIdx.x >> 6] = first;
+    marks[1][threadIdx.x >> 6] = last;
+  }
+  __syncthreads();
+  first = last = -1;
+#pragma unroll
+  for (int w = 0; w < kVfThreads / 64; ++w) {
+    if (first < 0) first = marks[0][w];
+    if (marks[1][w] >= 0) last = marks[1][w];
+  }
+}
+
 template <typename XT>
 __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) {
   __shared__ double waves[kVfThreads / 64], tab[kVfPowers], found_before;
-  __shared__ int verdict[2], last;
-  const int s = blockIdx.y, tid = threadIdx.x, D = a.D;
+  __shared__ int marks[2][kVfThreads / 64], last;
+  const int s = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, D = a.D;
   const Verdict j = a.verdicts[s];
+  const int id = tid < D ? a.ids[(int64_t)s * D + tid] : -1;  // for the answer
   float drop;
   const double c = power_unit(temperature(a, s), drop), ulast = a.uniforms[(int64_t)s * (D + 1) + D];
   fill_powers(tab);
@@ -391,11 +411,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
                           : 0.;
     mine += part[k];
   }
-  if (tid == 0) {
-    verdict[0] = 0x7FFFFFFF;
-    verdict[1] = -1;
-  }
-  double run = sums_before(mine, waves, total);  // its barriers lie between the marks and what follows
+  double run = sums_before(mine, waves, total);
   const double want = ulast * total;
   int hit = -1, heavy = -1;  // the first chunk past it; the last with any weight
   double at_hit = 0., at_heavy = 0.;
@@ -411,20 +427,17 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
     }
     run += part[k];
   }
-  if (hit >= 0) atomicMin(&verdict[0], hit);
-  if (heavy >= 0) atomicMax(&verdict[1], heavy);
-  __syncthreads();
-  const int ch = verdict[0] != 0x7FFFFFFF ? verdict[0] : verdict[1];
+  int first, rest;
+  first_and_last(hit, heavy, marks, first, rest);
+  const int ch = first >= 0 ? first : rest;
   if (ch < 0) {  // the target leaves nothing beside the draft, or the two are the same
-    if (tid == 0) {
-      const int id = j.refused ? a.ids[(int64_t)s * D + j.n] : -1;
-      answer(a, s, j.n, id < a.V ? id : -1);
-    }
+    const int draft = j.refused ? a.ids[(int64_t)s * D + j.n] : -1;
+    if (wave == 0) answer(a, s, j.n, draft < a.V ? draft : -1, id);
     return;
   }
   if (hit == ch)
     found_before = at_hit;
-  else if (heavy == ch && verdict[0] == 0x7FFFFFFF)
+  else if (heavy == ch && first < 0)
     found_before = at_heavy;
   __syncthreads();
   double before = found_before;
@@ -432,10 +445,6 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
   for (int k = 0; k < a.rounds; ++k) {
     const int64_t i0 = (int64_t)ch * span + k * kVfChunkW;
     double w[kVfLaneW], all;
-    if (tid == 0) {
-      verdict[0] = 0x7FFFFFFF;
-      verdict[1] = -1;
-    }
     Chunk x;
     load(x, i0, true);
     const double mine = weights(x, i0, true, w);
@@ -450,17 +459,13 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
       }
     }
     // the first hit; where rounding leaves none, the last index of the chunk with any weight
-    if (hit >= 0) atomicMin(&verdict[0], hit);
-    if (any >= 0) atomicMax(&verdict[1], any);
-    __syncthreads();
-    const int first = verdict[0];
-    if (verdict[1] >= 0) fallback = verdict[1];
-    if (first != 0x7FFFFFFF || k == a.rounds - 1) {
-      if (tid == 0) answer(a, s, j.n, first != 0x7FFFFFFF ? first : fallback);
+    first_and_last(hit, any, marks, first, rest);
+    if (rest >= 0) fallback = rest;
+    if (first >= 0 || k == a.rounds - 1) {
+      if (wave == 0) answer(a, s, j.n, first >= 0 ? first : fallback, id);
       return;
     }
     before += all;
-    __syncthreads();
   }
 }
 
