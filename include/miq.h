@@ -496,7 +496,7 @@ int miq_paged_attention(const void* q, int x_dtype, const void* cache, int cache
  * weights passes uniforms[s][D] times their total. Temperature 0 (or one that is no finite number above it): a draft is accepted if it is the largest logit's
  * index (the lowest of equal ones; NaN counts as -inf), which is the token too.
  * tokens int32 [S][D + 1]: the accepted drafts, the token, then -1; accepted int32 [S]: n. Logits of -inf are tokens of
- * probability 0. A target row without a distribution (NaN, +inf at a temperature above 0, nothing above -inf) accepts nothing and
+ * probability 0, as are in the draw those below 2^-899 of the likeliest's. A target row without a distribution (NaN, +inf at a temperature above 0, nothing above -inf) accepts nothing and
  * its token is -1; without one a draft's row is refused and p drawn from; so is a draft from V on. Where max(p - q, 0) has no weight
  * the token is the draft. fp64 exponentials and sums (2e-13). D <= 32, S (2 D + 1) <= 65535. workspace as for
  * miq_paged_attention (always needed).

@@ -34,26 +34,28 @@ __device__ __forceinline__ void fill_powers(double* tab) {
   tab[threadIdx.x] = exp2((double)threadIdx.x / kVfPowers);
   __syncthreads();
 }
-// x is taken to be no further below m than 623 times the temperature (-inf among it): 2^-899, which no sum sees
-__device__ __forceinline__ float power_floor(float m, float drop) { return fmaxf(m - drop, -3.402823466e38f); }
-// c of a temperature, and the drop of its floor
-__device__ __forceinline__ double power_unit(float temperature, float& drop) {
-  drop = 623.f * temperature;
-  return kVfPowers * 1.4426950408889634 / (double)temperature;
-}
-// 2^((x - m) c / 256) added to `sum`, 1 for m itself: whole multiples of 1 / 256 by the table and the exponent, the rest, |f| <= 1 / 512, by the
+// c of a temperature
+__device__ __forceinline__ double power_unit(float temperature) { return kVfPowers * 1.4426950408889634 / (double)temperature; }
+// High word of -899 kVfPowers. Powers are no lower than 2^-899 (-inf among them), which no sum sees. The border is drawn on the exponent: of the
+// fp32 logits, m less 623 temperatures rounds to m itself where the temperature is small. Exponents are 0 or negative, so that
+// their high words, as unsigned numbers, ascend as they descend: the least of two words bounds one, at the cost of an fp32 maximum.
+constexpr uint32_t kVfDeepest = 0xC10C1800u;
+// 2^((x - m) c / 256), x <= m, added to `sum`, 1 for m itself: whole multiples of 1 / 256 by the table and the exponent, the rest, |f| <= 1 / 512, by the
 // series of e^(f ln 2) to the third power (1.4e-13). 10 fp64 operations (a table of 32 takes 12, the series of |f| <= 1 / 2 alone 19),
-// which with the loads' latency bound the kernel of the rows (64 sequences of 4 drafts, V 128256: fp16 61 us, fp32 64, where its bytes take 62).
-__device__ __forceinline__ double power_plus(float x, double m, double c, const double* tab, double sum) {
-  const double y = ((double)x - m) * c, magic = 6755399441055744.;  // 1.5 2^52: the whole part in the low word
+// which with the loads' latency bound the kernel of the rows (64 sequences of 4 drafts, V 128256: fp16 61 us, fp32 64, where its bytes take 58).
+// ZERO: nothing for what is as low as the border, so that no draw falls on it.
+template <bool ZERO = false> __device__ __forceinline__ double power_plus(float x, double m, double c, const double* tab, double sum) {
+  const double far = ((double)x - m) * c, magic = 6755399441055744.;  // 1.5 2^52: the whole part in the low word
+  const uint32_t high = (uint32_t)__double2hiint(far);
+  const double y = __hiloint2double((int)min(high, kVfDeepest), __double2loint(far));
   const double up = y + magic, f = y - (up - magic);
   const int k = __double2loint(up);
   double p = 3.308302680541371e-09;  // (ln 2 / 256)^n / n!
   p = fma(p, f, 3.665565596910106e-06);
   p = fma(p, f, 0.0027076061740622863);
   p = fma(p, f, 1.0);
-  const double t = tab[k & (kVfPowers - 1)];
-  return fma(__hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t)), p, sum);
+  const double t = tab[k & (kVfPowers - 1)], power = __hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t));
+  return fma(ZERO && high >= kVfDeepest ? 0. : power, p, sum);
 }
 template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ double dpp_double(double v) {  // 0 where no lane is the source
   return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, false),
@@ -80,7 +82,7 @@ struct RowPart {
   double s;
 };
 // of the parts that the lanes of a wave hold
-__device__ __forceinline__ RowPart row_of_lanes(RowPart r, bool greedy, double c, float drop, const double* tab) {
+__device__ __forceinline__ RowPart row_of_lanes(RowPart r, bool greedy, double c, const double* tab) {
   const float top = wave_max(r.m);
   if (greedy) {
     uint32_t at = r.m == top && r.m > -INFINITY ? (uint32_t)r.at : 0xFFFFFFFFu;
@@ -88,7 +90,7 @@ __device__ __forceinline__ RowPart row_of_lanes(RowPart r, bool greedy, double c
     for (int d = 1; d < 64; d *= 2) at = min(at, (uint32_t)__shfl_xor((int)at, d));
     return RowPart{top, (int)at, 0.};
   }
-  const double s = r.m > -INFINITY ? r.s * power_plus(fmaxf(r.m, power_floor(top, drop)), top, c, tab, 0.) : r.s;  // 0 or NaN
+  const double s = r.m > -INFINITY ? r.s * power_plus(r.m, top, c, tab, 0.) : r.s;  // 0 or NaN
   return RowPart{top, -1, lane_double(scan_double(s), 63)};
 }
 
@@ -197,12 +199,10 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
   const bool inside = lane < drafts && id < a.V;
   const float tx = inside ? to_f32<XT>(tl[lane * a.lr + id]) : 0.f, dx = inside && dist ? to_f32<XT>(dl[lane * a.dr + id]) : 0.f;
   const float ux = lane < drafts ? a.uniforms[(int64_t)s * (D + 1) + lane] : 0.f;
-  float drop;
-  const double c = power_unit(temp, drop);
+  const double c = power_unit(temp);
   fill_powers(tab);
   RowPart r = {-INFINITY, -1, 0.};
   double top = 0.;
-  float floor = 0.f;
   for (int ch = seg; ch < chunks; ch += a.segs) {
     const Logits<XT, kVfLane> v = next;
     if (ch + a.segs < chunks) next.load(x, (int64_t)(ch + a.segs) * kVfChunk, a.V, false);
@@ -223,22 +223,21 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
       bad = bad || !(v[k] < INFINITY);
     }
     if (mx > r.m) {
-      r.s = r.m == -INFINITY ? r.s : r.s * power_plus(fmaxf(r.m, power_floor(mx, drop)), mx, c, tab, 0.);
+      r.s = r.m == -INFINITY ? r.s : r.s * power_plus(r.m, mx, c, tab, 0.);
       r.m = mx;
       top = mx;
-      floor = power_floor(mx, drop);
     }
     if (bad) r.s = NAN;
     if (r.m > -INFINITY) {
 #pragma unroll
-      for (int k = 0; k < kVfLane; ++k) r.s = power_plus(fmaxf(v[k], floor), top, c, tab, r.s);
+      for (int k = 0; k < kVfLane; ++k) r.s = power_plus(v[k], top, c, tab, r.s);
     }
   }
-  r = row_of_lanes(r, greedy, c, drop, tab);
+  r = row_of_lanes(r, greedy, c, tab);
   if (lane == 0) waves[wave] = r;
   __syncthreads();
   if (wave == 0) {
-    r = row_of_lanes(tid < kVfThreads / 64 ? waves[tid] : RowPart{-INFINITY, -1, 0.}, greedy, c, drop, tab);
+    r = row_of_lanes(tid < kVfThreads / 64 ? waves[tid] : RowPart{-INFINITY, -1, 0.}, greedy, c, tab);
     if (tid == 0) {
       uint64_t* o = a.parts + ((int64_t)row * a.segs + seg) * 2;
       __hip_atomic_store(o, (uint64_t)__float_as_uint(r.m) | ((uint64_t)(uint32_t)r.at << 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -264,7 +263,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     for (int j = 0; j < U; ++j) {
       RowPart one = {-INFINITY, -1, 0.};
       if (lane < a.segs) one = RowPart{__uint_as_float((uint32_t)w[j][0]), (int)(w[j][0] >> 32), __longlong_as_double((long long)w[j][1])};
-      one = row_of_lanes(one, greedy, c, drop, tab);
+      one = row_of_lanes(one, greedy, c, tab);
       const int k = k0 + j;
       if (lane == 0 && k < all) (k <= drafts ? trow[k] : drow[k - drafts - 1]) = one;
     }
@@ -338,15 +337,13 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
   const int s = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, D = a.D;
   const Verdict j = a.verdicts[s];
   const int id = tid < D ? a.ids[(int64_t)s * D + tid] : -1;  // for the answer
-  float drop;
-  const double c = power_unit(temperature(a, s), drop), ulast = a.uniforms[(int64_t)s * (D + 1) + D];
+  const double c = power_unit(temperature(a, s)), ulast = a.uniforms[(int64_t)s * (D + 1) + D];
   fill_powers(tab);
   if (j.token != kVfDraw) return;
   const bool minus = j.di > 0.;
   const XT* const trow = static_cast<const XT*>(a.logits) + s * a.ls + j.n * a.lr;
   const XT* const drow = minus ? static_cast<const XT*>(a.drafted) + s * a.ds + j.n * a.dr : nullptr;
   const double tmax = j.tmax, dmax = j.dmax;
-  const float tfloor = power_floor(j.tmax, drop), dfloor = power_floor(j.dmax, drop);
   struct Chunk {
     Logits<XT, kVfLaneW> t, d;
   };
@@ -357,11 +354,10 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
   auto weights = [&](const Chunk& x, int64_t i0, bool in_order, double* w) __attribute__((always_inline)) {
     const Logits<XT, kVfLaneW>&v = x.t, &q = x.d;
 #pragma unroll
-    for (int k = 0; k < kVfLaneW; ++k) w[k] = v[k] == -INFINITY ? 0. : power_plus(fmaxf(v[k], tfloor), tmax, c, tab, 0.) * j.ti;
+    for (int k = 0; k < kVfLaneW; ++k) w[k] = power_plus<true>(v[k], tmax, c, tab, 0.) * j.ti;
     if (minus) {
 #pragma unroll
-      for (int k = 0; k < kVfLaneW; ++k)
-        w[k] = fmax(q[k] == -INFINITY ? w[k] : w[k] - power_plus(fmaxf(q[k], dfloor), dmax, c, tab, 0.) * j.di, 0.);
+      for (int k = 0; k < kVfLaneW; ++k) w[k] = fmax(w[k] - power_plus<true>(q[k], dmax, c, tab, 0.) * j.di, 0.);
     }
     if (j.without >= i0 && j.without < i0 + kVfChunkW)
 #pragma unroll
