@@ -491,7 +491,7 @@ int miq_paged_attention(const void* q, int x_dtype, const void* cache, int cache
  * [S][D + 1] of V (row i judges draft i, row D follows the last one), draft_logits: the draft's rows [S][D] of the same type, or
  * null for drafts that were not drawn (looked up, or the likeliest): q_i(x_i) = 1. Sequences and rows lie ld_seq, ld_row values
  * apart. drafts int32 [S][D]: a sequence's end at the first id below 0. With p, q the softmaxes of rows over the temperature
- * (temperatures fp32 [S], or null: `temperature`) draft i is accepted while uniforms[s][i] q_i(x_i) < p_i(x_i); behind
+ * (temperatures fp32 [S], or null: `temperature`, not rounded to fp32) draft i is accepted while uniforms[s][i] q_i(x_i) < p_i(x_i); behind
  * n accepted ones a token is drawn from max(p_n - q_n, 0), or from p_n if none was refused: the lowest index whose running sum of
  * weights passes uniforms[s][D] times their total. Temperature 0 (or one that is no finite number above it): a draft is accepted if it is the largest logit's
  * index (the lowest of equal ones; NaN counts as -inf), which is the token too.
@@ -504,7 +504,7 @@ int miq_paged_attention(const void* q, int x_dtype, const void* cache, int cache
 int miq_verify_drafts_workspace(int S, int D, int V, size_t* bytes);
 int miq_verify_drafts(const void* logits, int x_dtype, int64_t ld_seq, int64_t ld_row, const int32_t* drafts,
                       const void* draft_logits, int64_t draft_ld_seq, int64_t draft_ld_row, const float* uniforms,
-                      const float* temperatures, float temperature, int32_t* tokens, int32_t* accepted, int S, int D, int V,
+                      const float* temperatures, double temperature, int32_t* tokens, int32_t* accepted, int S, int D, int V,
                       void* workspace, size_t ws_bytes, void* stream);
 
 /* out[t][i] = silu(gu[t][i]) * gu[t][I + i] for the fused gate|up rows.

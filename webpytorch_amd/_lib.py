@@ -68,7 +68,7 @@ SIGNATURES = {
     "miq_paged_attention_workspace": [_i] * 8 + [_p],
     "miq_paged_attention": [_p, _i, _p, _i, _i, _i, _p, _p, _i, _p] + [_i] * 5 + [_f, _p, _sz, _p],
     "miq_verify_drafts_workspace": [_i, _i, _i, _p],
-    "miq_verify_drafts": [_p, _i, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _f, _p, _p, _i, _i, _i, _p, _sz, _p],
+    "miq_verify_drafts": [_p, _i, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _d, _p, _p, _i, _i, _i, _p, _sz, _p],
     "miq_silu_mul": [_p, _p, _i, _i, _p],
     "miq_add": [_p, _p, _i64, _p],
     "miq_argmax_advance": [_p, _i, _p, _p, _i, _p, _i, _p],

@@ -1337,7 +1337,7 @@ def verify_drafts(logits, drafts, uniforms, draft_logits=None, temperature=1.0):
     (S, D + 1, V), fp32 or fp16: the target's rows, row i judging draft i; `drafts` (S, D) int32, a sequence's end at the first
     id below 0 (D may be 0: a draw alone); `uniforms` (S, D + 1) fp32 in [0, 1); `draft_logits` (S, D, V) of the same dtype,
     the rows the drafts were drawn from, or None for drafts that were not drawn. With p and q the softmaxes over
-    `temperature` (a number, or fp32 (S,); 0: all at the largest logit) draft i is accepted while
+    `temperature` (a number, taken as the float64 it is, or fp32 (S,); 0: all at the largest logit) draft i is accepted while
     uniforms[:, i] q_i(x_i) < p_i(x_i) (q = 1 without draft logits), and behind n accepted ones the token is drawn from max(p_n - q_n, 0),
     or p_n where none was refused: the lowest index whose running sum passes uniforms[:, D] times the total, so that
     tokens are distributed as the target's. Returns DraftVerdict of tokens (S, D + 1) int32 (accepted drafts, the token, then -1) and

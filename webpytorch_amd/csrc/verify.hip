@@ -6,7 +6,7 @@
 //
 // Which side of a border between tokens a draw falls on must not depend on rounding: 150000 borders lie in [0, 1), so that
 // sums right to 1e-7 would give another token once in a hundred draws. Exponentials and sums are fp64 (to 2e-13; a draw is
-// off once in 10^7).
+// off once in 10^7), and a temperature given for all sequences stays the fp64 number that it is: fp32's next to 0.8 gives another token in 5000 draws.
 //
 // Two launches. Every row's maximum and sum of exponentials, in segments (a row's largest logit where the temperature is 0), where the
 // last segment of a sequence to arrive judges its drafts; then a group of workgroups for each sequence sums the weights of its
@@ -34,8 +34,8 @@ __device__ __forceinline__ void fill_powers(double* tab) {
   tab[threadIdx.x] = exp2((double)threadIdx.x / kVfPowers);
   __syncthreads();
 }
-// c of a temperature
-__device__ __forceinline__ double power_unit(float temperature) { return kVfPowers * 1.4426950408889634 / (double)temperature; }
+// c of a temperature: at most 1e300, where the logits nearest to the largest (2^-149 below) are past every border, and 0 c is 0
+__device__ __forceinline__ double power_unit(double temperature) { return fmin(kVfPowers * 1.4426950408889634 / temperature, 1e300); }
 // High word of -899 kVfPowers. Powers are no lower than 2^-899 (-inf among them), which no sum sees. The border is drawn on the exponent: of the
 // fp32 logits, m less 623 temperatures rounds to m itself where the temperature is small. Exponents are 0 or negative, so that
 // their high words, as unsigned numbers, ascend as they descend: the least of two words bounds one, at the cost of an fp32 maximum.
@@ -151,7 +151,7 @@ struct VerifyArgs {
   const int32_t* ids;      // [S][D]
   const float* uniforms;   // [S][D + 1]
   const float* temps;      // [S] or null
-  float temp;
+  double temp;
   int32_t* tokens;         // [S][D + 1]
   int32_t* accepted;       // [S]
   int S, D, V, segs, groups, rounds;  // segments of a row, workgroups of a sequence, chunks a sum of weights
@@ -161,9 +161,9 @@ struct VerifyArgs {
   int* counters;           // [S][kVfCtrStride]: parts of rows, groups of weights
 };
 // 0 for what is no finite number above 0
-__device__ __forceinline__ float temperature(const VerifyArgs& a, int s) {
-  const float t = a.temps ? a.temps[s] : a.temp;
-  return t > 0.f && t < INFINITY ? t : 0.f;
+__device__ __forceinline__ double temperature(const VerifyArgs& a, int s) {
+  const double t = a.temps ? (double)a.temps[s] : a.temp;
+  return t > 0. && t < INFINITY ? t : 0.;
 }
 // by a wave, whose lane i has draft i: one store (with the marks by ballots, where LDS atomics and one thread in a loop were, the draw behind 4 drafts
 // 12.6 -> 7.8 us)
@@ -183,8 +183,8 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
   const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rows = a.S * (a.D + 1), D = a.D;
   const bool target = row < rows;
   const int s = target ? row / (D + 1) : (row - rows) / D, i = target ? row % (D + 1) : (row - rows) % D;
-  const float temp = temperature(a, s);
-  const bool greedy = !(temp > 0.f), dist = a.drafted && !greedy;
+  const double temp = temperature(a, s);
+  const bool greedy = !(temp > 0.), dist = a.drafted && !greedy;
   if (!target && greedy) return;
   const XT* const tl = static_cast<const XT*>(a.logits) + s * a.ls;
   const XT* const dl = static_cast<const XT*>(a.drafted) + s * a.ds;
@@ -519,14 +519,14 @@ extern "C" int miq_verify_drafts_workspace(int S, int D, int V, size_t* bytes) {
 
 extern "C" int miq_verify_drafts(const void* logits, int x_dtype, int64_t ld_seq, int64_t ld_row, const int32_t* drafts,
                                  const void* draft_logits, int64_t draft_ld_seq, int64_t draft_ld_row, const float* uniforms,
-                                 const float* temperatures, float temperature, int32_t* tokens, int32_t* accepted, int S, int D, int V,
+                                 const float* temperatures, double temperature, int32_t* tokens, int32_t* accepted, int S, int D, int V,
                                  void* workspace, size_t ws_bytes, void* stream) {
   if (int rc = check_verify("verify_drafts", S, D, V)) return rc;
   const bool dist = draft_logits && D > 0;
   MIQ_REQUIRE(x_dtype == MIQ_F32 || x_dtype == MIQ_F16, MIQ_ERR_UNSUPPORTED, "verify_drafts: logits dtype %d", x_dtype);
   MIQ_REQUIRE(ld_row >= V && ld_seq >= 0 && (!dist || (draft_ld_row >= V && draft_ld_seq >= 0)), MIQ_ERR_INVALID,
               "verify_drafts: rows %lld and %lld apart hold V=%d values", (long long)ld_row, (long long)draft_ld_row, V);
-  MIQ_REQUIRE(temperatures || (temperature >= 0.f && temperature <= 3.4e38f), MIQ_ERR_INVALID, "verify_drafts: temperature=%g", (double)temperature);
+  MIQ_REQUIRE(temperatures || (temperature >= 0. && temperature < INFINITY), MIQ_ERR_INVALID, "verify_drafts: temperature=%g", temperature);
   if (S == 0) return MIQ_OK;
   MIQ_REQUIRE(logits && (drafts || D == 0) && uniforms && tokens && accepted, MIQ_ERR_INVALID, "verify_drafts: null pointer");
   const int size = x_dtype == MIQ_F32 ? 4 : 2;
