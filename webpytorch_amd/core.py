@@ -1121,6 +1121,9 @@ def token_logprobs(logits, ids, top_k=0):
 PAGE_SIZES = (16, 4096)  # least and most positions of a page, a power of two
 MAX_DRAFTS = 32
 Rope = collections.namedtuple("Rope", "cos sin interleaved")
+# what changes the tables of each rope_type; "factor" where it is there at all has to be given
+_ROPE_KEYS = {"default": (), "linear": ("factor",), "dynamic": ("factor",), "yarn": ("factor", "beta_fast", "beta_slow", "attention_factor", "truncate"),
+              "wavelength": ("factor", "low_freq_factor", "high_freq_factor")}
 _FLOATS, _F32, _I32 = (torch.float32, torch.float16), (torch.float32,), (torch.int32,)
 
 
@@ -1135,19 +1138,29 @@ def rope_tables(n, rot, theta=10000.0, scaling=None, interleaved=False):
         beta_slow (1), a linear ramp over i between; cos and sin times attention_factor (0.1 ln factor + 1);
       "wavelength" (also "llama3"): f_i where 2 pi / f_i < original / high_freq_factor (4), f_i / factor where it is above original /
         low_freq_factor (1), and between them the two mixed linearly in original f_i / 2 pi;
-    with "factor" and (but for linear) "original_max_position_embeddings"."""
+    with "factor" and (but for linear) "original_max_position_embeddings". Any other key that is not None is refused: it would mean other
+    tables ("mscale", say, or "truncate": False); "rope_theta" may repeat theta."""
     n, rot = int(n), int(rot)
     if n < 1 or rot < 2 or rot % 2:
         raise ValueError("rope_tables: n=%d rot=%d" % (n, rot))
     i2 = np.arange(0, rot, 2, dtype=np.float64)
-    sc = dict(scaling or {})
+    sc = {k: v for k, v in dict(scaling or {}).items() if v is not None}
     kind = sc.get("rope_type", sc.get("type", "default"))
     factor, mul = float(sc.get("factor", 1.0)), 1.0
     original = float(sc.get("original_max_position_embeddings", 0) or 0)
-    kind = {"llama3": "wavelength", None: "default"}.get(kind, kind)
-    if kind not in ("default", "linear", "dynamic", "yarn", "wavelength"):
+    kind = {"llama3": "wavelength"}.get(kind, kind)
+    if kind not in _ROPE_KEYS:
         raise NotImplementedError("rope_type %r (linear, dynamic, yarn or wavelength)" % (kind,))
-    if not factor > 0 or not theta > 0 or (kind in ("dynamic", "yarn", "wavelength") and not original > 0) or (kind == "yarn" and theta <= 1):
+    other = sorted(set(sc) - set(_ROPE_KEYS[kind]) - {"rope_type", "type", "rope_theta", "original_max_position_embeddings"})
+    if not sc.get("truncate", True):
+        other.append("truncate: False")
+    if other:
+        raise NotImplementedError("rope_type %r does not know %s" % (kind, ", ".join(other)))
+    if "factor" in _ROPE_KEYS[kind] and "factor" not in sc:
+        raise ValueError("rope_type %r needs a factor" % (kind,))
+    if float(sc.get("rope_theta", theta)) != theta:
+        raise ValueError("rope_tables: theta=%g, rope_theta=%g" % (theta, float(sc["rope_theta"])))
+    if not 0 < factor < math.inf or not theta > 0 or (kind in ("dynamic", "yarn", "wavelength") and not original > 0) or (kind == "yarn" and theta <= 1):
         raise ValueError("rope_tables: theta=%g factor=%g original_max_position_embeddings=%g" % (theta, factor, original))
     if kind == "dynamic" and n > original and rot > 2:
         theta = theta * (factor * n / original - factor + 1.0) ** (rot / (rot - 2.0))
