@@ -26,6 +26,7 @@ File formats are kept exactly (they are formats); the code is this package's own
 import json
 import os
 import struct
+import warnings
 
 import numpy as np
 
@@ -162,7 +163,18 @@ def is_quantized_dir(path):
     return bool(full.get("quantization_config") or _text_config(full).get("quantization_config"))
 
 
+def _warn_positions(what):
+    """The decoder rotates whole heads by plain angles (as the reference does, `webtorch/llm.py:1270-1304`): a model that asks for
+    others runs, but says so."""
+    warnings.warn("%s is not applied: positions are rotated by the plain angles of rope_theta over whole heads" % what, stacklevel=4)
+
+
 def _shape_config(cfg, gs, bits):
+    scaling = cfg.get("rope_scaling") or {}
+    if scaling.get("rope_type", scaling.get("type", "default")) not in (None, "default", "mrope"):  # mrope: plain where all is text
+        _warn_positions("rope_scaling %r" % (scaling,))
+    if float(cfg.get("partial_rotary_factor") or 1.0) != 1.0:
+        _warn_positions("partial_rotary_factor %r" % (cfg["partial_rotary_factor"],))
     H, NH = int(cfg["hidden_size"]), int(cfg["num_attention_heads"])
     out = dict(L=int(cfg["num_hidden_layers"]), H=H, NH=NH, NKV=int(cfg.get("num_key_value_heads", NH)),
                HD=int(cfg.get("head_dim") or H // NH), I=int(cfg["intermediate_size"]),
@@ -546,6 +558,19 @@ def _gguf_experts(g, name, bits, gs, weights):
             for e in range(E)]
 
 
+def warn_gguf_positions(g, prefix):
+    """Says which scaling of the rotation a GGUF file asks for, if any."""
+    kind = g.meta.get(prefix + "rope.scaling.type")
+    said = [] if kind in (None, "none") else ["rope.scaling.type %r" % kind]
+    if kind is None:  # older files: a factor alone
+        factors = {k: float(g.meta.get(prefix + k) or 1.0) for k in ("rope.scaling.factor", "rope.scale_linear")}
+        said += ["%s %g" % kv for kv in factors.items() if kv[1] != 1.0]
+    if "rope_freqs.weight" in g.infos:
+        said.append("rope_freqs.weight")
+    if said:
+        _warn_positions(", ".join(said))
+
+
 def gguf_weights(path, bits=None, weights="native", gs=128):
     """Engine weights of a llama.cpp GGUF decoder (`CausalLM.from_gguf`, `webtorch/llm.py:
     856-1129`): shape, RoPE and norm settings from the file's `{arch}.*` metadata, QK-norm and
@@ -586,6 +611,7 @@ def gguf_weights(path, bits=None, weights="native", gs=128):
     HD = int(m("attention.key_length", 0, required=False) or H // NH)
     if int(m("rope.dimension_count", 0, required=False) or HD) != HD:
         raise NotImplementedError("partial RoPE (rope.dimension_count < head dim) is not part of this engine")
+    warn_gguf_positions(g, A)
     if m("full_attention_interval", 0, required=False) or m("attention.recurrent_layers", None, required=False) \
             or any(n.startswith("blk.0.ssm_") for n in g.infos):
         raise NotImplementedError("recurrent / state-space blocks are not part of this engine")
