@@ -276,6 +276,10 @@ extern "C" int miq_rope(const void* x, int x_dtype, int64_t ld, int64_t lh, cons
   const int64_t nx = span[0], no = span[1];
   const bool same = out == x && (T == 1 || out_ld == ld) && (H == 1 || out_lh == lh);
   MIQ_REQUIRE(same || !share_bytes(out, (size_t)no, x, (size_t)nx), MIQ_ERR_INVALID, "rope: out must be x itself or lie apart from it");
+  const size_t table = (size_t)rows * (rot / 2) * 4;
+  MIQ_REQUIRE(!share_bytes(out, (size_t)no, positions, (size_t)T * 4) && !share_bytes(out, (size_t)no, cos_tab, table) &&
+                  !share_bytes(out, (size_t)no, sin_tab, table),
+              MIQ_ERR_INVALID, "rope: out must lie apart from the positions and the tables");
   const int U = rope_many(T, H) ? kRopeHeads : 1;
   const int64_t threads = (int64_t)T * ((H + U - 1) / U) * ((HD + 7) / 8);
   MIQ_REQUIRE(threads < (1ll << 32) - kRopeThreads, MIQ_ERR_UNSUPPORTED, "rope: T=%d is past the grid", T);
