@@ -17,6 +17,7 @@
 #include <math.h>
 
 #include "attention_parts.h"
+#include "kv4.h"
 
 namespace miq {
 
@@ -536,6 +537,16 @@ extern "C" int miq_verify_drafts(const void* logits, int x_dtype, int64_t ld_seq
   MIQ_REQUIRE(workspace && ws_bytes >= need, MIQ_ERR_INVALID, "verify_drafts: workspace of %zu bytes, %zu needed", workspace ? ws_bytes : (size_t)0,
               need);
   MIQ_REQUIRE(aligned(workspace, 256), MIQ_ERR_ALIGN, "verify_drafts: the workspace must be 256-byte aligned");
+  // the answers are written while other sequences are read
+  const auto span = [&](int64_t ls, int64_t lr, int rows) { return (((__int128)(S - 1) * ls + (__int128)(rows - 1) * (rows > 1 ? lr : 0) + V) * size); };
+  const __int128 nx = span(S > 1 ? ld_seq : 0, ld_row, D + 1), nd = dist ? span(S > 1 ? draft_ld_seq : 0, draft_ld_row, D) : 0, most = (__int128)1 << 48;
+  MIQ_REQUIRE(nx < most && nd < most, MIQ_ERR_INVALID, "verify_drafts: sequences %lld and %lld, rows %lld and %lld apart pass the address space",
+              (long long)ld_seq, (long long)draft_ld_seq, (long long)ld_row, (long long)draft_ld_row);
+  const size_t na = (size_t)S * 4, nt = na * (D + 1);
+  const auto apart = [&](const void* p, size_t n) { return !p || n == 0 || (!share_bytes(tokens, nt, p, n) && !share_bytes(accepted, na, p, n)); };
+  MIQ_REQUIRE(apart(logits, (size_t)nx) && apart(dist ? draft_logits : nullptr, (size_t)nd) && apart(drafts, na * D) && apart(uniforms, nt) &&
+                  apart(temperatures, na) && apart(workspace, need) && !share_bytes(tokens, nt, accepted, na),
+              MIQ_ERR_INVALID, "verify_drafts: tokens and accepted must lie apart from each other, the inputs and the workspace");
   VerifyArgs a;
   a.logits = logits;
   a.drafted = dist ? draft_logits : nullptr;
