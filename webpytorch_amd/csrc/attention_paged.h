@@ -197,7 +197,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attention_kernel(
     int id[NT];  // -1: no keys
   };
   miq_u32x4 kr[NT][NJ];
-  uint32_t vr[NT][4][NV];
+  alignas(16) uint32_t vr[NT][4][NV];  // stored to as vectors of 4 words, or 2
   auto tile_at = [&](int blk, int a, int id) __attribute__((always_inline)) {
     return mine + 2 * plane * (int64_t)max(id, 0) + (int64_t)((blk * KB + 16 * a) & ((1 << pshift) - 1)) * HD;
   };
