@@ -496,9 +496,9 @@ int miq_paged_attention(const void* q, int x_dtype, const void* cache, int cache
  * weights passes uniforms[s][D] times their total. Temperature 0 (or one that is no finite number above it): a draft is accepted if it is the largest logit's
  * index (the lowest of equal ones; NaN counts as -inf), which is the token too.
  * tokens int32 [S][D + 1]: the accepted drafts, the token, then -1; accepted int32 [S]: n. Logits of -inf are tokens of
- * probability 0, as are in the draw those below 2^-899 of the likeliest's. A target row without a distribution (NaN, +inf at a temperature above 0, nothing above -inf) accepts nothing and
- * its token is -1; without one a draft's row is refused and p drawn from; so is a draft from V on. Where max(p - q, 0) has no weight
- * the token is the draft. fp64 exponentials and sums (2e-13). D <= 32, S (2 D + 1) <= 65535. tokens and accepted may not
+ * probability 0, as are in the draw those below 2^-899 of the likeliest's. A target row without a distribution (NaN, +inf at a
+ * temperature above 0, nothing above -inf) accepts nothing and its token is -1; where a draft's row is without one, its draft is refused and the
+ * token drawn from p. A draft from V on is refused as others are. Where max(p - q, 0) has no weight the token is the draft. fp64 exponentials and sums (2e-13). D <= 32, S (2 D + 1) <= 65535. tokens and accepted may not
  * overlap each other or what the call reads (refused). workspace as for miq_paged_attention (always needed).
  * Replaces: the host's draw from logits read back, one token a pass (`_pick`: webtorch/llm.py:1309-1336). */
 int miq_verify_drafts_workspace(int S, int D, int V, size_t* bytes);

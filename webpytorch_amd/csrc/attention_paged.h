@@ -14,12 +14,14 @@
 //
 // The work is split by the lengths, which are the device's: every workgroup adds them up and takes its part of a sequence, the
 // parts as long as give the chip the workgroups that it holds, so that long sequences beside short ones fill it too. The last
-// part of a sequence and head to arrive adds the parts, in their order.
+// part of a sequence and head to arrive adds the parts, in their order. Calls that are not split look for their sequence in the same way.
 //
 // Bound and measured (us a replay over three states; a large copy moves 5.1 TB/s): memory for long caches, 64 sequences of 50 to 8000 positions,
 // 32 / 8 heads of 128, fp16 199 (1.06 GB), one token behind 131000 positions 111 (537 MB); the chain of positions, pages, blocks and joins, and
 // code fetched cold, for short ones, one token behind 700 positions of 14 / 2 heads of 64 9.0, behind 120 of 32 / 8 of 128 7.6; the fp32 matrix cores
 // where an fp32 cache meets several tiles, 16 sequences of up to 5000, 5 tokens of 28 / 4 heads 70 (174 MB, a block of 16 keys and 48 rows 2.6 us a wave).
+// Scratch, which the largest forms spill to (bytes a lane): heads of 128, three tiles, 8 waves, fp32 cache 148 (39 registers), fp16 24; heads of 192,
+// one tile, 8 waves, fp32 84; heads of 256, two tiles, fp32 216 (96 registers), fp16 80 to 96.
 #pragma once
 #include <math.h>
 

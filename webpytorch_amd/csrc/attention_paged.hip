@@ -15,10 +15,14 @@ struct PagedPlan {
   int nr, nw, tiles, target, fit;
   int64_t grid, units;
 };
-// Workgroups of 8 waves, one a CU (two waves a SIMD fill the registers). From kPaMany sequences x heads x tiles on, of 4 waves, two
-// of them a CU, so that one starts while the other ends (256 sequences of 10 to 500 positions 98 -> 74 us; 64 of up to 8000 196 -> 200);
-// of 4 and one a CU where the sums take most of the registers (heads of 256, wide heads of several tiles).
-// The parts: where sequences, heads and tiles are at most half of what the chip holds, no more parts than it holds (320 parts on 256 CUs took
+// Workgroups of 8 waves, one a CU (two waves a SIMD fill the registers). From kPaMany sequences x heads x tiles on, of 4 waves, so that one
+// workgroup starts while another ends (fp16 cache, one token, 256 sequences of 10 to 500 positions 98 -> 74 us; 64 of up to 8000 196 -> 200);
+// of 4 also where the sums take most of the registers (heads of 256, wide heads of several tiles).
+// A CU holds two or three workgroups of 4 waves at heads of 64 with one or two tiles and at heads of 128 with one tile of an fp16 cache. The other
+// kernels take accumulation registers beside the vector ones in this form and keep one wave a SIMD; their 8-wave form, where they have one, keeps two. From kPaMany on
+// both forms of those are not compared; as they run: 64 sequences of 50 to 8000, 32 / 8 heads of 128, fp32 cache 405 us (2.1 GB, 5.2 TB/s: memory), fp16
+// cache and 5 tokens 242 (1.07 GB, 4.4 TB/s).
+// The parts: where sequences, heads and tiles are at most half of the CUs, no more parts than there are CUs (320 parts on 256 CUs took
 // twice the time of 256: 16 sequences of 300 to 5000, 5 tokens, fp32 90 -> 75 us); otherwise kPaParts of them, which ends evenly
 // (64 sequences of up to 8000, us at 256 / 512 / 1024 / 2048 parts: 223 / 212 / 200 / 196, but 256 short ones 74 / 74 / 74 / 82).
 constexpr int kPaMany = 512, kPaParts = 1024;
@@ -30,11 +34,10 @@ static PagedPlan pa_plan(int S, int T, int NH, int NKV, int HD, int64_t cap, boo
   p.units = (int64_t)NKV * p.tiles;
   const bool wide = HD == 256 || (HD == 192 && p.nr == 2);
   p.nw = wide || S * p.units >= kPaMany ? 4 : 8;
-  const int hold = wide || p.nw == 8 ? kCUs : 2 * kCUs;
   const int64_t step = (c16 ? 32 : 16) * p.nw, most = cap <= kPaWhole * step ? 1 : (cap + kPaMinSteps * step - 1) / (kPaMinSteps * step);
   const bool split = S * p.units <= kPaMaxSplit && most > 1;  // most: parts of a full sequence
-  p.fit = split && S <= 64 && S * p.units * 2 <= hold;
-  p.target = !split ? 0 : p.fit ? hold : kPaParts;
+  p.fit = split && S <= 64 && S * p.units * 2 <= kCUs;
+  p.target = !split ? 0 : p.fit ? kCUs : kPaParts;
   p.grid = S * p.units;
   if (split) p.grid = p.grid * most < p.grid + p.target ? p.grid * most : p.grid + p.target;
   return p;

@@ -12,7 +12,7 @@
 // last segment of a sequence to arrive judges its drafts; then a group of workgroups for each sequence sums the weights of its
 // chunks, and the last of them to arrive finds the chunk, the thread and the index.
 //
-// Bound and measured (us a replay): 64 sequences of 4 drafts, V 128256, fp32 95: the rows 65 (295 MB, 4.5 TB/s) and the draw 27 (66 MB of them
+// Bound and measured (us a replay): 64 sequences of 4 drafts, V 128256, fp32 93: the rows 65 (295 MB, 4.5 TB/s) and the draw 26 (66 MB of them
 // again, fp64 issue); one sequence, V 151936, 21: the chain logits, part, counter, judgement and then weights, sum, counter, chunk.
 #include <math.h>
 
@@ -43,7 +43,7 @@ __device__ __forceinline__ double power_unit(double temperature) { return fmin(k
 constexpr uint32_t kVfDeepest = 0xC10C1800u;
 // 2^((x - m) c / 256), x <= m, added to `sum`, 1 for m itself: whole multiples of 1 / 256 by the table and the exponent, the rest, |f| <= 1 / 512, by the
 // series of e^(f ln 2) to the third power (1.4e-13). 10 fp64 operations (a table of 32 takes 12, the series of |f| <= 1 / 2 alone 19),
-// which with the loads' latency bound the kernel of the rows (64 sequences of 4 drafts, V 128256: fp16 61 us, fp32 64, where its bytes take 58).
+// which with the loads' latency bound the kernel of the rows (64 sequences of 4 drafts, V 128256: fp16 61 us, fp32 65, where its bytes take 58).
 // ZERO: nothing for what is as low as the border, so that no draw falls on it.
 template <bool ZERO = false> __device__ __forceinline__ double power_plus(float x, double m, double c, const double* tab, double sum) {
   const double far = ((double)x - m) * c, magic = 6755399441055744.;  // 1.5 2^52: the whole part in the low word
