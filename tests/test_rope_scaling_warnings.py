@@ -29,7 +29,7 @@ def test_a_configuration_that_is_not_followed(tmp_path, key, value):
     assert len(said) == 1 and key in said[0]
 
 
-@pytest.mark.parametrize("more", [{"rope_scaling": None}, {"rope_scaling": {"type": "default"}}, {"partial_rotary_factor": 1.0},
+@pytest.mark.parametrize("more", [{"rope_scaling": None}, {"rope_scaling": "none"}, {"rope_scaling": {"type": "default"}}, {"partial_rotary_factor": 1.0},
                                   {"rope_scaling": {"rope_type": "default", "mrope_section": [16, 24, 24], "type": "mrope"}}])
 def test_plain_positions(tmp_path, more):
     assert load(tmp_path, **more)[1] == []

@@ -170,7 +170,8 @@ def _warn_positions(what):
 
 
 def _shape_config(cfg, gs, bits):
-    scaling = cfg.get("rope_scaling") or {}
+    scaling = cfg.get("rope_scaling")
+    scaling = scaling if isinstance(scaling, dict) else {}
     if scaling.get("rope_type", scaling.get("type", "default")) not in (None, "default", "mrope"):  # mrope: plain where all is text
         _warn_positions("rope_scaling %r" % (scaling,))
     if float(cfg.get("partial_rotary_factor") or 1.0) != 1.0:
